@@ -6,30 +6,12 @@
 #include <new>
 #include <vector>
 
+#include "entry.h"
 #include "internal.h"
 
 using namespace t2sc;
 
 namespace {
-
-// Makes the context's device current for the duration of a call and
-// restores the caller's device afterwards.
-struct DeviceGuard {
-  int prev = -1;
-  explicit DeviceGuard(int dev) {
-    if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
-    if (prev != dev) cudaSetDevice(dev);
-  }
-  ~DeviceGuard() {
-    int cur = -1;
-    if (prev >= 0 && cudaGetDevice(&cur) == cudaSuccess && cur != prev) cudaSetDevice(prev);
-  }
-};
-
-int fail(t2sc_ctx *ctx, int code, const std::string &msg) {
-  if (ctx) ctx->last_error = msg;
-  return code;
-}
 
 size_t elem_size(int dtype) { return dtype == T2SC_DT_F32 ? 4 : 2; }
 
@@ -49,24 +31,6 @@ struct DevBuf {
     return T2SC_OK;
   }
 };
-
-#define T2SC_TRY(expr)                   \
-  do {                                   \
-    int _rc = (expr);                    \
-    if (_rc != T2SC_OK) return _rc;      \
-  } while (0)
-
-// Runs an entry point's body; C++ exceptions never cross the C ABI.
-template <class F>
-int guarded(t2sc_ctx *ctx, F &&body) {
-  try {
-    return body();
-  } catch (const std::bad_alloc &) {
-    return fail(ctx, T2SC_ERR_OOM, "host allocation failed");
-  } catch (...) {
-    return fail(ctx, T2SC_ERR_INVALID, "unexpected exception");
-  }
-}
 
 int check_sync(t2sc_ctx *ctx) {
   std::string &err = ctx->last_error;
