@@ -49,6 +49,8 @@ extern "C" {
 /* ---- epilogue flags, applied in this order after the bias ---- */
 #define T2SC_SILU 1     /* y = y / (1 + exp(-y)) */
 #define T2SC_RESIDUAL 2 /* y += residual (same dtype and shape as y) */
+#define T2SC_GELU 4     /* y = 0.5 y (1 + tanh(sqrt(2/pi) (y + 0.044715 y^3))), t2sc_dense_linear_device only,
+                           in the place of T2SC_SILU */
 
 /* ---- subdivision ---- */
 #define T2SC_SUB_NONZERO 0  /* keep child c of row r iff sub[r*8+c] != 0 (forward_subdivision) */
@@ -259,6 +261,79 @@ int t2sc_c2s_block_destroy(t2sc_c2s_block *block);
  * children with the conv2 map already built, owned by the caller. */
 int t2sc_c2s_block_forward_device(t2sc_c2s_block *block, t2sc_coords *coords, const void *x, float *subdiv,
                                   int32_t *out_coords, void *out_feats, int64_t *m, t2sc_coords **out_child);
+
+/* ---- the attention block over voxel tokens ----
+ * The reference's transformer blocks run over the same [N, C] rows and
+ * [N, 4] coordinates as its decoder: packed or separate projections, an RMS
+ * norm of every head of q and k, rotary positions over the voxel axes,
+ * attention inside each shape of the batch, the output and feed-forward
+ * products (trellis2_mojo/modules/attention.mojo, modules/rope.mojo,
+ * sparse/attention, gpu/attention.mojo, gpu/block.mojo).
+ * Rows of every buffer may be strided: row r of x starts at x + r * x_stride
+ * elements, so q, k and v can be slices of one packed [N, 3, heads,
+ * head_dim] projection. A stride of a buffer of more than one row is at
+ * least the row's width and at most 2^28. All calls are asynchronous on the
+ * context's stream and capturable in a CUDA graph. */
+
+/* y [rows, co] = act(x [rows, ci] @ w [co, ci]^T + bias) + residual, all of
+ * dtype (bias: device f32 [co] or NULL), with sums, activation and residual
+ * in f32 and one rounding. flags: T2SC_SILU or T2SC_GELU, T2SC_RESIDUAL
+ * (with residual [rows, co]). Unlike t2sc_linear_forward_device it takes the
+ * weight as it lies on the device and keeps nothing. y may be residual
+ * itself (same address and stride); any other overlap with an input is
+ * refused. 16-bit rows that start on 16 bytes (addresses, strides and ci
+ * multiples of 8 elements) run on the tensor cores, f32 and other 16-bit
+ * rows on the CUDA cores. */
+int t2sc_dense_linear_device(t2sc_ctx *ctx, const void *x, int64_t x_stride, const void *w, int64_t w_stride,
+                             const float *bias, const void *residual, int64_t residual_stride, void *y,
+                             int64_t y_stride, int64_t rows, int co, int ci, int flags, int dtype);
+
+/* Rotary positions with three axes: pair j of axis a (a = 0, 1, 2 for
+ * columns x, y, z of the coordinates) turns by coords[row, 1 + a] *
+ * theta^(-j / pairs_a) radians. Pairs are taken by the axes in order; the
+ * head's remaining pairs do not turn. layout: pair p is channels 2p and
+ * 2p + 1 (PAIRS) or p and p + head_dim / 2 (HALVES). Angles are formed in 64
+ * bits: every int32 position is exact to f32. head_dim even, 2..256. */
+#define T2SC_ROPE_PAIRS 0
+#define T2SC_ROPE_HALVES 1
+typedef struct t2sc_rope t2sc_rope;
+int t2sc_rope_create(t2sc_ctx *ctx, int head_dim, int pairs_x, int pairs_y, int pairs_z, double theta, int layout,
+                     t2sc_rope **out);
+int t2sc_rope_destroy(t2sc_rope *rope);
+/* x, y: device [rows, heads, head_dim] of dtype; coords: device int32
+ * [rows, 4]. y may be x itself (same address and stride). */
+int t2sc_rope_apply_device(t2sc_rope *rope, const int32_t *coords, const void *x, int64_t x_stride, void *y,
+                           int64_t y_stride, int64_t rows, int heads, int dtype);
+/* Every head of q and of k [rows, heads, head_dim]: z = x / sqrt(mean(x^2) +
+ * eps) * gain[head, :], then the rotation (rope NULL: none, coords unused),
+ * in one pass; gains device f32 [heads, head_dim]. k and k_out NULL: q
+ * alone. q_out may be q and k_out k (same address and stride); any other
+ * overlap is refused. eps > 0. */
+int t2sc_qk_norm_rope_device(t2sc_ctx *ctx, t2sc_rope *rope, const int32_t *coords, const void *q, int64_t q_stride,
+                             const void *k, int64_t k_stride, const float *gain_q, const float *gain_k, void *q_out,
+                             int64_t q_out_stride, void *k_out, int64_t k_out_stride, int64_t rows, int heads,
+                             int head_dim, float eps, int dtype);
+
+/* The sequences of a ragged batch: sequence b's queries are rows
+ * [q_offsets[b], q_offsets[b + 1]) and its keys rows [kv_offsets[b],
+ * kv_offsets[b + 1]) (host int64 [batch + 1], not falling; kv_offsets NULL:
+ * the same as q_offsets, self-attention). Built once per set of coordinates
+ * and shared by every layer. */
+typedef struct t2sc_seqs t2sc_seqs;
+int t2sc_seqs_create(t2sc_ctx *ctx, const int64_t *q_offsets, const int64_t *kv_offsets, int64_t batch,
+                     t2sc_seqs **out);
+int t2sc_seqs_destroy(t2sc_seqs *seqs);
+/* out[i, h] = sum_j softmax_j(scale * q[i, h] . k[j, h]) v[j, h] over the
+ * keys j of i's sequence, statistics and sums in f32; a sequence without
+ * keys gives zeros. q, out: device [rows, heads, head_dim] of dtype with
+ * rows >= the last q offset; k, v likewise with the kv offsets. Rows outside
+ * the sequences are neither read for a result nor written. out must not
+ * overlap q, k or v. head_dim 1..256; 16-bit types with head_dim a multiple
+ * of 8 up to 128 and rows that start on 16 bytes run on the tensor cores,
+ * everything else on the CUDA cores. */
+int t2sc_attention_device(t2sc_seqs *seqs, const void *q, int64_t q_stride, const void *k, int64_t k_stride,
+                          const void *v, int64_t v_stride, void *out, int64_t out_stride, int heads, int head_dim,
+                          float scale, int dtype);
 
 /* ---- multi-GPU data plane (no reference counterpart: the reference is
  * single-device, trellis2_mojo/gpu/context.mojo:116-165). One process per

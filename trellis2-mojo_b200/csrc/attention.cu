@@ -1,0 +1,232 @@
+// Softmax attention inside each sequence of a ragged batch:
+//   out[i, h] = sum_j softmax_j(scale * q[i, h] . k[j, h]) v[j, h],
+// j over the keys of i's sequence; a sequence without keys gives zeros.
+//
+// One pass over the keys: with m the running maximum and l the running sum of
+// a row, a block of scores s updates m' = max(m, s), o = o e^(m - m') + sum
+// e^(s - m') v and l likewise; out = o / l. m, l and o are f32.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cmath>
+
+#include "attention.h"
+#include "entry.h"
+
+namespace t2sc {
+namespace {
+
+constexpr int kMaxHeadDim = 256;
+
+template <int DT>
+__device__ __forceinline__ float ld1(const char *p, int64_t i) {
+  if (DT == T2SC_DT_F32) return reinterpret_cast<const float *>(p)[i];
+  if (DT == T2SC_DT_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(p)[i]);
+  return __half2float(reinterpret_cast<const __half *>(p)[i]);
+}
+template <int DT>
+__device__ __forceinline__ void st1(char *p, int64_t i, float v) {
+  if (DT == T2SC_DT_F32)
+    reinterpret_cast<float *>(p)[i] = v;
+  else if (DT == T2SC_DT_BF16)
+    reinterpret_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(v);
+  else
+    reinterpret_cast<__half *>(p)[i] = __float2half_rn(v);
+}
+
+// CUDA-core kernel for every type, head_dim up to 256, stride and alignment:
+// 32 queries of one head a CTA, four threads a query, keys in blocks of 32
+// through shared memory. Products are f32. f32 runs here; the 16-bit types
+// only where the tensor-core kernel's TMA loads do not apply.
+constexpr int kBQ = 32, kBKV = 32, kThreads = 128;
+
+template <int DT>
+__global__ void __launch_bounds__(kThreads) attention_simt_kernel(const AttnArgs a) {
+  extern __shared__ float smem[];
+  const int D = a.head_dim, pitch = D + 1;
+  float *qs = smem, *kv = qs + kBQ * pitch, *ps = kv + kBKV * pitch;  // ps: [kBQ][kBKV + 1]
+  const int tid = threadIdx.x, row = tid >> 2, part = tid & 3;
+  const int head = blockIdx.y;
+  // the CTA's sequence and its block of queries inside it
+  int64_t left = blockIdx.x;
+  int4 seq = make_int4(0, 0, 0, 0);
+  int b = 0;
+  for (; b < a.batch; b++) {
+    seq = __ldg(a.seqs + b);
+    const int64_t blocks = ((int64_t)seq.y + kBQ - 1) / kBQ;
+    if (left < blocks) break;
+    left -= blocks;
+  }
+  if (b == a.batch) return;
+  const int64_t q0 = seq.x + left * kBQ;
+  const int here = (int)min((int64_t)kBQ, seq.x + (int64_t)seq.y - q0);
+  const int64_t at = (int64_t)head * D;
+  for (int i = tid; i < kBQ * D; i += kThreads) {
+    const int r = i / D, c = i % D;
+    qs[r * pitch + c] = r < here ? ld1<DT>(a.q, (q0 + r) * a.ldq + at + c) * a.scale : 0.f;
+  }
+  float m = -INFINITY, l = 0.f;
+  constexpr int P = kMaxHeadDim / 4;
+  float o[P];
+#pragma unroll
+  for (int i = 0; i < P; i++) o[i] = 0.f;
+  for (int64_t k0 = 0; k0 < seq.w; k0 += kBKV) {
+    const int keys = (int)min((int64_t)kBKV, seq.w - k0);
+    __syncthreads();
+    for (int i = tid; i < kBKV * D; i += kThreads) {
+      const int r = i / D, c = i % D;
+      kv[r * pitch + c] = r < keys ? ld1<DT>(a.k, (seq.z + k0 + r) * a.ldk + at + c) : 0.f;
+    }
+    __syncthreads();
+    float s[kBKV / 4], top = m;
+#pragma unroll
+    for (int j = 0; j < kBKV / 4; j++) s[j] = 0.f;
+    for (int c = 0; c < D; c++) {
+      const float qc = qs[row * pitch + c];
+#pragma unroll
+      for (int j = 0; j < kBKV / 4; j++) s[j] += qc * kv[(j * 4 + part) * pitch + c];
+    }
+#pragma unroll
+    for (int j = 0; j < kBKV / 4; j++) {
+      if (j * 4 + part >= keys) s[j] = -INFINITY;
+      top = fmaxf(top, s[j]);
+    }
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const float base = top == -INFINITY ? 0.f : top;  // every score -inf so far: their weights are 0
+    const float keep = expf(m - base);
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < kBKV / 4; j++) {
+      const float p = expf(s[j] - base);
+      ps[row * (kBKV + 1) + j * 4 + part] = p;
+      sum += p;
+    }
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    l = l * keep + sum, m = top;
+    __syncthreads();
+    for (int i = tid; i < kBKV * D; i += kThreads) {
+      const int r = i / D, c = i % D;
+      kv[r * pitch + c] = r < keys ? ld1<DT>(a.v, (seq.z + k0 + r) * a.ldv + at + c) : 0.f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < P; i++) {
+      const int c = i * 4 + part;
+      if (c >= D) break;
+      float t = o[i] * keep;
+      for (int j = 0; j < keys; j++) t += ps[row * (kBKV + 1) + j] * kv[j * pitch + c];
+      o[i] = t;
+    }
+  }
+  if (row >= here) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;  // no key, or every score -inf: zeros
+#pragma unroll
+  for (int i = 0; i < P; i++) {
+    const int c = i * 4 + part;
+    if (c >= D) break;
+    st1<DT>(a.out, (q0 + row) * a.ldo + at + c, o[i] * inv);
+  }
+}
+
+}  // namespace
+
+int attention_simt(t2sc_seqs *s, const AttnArgs &a, int dtype, std::string &err) {
+  t2sc_ctx *ctx = s->ctx;
+  int64_t blocks = 0;
+  for (int64_t b = 0; b < s->batch; b++) blocks += (s->q_off[b + 1] - s->q_off[b] + kBQ - 1) / kBQ;
+  if (blocks == 0) return T2SC_OK;
+  const size_t smem = ((kBQ + kBKV) * (size_t)(a.head_dim + 1) + kBQ * (kBKV + 1)) * sizeof(float);
+  const dim3 grid((unsigned)blocks, (unsigned)a.heads);
+  auto go = [&](auto kernel) -> int {
+    T2SC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "attention");
+    kernel<<<grid, kThreads, smem, ctx->stream>>>(a);
+    T2SC_LAUNCHED(ctx, "attention");
+    return T2SC_OK;
+  };
+  if (dtype == T2SC_DT_F32) return go(attention_simt_kernel<T2SC_DT_F32>);
+  if (dtype == T2SC_DT_BF16) return go(attention_simt_kernel<T2SC_DT_BF16>);
+  return go(attention_simt_kernel<T2SC_DT_F16>);
+}
+
+}  // namespace t2sc
+
+using namespace t2sc;
+
+extern "C" {
+
+int t2sc_seqs_create(t2sc_ctx *ctx, const int64_t *q_offsets, const int64_t *kv_offsets, int64_t batch, t2sc_seqs **out) {
+  if (!ctx || !out) return T2SC_ERR_INVALID;
+  *out = nullptr;
+  if (batch < 0 || batch > (1 << 20)) return fail(ctx, T2SC_ERR_INVALID, "seqs: batch must be in [0, 2^20]");
+  if (!q_offsets) return fail(ctx, T2SC_ERR_INVALID, "seqs: null offsets");
+  if (!kv_offsets) kv_offsets = q_offsets;
+  for (const int64_t *off : {q_offsets, kv_offsets}) {
+    if (off[0] < 0 || off[batch] > INT32_MAX) return fail(ctx, T2SC_ERR_INVALID, "seqs: offsets must be in [0, 2^31)");
+    for (int64_t b = 0; b < batch; b++)
+      if (off[b + 1] < off[b]) return fail(ctx, T2SC_ERR_INVALID, "seqs: offsets must not fall");
+  }
+  return guarded(ctx, [&]() -> int {
+    DeviceGuard g(ctx->device);
+    std::string &err = ctx->last_error;
+    std::unique_ptr<t2sc_seqs, int (*)(t2sc_seqs *)> s(new t2sc_seqs(), t2sc_seqs_destroy);
+    s->ctx = ctx;
+    s->batch = batch;
+    s->q_off.assign(q_offsets, q_offsets + batch + 1);
+    s->kv_off.assign(kv_offsets, kv_offsets + batch + 1);
+    s->q_rows = s->q_off[batch], s->kv_rows = s->kv_off[batch];
+    s->q_total = s->q_off[batch] - s->q_off[0];
+    std::vector<int4> h((size_t)batch + 1);
+    for (int64_t b = 0; b < batch; b++)
+      h[b] = make_int4((int)s->q_off[b], (int)(s->q_off[b + 1] - s->q_off[b]), (int)s->kv_off[b],
+                       (int)(s->kv_off[b + 1] - s->kv_off[b]));
+    T2SC_CUDA(cudaMalloc((void **)&s->d_seqs, h.size() * sizeof(int4)), "seqs");
+    T2SC_CUDA(cudaMemcpy(s->d_seqs, h.data(), h.size() * sizeof(int4), cudaMemcpyHostToDevice), "seqs");
+    *out = s.release();
+    return T2SC_OK;
+  });
+}
+
+int t2sc_seqs_destroy(t2sc_seqs *s) {
+  if (!s) return T2SC_OK;
+  DeviceGuard g(s->ctx->device);
+  if (s->d_seqs) cudaFree(s->d_seqs);
+  delete s;
+  return T2SC_OK;
+}
+
+int t2sc_attention_device(t2sc_seqs *seqs, const void *q, int64_t q_stride, const void *k, int64_t k_stride, const void *v,
+                          int64_t v_stride, void *out, int64_t out_stride, int heads, int head_dim, float scale, int dtype) {
+  if (!seqs) return T2SC_ERR_INVALID;
+  t2sc_ctx *ctx = seqs->ctx;
+  return guarded(ctx, [&]() -> int {
+    if (heads < 1 || heads > 4096) return fail(ctx, T2SC_ERR_INVALID, "attention: heads must be in [1, 4096]");
+    if (head_dim < 1 || head_dim > kMaxHeadDim) return fail(ctx, T2SC_ERR_INVALID, "attention: head_dim must be in [1, 256]");
+    if (!std::isfinite(scale)) return fail(ctx, T2SC_ERR_INVALID, "attention: scale must be finite");
+    if (!dtype_known(dtype)) return fail(ctx, T2SC_ERR_INVALID, "attention: unknown dtype");
+    if (seqs->q_total == 0) return T2SC_OK;
+    const int64_t width = (int64_t)heads * head_dim;
+    const int es = dtype_size(dtype);
+    const bool keys = seqs->kv_off[seqs->batch] > seqs->kv_off[0];
+    if (!q || !out || (keys && (!k || !v))) return fail(ctx, T2SC_ERR_INVALID, "attention: null buffer");
+    // rows [0, last offset) of every buffer
+    const Rows rq{q, q_stride, seqs->q_rows, width, es}, ro{out, out_stride, seqs->q_rows, width, es},
+        rk{k, k_stride, keys ? seqs->kv_rows : 0, width, es}, rv{v, v_stride, keys ? seqs->kv_rows : 0, width, es};
+    for (const Rows *r : {&rq, &rk, &rv, &ro}) {
+      if (!stride_ok(*r)) return fail(ctx, T2SC_ERR_INVALID, "attention: a row stride must be in [heads * head_dim, 2^28]");
+      if (!aligned_to_elem(*r)) return fail(ctx, T2SC_ERR_INVALID, "attention: a buffer is not aligned to its element type");
+    }
+    for (const Rows *r : {&rq, &rk, &rv})
+      if (overlaps(ro, *r)) return fail(ctx, T2SC_ERR_INVALID, "attention: out overlaps q, k or v");
+    AttnArgs a;
+    a.q = static_cast<const char *>(q), a.k = static_cast<const char *>(k), a.v = static_cast<const char *>(v);
+    a.out = static_cast<char *>(out);
+    a.ldq = q_stride, a.ldk = k_stride, a.ldv = v_stride, a.ldo = out_stride;
+    a.seqs = seqs->d_seqs, a.batch = (int)seqs->batch, a.heads = heads, a.head_dim = head_dim, a.scale = scale;
+    DeviceGuard g(ctx->device);
+    return attention_simt(seqs, a, dtype, ctx->last_error);
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,32 @@
+// A ragged batch's sequences and the launch arguments of the attention kernels.
+#pragma once
+#include <stdint.h>
+
+#include <string>
+#include <vector>
+
+#include "internal.h"
+
+struct t2sc_seqs {
+  t2sc_ctx *ctx = nullptr;
+  int64_t batch = 0;
+  std::vector<int64_t> q_off, kv_off;  // [batch + 1]
+  int64_t q_rows = 0, kv_rows = 0;     // rows up to the last offset
+  int64_t q_total = 0;                 // query rows inside sequences
+  int4 *d_seqs = nullptr;              // [batch] first query row, query rows, first key row, key rows
+};
+
+namespace t2sc {
+
+struct AttnArgs {
+  const char *q = nullptr, *k = nullptr, *v = nullptr;
+  char *out = nullptr;
+  int64_t ldq = 0, ldk = 0, ldv = 0, ldo = 0;  // elements between rows
+  const int4 *seqs = nullptr;
+  int batch = 0, heads = 0, head_dim = 0;
+  float scale = 0.f;
+};
+
+int attention_simt(t2sc_seqs *s, const AttnArgs &a, int dtype, std::string &err);
+
+}  // namespace t2sc

@@ -1,0 +1,39 @@
+// Launch arguments and epilogue arithmetic of the dense linear kernels.
+#pragma once
+#include <stdint.h>
+
+#include <string>
+
+#include "../../include/t2sc.h"
+#include "epilogue.cuh"
+
+struct t2sc_ctx;
+
+namespace t2sc {
+
+struct DenseArgs {
+  const char *x = nullptr, *w = nullptr, *res = nullptr;
+  const float *bias = nullptr;
+  char *y = nullptr;
+  int64_t ldx = 0, ldw = 0, ldr = 0, ldy = 0;  // elements
+  int64_t rows = 0;
+  int co = 0, ci = 0, act = 0;
+};
+
+// 0.5 v (1 + tanh(u)) = v / (1 + e^(-2u)), u = sqrt(2/pi) (v + 0.044715 v^3):
+// one exponential, and no cancellation in the negative tail. The exponent is
+// clamped as in silu().
+__device__ __forceinline__ float gelu_tanh(float v) {
+  const float u2 = v * (1.5957691216057308f + 0.07135481627f * v * v);
+  return __fdividef(v, 1.0f + __expf(fminf(-u2, 80.0f)));
+}
+
+__device__ __forceinline__ float activate(float v, int act) {
+  if (act & T2SC_SILU) return silu(v);
+  if (act & T2SC_GELU) return gelu_tanh(v);
+  return v;
+}
+
+int dense_simt(t2sc_ctx *ctx, const DenseArgs &a, int dtype, std::string &err);
+
+}  // namespace t2sc

@@ -1,0 +1,441 @@
+// Rotary positions over the voxel axes, alone or behind an RMS norm of every
+// head: z = x / sqrt(mean(x^2) + eps) * gain, then every pair (u, v) of a
+// head turns by its angle, (u cos - v sin, u sin + v cos).
+//
+// Pair j of axis a turns by coords[row, 1 + a] * theta^(-j / n_a). The angle
+// is formed in turns (2 pi = 1) and in 64 bits and reduced to half a turn
+// before it is rounded: a 32-bit angle of a position of 10^3 would already be
+// off by 3e-5, and any int32 position is allowed here.
+//
+// The operators move their rows once in and once out and do ~10 operations a
+// value, so HBM bounds them if enough bytes are in flight. A CTA takes T
+// rows; a group of g lanes (a power of two) owns one head, every lane the
+// two 16-byte chunks at the same place of the head's two halves, which holds
+// whole pairs in either layout. All loads of up to R heads a group are issued
+// before the CTA's T x pairs sines and cosines are computed into shared
+// memory, so that their latency hides behind them, and one angle serves all
+// heads of q and k.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cmath>
+#include <vector>
+
+#include "entry.h"
+#include "internal.h"
+
+struct t2sc_rope {
+  t2sc_ctx *ctx = nullptr;
+  int head_dim = 0, layout = 0, rotated = 0;  // rotated: pairs that turn; the others stay
+  double *d_turns = nullptr;                  // [rotated] turns per unit of position
+  int n_axis[3] = {0, 0, 0};
+};
+
+namespace t2sc {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxHeadDim = 256;
+
+struct RopeArgs {
+  const int32_t *coords = nullptr;   // [rows, 4]
+  const double *turns = nullptr;     // [rotated]
+  int n0 = 0, n01 = 0, rotated = 0;  // pairs of axis 0, of axes 0 and 1, of all
+  const char *in[2] = {nullptr, nullptr};
+  char *out[2] = {nullptr, nullptr};
+  int64_t in_stride[2] = {0, 0}, out_stride[2] = {0, 0};  // bytes
+  const float *gain[2] = {nullptr, nullptr};              // [heads, head_dim]
+  int64_t rows = 0;
+  int heads = 0, head_dim = 0, per_row = 0;  // per_row: heads of one row, of q and k together
+  float eps = 0.f, inv_dim = 0.f;
+};
+
+// cos and sin of pair p at the coordinates of one row.
+__device__ __forceinline__ float2 turn_of(const RopeArgs &a, int64_t row, int p) {
+  const int axis = p < a.n0 ? 0 : (p < a.n01 ? 1 : 2);
+  double t = (double)__ldg(a.coords + row * 4 + 1 + axis) * __ldg(a.turns + p);
+  t -= rint(t);
+  float s, c;
+  sincospif((float)(2.0 * t), &s, &c);
+  return make_float2(c, s);
+}
+
+template <int DT>
+struct Chunk {  // 16 bytes
+  static constexpr int kElems = DT == T2SC_DT_F32 ? 4 : 8;
+  __device__ __forceinline__ static void unpack(const uint4 &u, float *f) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      if (DT == T2SC_DT_F32) {
+        f[j] = __uint_as_float(w[j]);
+      } else if (DT == T2SC_DT_BF16) {
+        f[2 * j] = __uint_as_float(w[j] << 16), f[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+      } else {
+        const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&w[j]));
+        f[2 * j] = h.x, f[2 * j + 1] = h.y;
+      }
+    }
+  }
+  __device__ __forceinline__ static uint4 pack(const float *f) {
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      if (DT == T2SC_DT_F32) {
+        w[j] = __float_as_uint(f[j]);
+      } else if (DT == T2SC_DT_BF16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * j], f[2 * j + 1]);
+        w[j] = *reinterpret_cast<const uint32_t *>(&h);
+      } else {
+        const __half2 h = __floats2half2_rn(f[2 * j], f[2 * j + 1]);
+        w[j] = *reinterpret_cast<const uint32_t *>(&h);
+      }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+
+// NORM: RMS norm and gains first. PAIRS: adjacent channels are a pair, else
+// channels j and j + head_dim / 2. R: heads a group holds at once.
+template <int DT, bool NORM, bool PAIRS, int R>
+__global__ void __launch_bounds__(kThreads) rope_vec_kernel(const RopeArgs a, int t_rows, int lanes, int chunks) {
+  constexpr int E = Chunk<DT>::kElems;
+  extern __shared__ float2 turn[];  // [t_rows][rotated]
+  const int groups = kThreads / lanes, gid = (int)threadIdx.x / lanes, sub = (int)threadIdx.x % lanes;
+  const int64_t row0 = (int64_t)blockIdx.x * t_rows;
+  const int here = (int)min((int64_t)t_rows, a.rows - row0);
+  const int total = here * a.per_row;
+  const int half_bytes = a.head_dim / 2 * (16 / E);
+  const bool lane_live = sub < chunks;
+  for (int base = 0; base < total; base += groups * R) {
+    uint4 raw[R][2];
+    int vrow[R], vhead[R], vt[R];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      const int v = base + r * groups + gid;
+      vrow[r] = v < total ? v / a.per_row : -1;
+      const int h = v - vrow[r] * a.per_row;
+      vt[r] = h >= a.heads, vhead[r] = h - vt[r] * a.heads;
+      if (vrow[r] >= 0 && lane_live) {
+        const char *p = a.in[vt[r]] + (row0 + vrow[r]) * a.in_stride[vt[r]] + vhead[r] * 2 * half_bytes + sub * 16;
+        raw[r][0] = __ldcs(reinterpret_cast<const uint4 *>(p));
+        raw[r][1] = __ldcs(reinterpret_cast<const uint4 *>(p + half_bytes));
+      } else {
+        raw[r][0] = raw[r][1] = make_uint4(0, 0, 0, 0);
+      }
+    }
+    if (base == 0) {
+      for (int i = threadIdx.x; i < here * a.rotated; i += kThreads) turn[i] = turn_of(a, row0 + i / a.rotated, i % a.rotated);
+      __syncthreads();
+    }
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      float x[2 * E];
+      Chunk<DT>::unpack(raw[r][0], x);
+      Chunk<DT>::unpack(raw[r][1], x + E);
+      if (NORM) {
+        float ss = 0.f;
+#pragma unroll
+        for (int e = 0; e < 2 * E; e++) ss += x[e] * x[e];
+        for (int d = lanes >> 1; d > 0; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+        const float inv = rsqrtf(ss * a.inv_dim + a.eps);
+        if (vrow[r] >= 0 && lane_live) {
+          const float *g = a.gain[vt[r]] + vhead[r] * a.head_dim + sub * E;
+#pragma unroll
+          for (int q = 0; q < 2; q++)
+#pragma unroll
+            for (int e4 = 0; e4 < E / 4; e4++) {
+              const float4 w = __ldg(reinterpret_cast<const float4 *>(g + q * (a.head_dim / 2)) + e4);
+              float *z = x + q * E + e4 * 4;
+              z[0] *= inv * w.x, z[1] *= inv * w.y, z[2] *= inv * w.z, z[3] *= inv * w.w;
+            }
+        }
+      }
+      if (vrow[r] < 0 || !lane_live) continue;
+      const float2 *t = turn + vrow[r] * a.rotated;
+      if (PAIRS) {
+#pragma unroll
+        for (int q = 0; q < 2; q++)
+#pragma unroll
+          for (int e = 0; e < E; e += 2) {
+            const int p = (q * (a.head_dim / 2) + sub * E + e) / 2;
+            if (p < a.rotated) {
+              const float2 cs = t[p];
+              const float u = x[q * E + e], v = x[q * E + e + 1];
+              x[q * E + e] = u * cs.x - v * cs.y, x[q * E + e + 1] = u * cs.y + v * cs.x;
+            }
+          }
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+          const int p = sub * E + e;
+          if (p < a.rotated) {
+            const float2 cs = t[p];
+            const float u = x[e], v = x[E + e];
+            x[e] = u * cs.x - v * cs.y, x[E + e] = u * cs.y + v * cs.x;
+          }
+        }
+      }
+      char *p = a.out[vt[r]] + (row0 + vrow[r]) * a.out_stride[vt[r]] + vhead[r] * 2 * half_bytes + sub * 16;
+      __stcs(reinterpret_cast<uint4 *>(p), Chunk<DT>::pack(x));
+      __stcs(reinterpret_cast<uint4 *>(p + half_bytes), Chunk<DT>::pack(x + E));
+    }
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ float ld1(const char *p, int i) {
+  if (DT == T2SC_DT_F32) return reinterpret_cast<const float *>(p)[i];
+  if (DT == T2SC_DT_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(p)[i]);
+  return __half2float(reinterpret_cast<const __half *>(p)[i]);
+}
+template <int DT>
+__device__ __forceinline__ void st1(char *p, int i, float v) {
+  if (DT == T2SC_DT_F32)
+    reinterpret_cast<float *>(p)[i] = v;
+  else if (DT == T2SC_DT_BF16)
+    reinterpret_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(v);
+  else
+    reinterpret_cast<__half *>(p)[i] = __float2half_rn(v);
+}
+
+// Any even head_dim and any element alignment: one warp a head, one pair a
+// lane at a time, the whole head read before any of it is written.
+template <int DT, bool NORM, bool PAIRS>
+__global__ void __launch_bounds__(kThreads) rope_scalar_kernel(const RopeArgs a) {
+  constexpr int P = kMaxHeadDim / 2 / 32;
+  const int lane = threadIdx.x & 31;
+  const int64_t i = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+  if (i >= a.rows * a.per_row) return;
+  const int64_t row = i / a.per_row;
+  int h = (int)(i - row * a.per_row);
+  const int t = h >= a.heads;
+  h -= t * a.heads;
+  const int half = a.head_dim / 2, es = DT == T2SC_DT_F32 ? 4 : 2;
+  const char *in = a.in[t] + row * a.in_stride[t] + (int64_t)h * a.head_dim * es;
+  char *out = a.out[t] + row * a.out_stride[t] + (int64_t)h * a.head_dim * es;
+  float u[P], v[P], ss = 0.f;
+#pragma unroll
+  for (int q = 0; q < P; q++) {
+    const int p = q * 32 + lane;
+    u[q] = p < half ? ld1<DT>(in, PAIRS ? 2 * p : p) : 0.f;
+    v[q] = p < half ? ld1<DT>(in, PAIRS ? 2 * p + 1 : p + half) : 0.f;
+    ss += u[q] * u[q] + v[q] * v[q];
+  }
+  if (NORM) {
+    for (int d = 16; d > 0; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+  }
+  const float inv = NORM ? rsqrtf(ss * a.inv_dim + a.eps) : 1.f;
+#pragma unroll
+  for (int q = 0; q < P; q++) {
+    const int p = q * 32 + lane;
+    if (p >= half) continue;
+    const int iu = PAIRS ? 2 * p : p, iv = PAIRS ? 2 * p + 1 : p + half;
+    if (NORM) {
+      const float *g = a.gain[t] + h * a.head_dim;
+      u[q] *= inv * __ldg(g + iu), v[q] *= inv * __ldg(g + iv);
+    }
+    if (p < a.rotated) {
+      const float2 cs = turn_of(a, row, p);
+      const float x = u[q], y = v[q];
+      u[q] = x * cs.x - y * cs.y, v[q] = x * cs.y + y * cs.x;
+    }
+    st1<DT>(out, iu, u[q]);
+    st1<DT>(out, iv, v[q]);
+  }
+}
+
+template <int DT, bool NORM, bool PAIRS>
+int launch(t2sc_ctx *ctx, const RopeArgs &a, std::string &err) {
+  const int es = DT == T2SC_DT_F32 ? 4 : 2;
+  constexpr int E = Chunk<DT>::kElems;
+  bool vec = a.head_dim % (2 * E) == 0;
+  for (int t = 0; t < (a.per_row > a.heads ? 2 : 1); t++) {
+    auto off = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; };
+    if (off(a.in[t]) || off(a.out[t]) || a.in_stride[t] % 16 || a.out_stride[t] % 16 || (NORM && off(a.gain[t]))) vec = false;
+  }
+  if (vec) {
+    constexpr int R = 4;
+    const int chunks = a.head_dim / 2 / E;
+    int lanes = 1;
+    while (lanes < chunks) lanes <<= 1;
+    // Rows a CTA takes: as many as its groups hold at once (R heads each), so
+    // that one angle serves all heads; fewer when that would leave SMs idle.
+    const int held = kThreads / lanes * R;
+    int64_t t_rows = held / a.per_row;
+    if (t_rows > 16) t_rows = 16;
+    while (t_rows > 1 && (a.rows + t_rows - 1) / t_rows < 2 * ctx->num_sms) t_rows--;
+    if (t_rows < 1) t_rows = 1;
+    const int64_t grid = (a.rows + t_rows - 1) / t_rows;
+    if (grid <= INT32_MAX) {
+      const size_t smem = (size_t)t_rows * a.rotated * sizeof(float2);  // <= 16 x 128 x 8 bytes
+      rope_vec_kernel<DT, NORM, PAIRS, R><<<(unsigned)grid, kThreads, smem, ctx->stream>>>(a, (int)t_rows, lanes, chunks);
+      T2SC_LAUNCHED(ctx, "rope");
+      return T2SC_OK;
+    }
+  }
+  const int64_t warps = a.rows * a.per_row, grid = (warps + kThreads / 32 - 1) / (kThreads / 32);
+  if (grid > INT32_MAX) return fail(ctx, T2SC_ERR_UNSUPPORTED, "rope: too many heads in one call");
+  (void)es;
+  rope_scalar_kernel<DT, NORM, PAIRS><<<(unsigned)grid, kThreads, 0, ctx->stream>>>(a);
+  T2SC_LAUNCHED(ctx, "rope");
+  return T2SC_OK;
+}
+
+template <int DT>
+int launch_dt(t2sc_ctx *ctx, const RopeArgs &a, bool norm, bool pairs, std::string &err) {
+  if (norm) return pairs ? launch<DT, true, true>(ctx, a, err) : launch<DT, true, false>(ctx, a, err);
+  return pairs ? launch<DT, false, true>(ctx, a, err) : launch<DT, false, false>(ctx, a, err);
+}
+
+int launch_any(t2sc_ctx *ctx, const RopeArgs &a, bool norm, bool pairs, int dtype) {
+  std::string &err = ctx->last_error;
+  if (dtype == T2SC_DT_F32) return launch_dt<T2SC_DT_F32>(ctx, a, norm, pairs, err);
+  if (dtype == T2SC_DT_BF16) return launch_dt<T2SC_DT_BF16>(ctx, a, norm, pairs, err);
+  return launch_dt<T2SC_DT_F16>(ctx, a, norm, pairs, err);
+}
+
+// Checks one input/output pair and enters it into the launch arguments.
+int enter(t2sc_ctx *ctx, RopeArgs &a, int t, const void *in, int64_t in_stride, void *out, int64_t out_stride, int dtype,
+          const char *what, Rows *ri, Rows *ro) {
+  const int64_t width = (int64_t)a.heads * a.head_dim;
+  *ri = Rows{in, in_stride, a.rows, width, dtype_size(dtype)};
+  *ro = Rows{out, out_stride, a.rows, width, dtype_size(dtype)};
+  if (!in || !out) return fail(ctx, T2SC_ERR_INVALID, std::string(what) + ": null buffer");
+  if (!stride_ok(*ri) || !stride_ok(*ro))
+    return fail(ctx, T2SC_ERR_INVALID, std::string(what) + ": a row stride must be in [heads * head_dim, 2^28]");
+  if (!aligned_to_elem(*ri) || !aligned_to_elem(*ro))
+    return fail(ctx, T2SC_ERR_INVALID, std::string(what) + ": a buffer is not aligned to its element type");
+  if (!same_rows(*ri, *ro) && overlaps(*ri, *ro))
+    return fail(ctx, T2SC_ERR_INVALID, std::string(what) + ": the output overlaps the input without being the input");
+  a.in[t] = static_cast<const char *>(in), a.out[t] = static_cast<char *>(out);
+  a.in_stride[t] = in_stride * dtype_size(dtype), a.out_stride[t] = out_stride * dtype_size(dtype);
+  return T2SC_OK;
+}
+
+int check_coords(t2sc_ctx *ctx, const int32_t *coords, const char *what) {
+  if (!coords) return fail(ctx, T2SC_ERR_INVALID, std::string(what) + ": null coords");
+  if (reinterpret_cast<uintptr_t>(coords) % 4)
+    return fail(ctx, T2SC_ERR_INVALID, std::string(what) + ": coords are not aligned to 4 bytes");
+  return T2SC_OK;
+}
+
+void enter_rope(RopeArgs &a, const t2sc_rope *r, const int32_t *coords) {
+  a.coords = coords;
+  a.turns = r->d_turns;
+  a.n0 = r->n_axis[0], a.n01 = r->n_axis[0] + r->n_axis[1], a.rotated = r->rotated;
+}
+
+}  // namespace
+}  // namespace t2sc
+
+using namespace t2sc;
+
+extern "C" {
+
+int t2sc_rope_create(t2sc_ctx *ctx, int head_dim, int pairs_x, int pairs_y, int pairs_z, double theta, int layout,
+                     t2sc_rope **out) {
+  if (!ctx || !out) return T2SC_ERR_INVALID;
+  *out = nullptr;
+  if (head_dim < 2 || head_dim % 2 || head_dim > kMaxHeadDim)
+    return fail(ctx, T2SC_ERR_INVALID, "rope: head_dim must be even and in [2, 256]");
+  const int n[3] = {pairs_x, pairs_y, pairs_z};
+  for (int i = 0; i < 3; i++)
+    if (n[i] < 0 || n[i] > head_dim / 2) return fail(ctx, T2SC_ERR_INVALID, "rope: pairs of an axis must be in [0, head_dim / 2]");
+  if (n[0] + n[1] + n[2] > head_dim / 2) return fail(ctx, T2SC_ERR_INVALID, "rope: the axes take more pairs than a head has");
+  if (!(theta > 0.0) || !std::isfinite(theta)) return fail(ctx, T2SC_ERR_INVALID, "rope: theta must be positive and finite");
+  if (layout != T2SC_ROPE_PAIRS && layout != T2SC_ROPE_HALVES) return fail(ctx, T2SC_ERR_INVALID, "rope: unknown layout");
+  return guarded(ctx, [&]() -> int {
+    DeviceGuard g(ctx->device);
+    std::string &err = ctx->last_error;
+    std::unique_ptr<t2sc_rope, int (*)(t2sc_rope *)> r(new t2sc_rope(), t2sc_rope_destroy);
+    r->ctx = ctx;
+    r->head_dim = head_dim;
+    r->layout = layout;
+    r->rotated = n[0] + n[1] + n[2];
+    std::vector<double> turns;
+    for (int i = 0; i < 3; i++) {
+      r->n_axis[i] = n[i];
+      for (int j = 0; j < n[i]; j++) turns.push_back(std::pow(theta, -(double)j / n[i]) / (2.0 * 3.14159265358979323846));
+    }
+    T2SC_CUDA(cudaMalloc((void **)&r->d_turns, (turns.size() + 1) * sizeof(double)), "rope frequencies");
+    if (!turns.empty())
+      T2SC_CUDA(cudaMemcpy(r->d_turns, turns.data(), turns.size() * sizeof(double), cudaMemcpyHostToDevice), "rope frequencies");
+    *out = r.release();
+    return T2SC_OK;
+  });
+}
+
+int t2sc_rope_destroy(t2sc_rope *r) {
+  if (!r) return T2SC_OK;
+  DeviceGuard g(r->ctx->device);
+  if (r->d_turns) cudaFree(r->d_turns);
+  delete r;
+  return T2SC_OK;
+}
+
+int t2sc_rope_apply_device(t2sc_rope *rope, const int32_t *coords, const void *x, int64_t x_stride, void *y,
+                           int64_t y_stride, int64_t rows, int heads, int dtype) {
+  if (!rope) return T2SC_ERR_INVALID;
+  t2sc_ctx *ctx = rope->ctx;
+  return guarded(ctx, [&]() -> int {
+    if (rows < 0 || rows > INT32_MAX) return fail(ctx, T2SC_ERR_INVALID, "rope: rows must be in [0, 2^31)");
+    if (heads < 1 || heads > 4096) return fail(ctx, T2SC_ERR_INVALID, "rope: heads must be in [1, 4096]");
+    if (!dtype_known(dtype)) return fail(ctx, T2SC_ERR_INVALID, "rope: unknown dtype");
+    if (rows == 0) return T2SC_OK;
+    RopeArgs a;
+    a.rows = rows, a.heads = a.per_row = heads, a.head_dim = rope->head_dim;
+    Rows ri, ro;
+    T2SC_TRY(check_coords(ctx, coords, "rope"));
+    T2SC_TRY(enter(ctx, a, 0, x, x_stride, y, y_stride, dtype, "rope", &ri, &ro));
+    if (overlaps(ro, Rows{coords, 4, rows, 4, 4})) return fail(ctx, T2SC_ERR_INVALID, "rope: the output overlaps coords");
+    enter_rope(a, rope, coords);
+    DeviceGuard g(ctx->device);
+    return launch_any(ctx, a, false, rope->layout == T2SC_ROPE_PAIRS, dtype);
+  });
+}
+
+int t2sc_qk_norm_rope_device(t2sc_ctx *ctx, t2sc_rope *rope, const int32_t *coords, const void *q, int64_t q_stride,
+                             const void *k, int64_t k_stride, const float *gain_q, const float *gain_k, void *q_out,
+                             int64_t q_out_stride, void *k_out, int64_t k_out_stride, int64_t rows, int heads,
+                             int head_dim, float eps, int dtype) {
+  if (!ctx) return T2SC_ERR_INVALID;
+  return guarded(ctx, [&]() -> int {
+    if (rows < 0 || rows > INT32_MAX) return fail(ctx, T2SC_ERR_INVALID, "qk_norm_rope: rows must be in [0, 2^31)");
+    if (heads < 1 || heads > 4096) return fail(ctx, T2SC_ERR_INVALID, "qk_norm_rope: heads must be in [1, 4096]");
+    if (head_dim < 2 || head_dim % 2 || head_dim > kMaxHeadDim)
+      return fail(ctx, T2SC_ERR_INVALID, "qk_norm_rope: head_dim must be even and in [2, 256]");
+    if (!dtype_known(dtype)) return fail(ctx, T2SC_ERR_INVALID, "qk_norm_rope: unknown dtype");
+    if (!(eps > 0.f) || !std::isfinite(eps)) return fail(ctx, T2SC_ERR_INVALID, "qk_norm_rope: eps must be positive and finite");
+    if (rope && (rope->ctx != ctx || rope->head_dim != head_dim))
+      return fail(ctx, T2SC_ERR_INVALID, "qk_norm_rope: rope handle of another context or head_dim");
+    if ((k == nullptr) != (k_out == nullptr)) return fail(ctx, T2SC_ERR_INVALID, "qk_norm_rope: k and k_out must both be set or both NULL");
+    if (rows == 0) return T2SC_OK;
+    RopeArgs a;
+    a.rows = rows, a.heads = heads, a.head_dim = head_dim, a.per_row = k ? 2 * heads : heads;
+    a.eps = eps, a.inv_dim = 1.0f / (float)head_dim;
+    Rows qi, qo, ki, ko;
+    const char *what = "qk_norm_rope";
+    T2SC_TRY(enter(ctx, a, 0, q, q_stride, q_out, q_out_stride, dtype, what, &qi, &qo));
+    if (k) T2SC_TRY(enter(ctx, a, 1, k, k_stride, k_out, k_out_stride, dtype, what, &ki, &ko));
+    if (k && (overlaps(qo, ki) || overlaps(ko, qi) || overlaps(qo, ko)))
+      return fail(ctx, T2SC_ERR_INVALID, "qk_norm_rope: an output overlaps the other input or output");
+    const float *gains[2] = {gain_q, gain_k};
+    for (int t = 0; t < (k ? 2 : 1); t++) {
+      const Rows gr{gains[t], head_dim, heads, head_dim, 4};
+      if (!gains[t] || !aligned_to_elem(gr)) return fail(ctx, T2SC_ERR_INVALID, "qk_norm_rope: null or unaligned gain");
+      if (overlaps(qo, gr) || (k && overlaps(ko, gr))) return fail(ctx, T2SC_ERR_INVALID, "qk_norm_rope: an output overlaps a gain");
+      a.gain[t] = gains[t];
+    }
+    if (rope) {
+      T2SC_TRY(check_coords(ctx, coords, what));
+      const Rows cr{coords, 4, rows, 4, 4};
+      if (overlaps(qo, cr) || (k && overlaps(ko, cr))) return fail(ctx, T2SC_ERR_INVALID, "qk_norm_rope: an output overlaps coords");
+      enter_rope(a, rope, coords);
+    }
+    DeviceGuard g(ctx->device);
+    return launch_any(ctx, a, true, !rope || rope->layout == T2SC_ROPE_PAIRS, dtype);
+  });
+}
+
+}  // extern "C"

@@ -12,7 +12,8 @@ LIB_PATH = os.path.join(_HERE, "libt2sc.so")
 OK = 0
 ERR_INVALID, ERR_CUDA, ERR_OOM, ERR_RANGE, ERR_TIMEOUT, ERR_UNSUPPORTED, ERR_CAPACITY = 1, 2, 3, 4, 5, 6, 7
 DT_F32, DT_F16, DT_BF16 = 0, 1, 2
-SILU, RESIDUAL = 1, 2
+SILU, RESIDUAL, GELU = 1, 2, 4
+ROPE_PAIRS, ROPE_HALVES = 0, 1
 SUB_NONZERO, SUB_POSITIVE = 0, 1
 FEATS_NONE, FEATS_UPSAMPLE, FEATS_C2S = 0, 1, 2
 
@@ -69,6 +70,14 @@ SIGNATURES = {
     "t2sc_comm_abort": (I32, [P]),
     "t2sc_halo_exchange_device": (I32, [P, P, I64, P]),
     "t2sc_comm_wait": (I32, [P, I32]),
+    "t2sc_dense_linear_device": (I32, [P, P, I64, P, I64, P, P, I64, P, I64, I64, I32, I32, I32, I32]),
+    "t2sc_rope_create": (I32, [P, I32, I32, I32, I32, D, I32, PP]),
+    "t2sc_rope_destroy": (I32, [P]),
+    "t2sc_rope_apply_device": (I32, [P, P, P, I64, P, I64, I64, I32, I32]),
+    "t2sc_qk_norm_rope_device": (I32, [P, P, P, P, I64, P, I64, P, P, P, I64, P, I64, I64, I32, I32, F, I32]),
+    "t2sc_seqs_create": (I32, [P, P, P, I64, PP]),
+    "t2sc_seqs_destroy": (I32, [P]),
+    "t2sc_attention_device": (I32, [P, P, I64, P, I64, P, I64, P, I64, I32, I32, F, I32]),
     "t2sc_synth_shell": (I32, [I32, D, D, U64, I32, P, I64, PI64]),
     "t2sc_synth_normal": (I32, [U64, F, P, I64]),
     "t2sc_synth_bernoulli": (I32, [U64, D, P, I64]),

@@ -1,0 +1,411 @@
+"""The attention block over voxel tokens, on the device.
+
+Operators over CUDA tensors of rows, each one C-ABI call on torch's current
+stream:
+  dense_linear_device      act(x @ w^T + bias) + residual   (linear, trellis2_mojo/modules/nn.mojo:27-266)
+  RotaryPositionEmbedder   rotary positions over x, y, z    (trellis2_mojo/modules/rope.mojo)
+  qk_norm_rope_device      per-head RMS norm + rotation     (bias_rms_rope_qkv, trellis2_mojo/gpu/attention.mojo:507)
+  SequenceLayout           a ragged batch; attention inside each sequence (trellis2_mojo/sparse/attention)
+and the block's two halves made of them:
+  SparseMultiHeadAttention, SparseFeedForwardNet
+"""
+import ctypes
+
+import numpy as np
+
+from . import _lib
+from ._lib import check, lib
+from .decoder import _on_torch_stream
+from .sparse import _DTYPES, Context, SparseTensor, _check_on_ctx_device
+
+_ACTIVATIONS = {None: 0, "silu": _lib.SILU, "gelu": _lib.GELU}
+_LAYOUTS = {"pairs": _lib.ROPE_PAIRS, "halves": _lib.ROPE_HALVES}
+_CODES = None
+
+
+def _code(dtype):
+    global _CODES
+    if _CODES is None:
+        import torch
+        _CODES = {torch.float32: _lib.DT_F32, torch.float16: _lib.DT_F16, torch.bfloat16: _lib.DT_BF16}
+    return _CODES.get(dtype)
+
+
+def _rows2d(t, ctx, dtype, what):
+    """Row stride of a [rows, width] tensor whose rows are contiguous."""
+    _check_on_ctx_device(t, ctx, what)
+    if t.dtype != dtype:
+        raise ValueError(f"{what} must be {dtype}")
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{what} must be [rows, width] with contiguous rows")
+    return _row_stride(t, t.shape[1], what)
+
+
+def _heads3d(t, ctx, dtype, what):
+    """Row stride of a [rows, heads, head_dim] tensor whose rows are contiguous."""
+    _check_on_ctx_device(t, ctx, what)
+    if t.dtype != dtype:
+        raise ValueError(f"{what} must be {dtype}")
+    if t.dim() != 3:
+        raise ValueError(f"{what} must be [rows, heads, head_dim]")
+    _, h, d = t.shape
+    if (d > 1 and t.stride(2) != 1) or (h > 1 and t.stride(1) != d):
+        raise ValueError(f"{what} must be [rows, heads, head_dim] with contiguous rows")
+    return _row_stride(t, h * d, what)
+
+
+def _row_stride(t, width, what):
+    if t.shape[0] <= 1:
+        return width
+    s = t.stride(0)
+    if s < width:
+        raise ValueError(f"{what}: rows overlap")
+    return s
+
+
+def _f32(t, ctx, shape, what):
+    import torch
+    _check_on_ctx_device(t, ctx, what)
+    if t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f"{what} must be contiguous float32 {list(shape)}")
+    return t.data_ptr()
+
+
+def _coords(t, ctx, rows):
+    import torch
+    _check_on_ctx_device(t, ctx, "coords")
+    if t.dtype != torch.int32 or tuple(t.shape) != (rows, 4) or not t.is_contiguous():
+        raise ValueError("coords must be contiguous int32 [rows, 4]")
+    return t.data_ptr()
+
+
+def _context(ctx, t):
+    if ctx is not None:
+        return ctx
+    if not getattr(t, "is_cuda", False):
+        raise ValueError("the operator takes CUDA tensors")
+    return Context.default(t.device.index)
+
+
+def dense_linear_device(x, weight, bias=None, activation=None, residual=None, out=None, ctx=None):
+    """act(x @ weight.T + bias) + residual. x [rows, ci] and weight [co, ci]:
+    CUDA tensors of one type (float16, bfloat16 or float32) whose rows may be
+    strided; bias float32 [co]; activation None, "silu" or "gelu" (tanh
+    form); residual and out [rows, co] of x's type, out may be residual."""
+    ctx = _context(ctx, x)
+    if activation not in _ACTIVATIONS:
+        raise ValueError('dense_linear: activation must be None, "silu" or "gelu"')
+    code = _code(x.dtype)
+    if code is None:
+        raise ValueError("dense_linear: x must be float32, float16 or bfloat16")
+    ldx = _rows2d(x, ctx, x.dtype, "dense_linear: x")
+    ldw = _rows2d(weight, ctx, x.dtype, "dense_linear: weight")
+    rows, ci = x.shape
+    co = weight.shape[0]
+    if weight.shape[1] != ci or ci < 1 or co < 1:
+        raise ValueError("dense_linear: weight must be [co, ci] with x's ci")
+    flags = _ACTIVATIONS[activation]
+    ldr = 0
+    if residual is not None:
+        ldr = _rows2d(residual, ctx, x.dtype, "dense_linear: residual")
+        if tuple(residual.shape) != (rows, co):
+            raise ValueError("dense_linear: residual must be [rows, co]")
+        flags |= _lib.RESIDUAL
+    if out is None:
+        out = x.new_empty((rows, co))
+    elif tuple(out.shape) != (rows, co):
+        raise ValueError("dense_linear: out must be [rows, co]")
+    ldy = _rows2d(out, ctx, x.dtype, "dense_linear: out")
+    if rows == 0:
+        return out
+    _on_torch_stream(ctx, x.device)
+    check(lib.t2sc_dense_linear_device(ctx.handle, x.data_ptr(), ldx, weight.data_ptr(), ldw,
+                                       None if bias is None else _f32(bias, ctx, (co,), "dense_linear: bias"),
+                                       None if residual is None else residual.data_ptr(), ldr, out.data_ptr(), ldy,
+                                       rows, co, ci, flags, code), ctx.handle)
+    return out
+
+
+class RotaryPositionEmbedder:
+    """Rotary positions over the voxel axes x, y, z (columns 1..3 of the
+    coordinates). Each axis takes pairs[a] of a head's head_dim / 2 pairs
+    (default: a third each, rounded down), pair j of an axis turning by
+    position * theta^(-j / pairs[a]); the rest do not turn. layout: "pairs"
+    (channels 2p, 2p + 1) or "halves" (channels p, p + head_dim / 2)."""
+
+    def __init__(self, head_dim, pairs=None, theta=10000.0, layout="pairs", ctx=None):
+        if layout not in _LAYOUTS:
+            raise ValueError('RotaryPositionEmbedder: layout must be "pairs" or "halves"')
+        self.head_dim, self.theta, self.layout = int(head_dim), float(theta), layout
+        self.pairs = tuple(int(p) for p in pairs) if pairs is not None else (self.head_dim // 6,) * 3
+        if len(self.pairs) != 3:
+            raise ValueError("RotaryPositionEmbedder: pairs are three counts, of x, y and z")
+        self.ctx = ctx or Context.default()
+        h = ctypes.c_void_p()
+        check(lib.t2sc_rope_create(self.ctx.handle, self.head_dim, *self.pairs, self.theta, _LAYOUTS[layout],
+                                   ctypes.byref(h)), self.ctx.handle)
+        self.handle = h
+
+    def forward_device(self, x, coords, out=None):
+        """x [rows, heads, head_dim] (rows may be strided), coords int32 [rows, 4]; out may be x."""
+        code = _code(x.dtype)
+        if code is None:
+            raise ValueError("RotaryPositionEmbedder: x must be float32, float16 or bfloat16")
+        ldx = _heads3d(x, self.ctx, x.dtype, "RotaryPositionEmbedder: x")
+        rows, heads, d = x.shape
+        if d != self.head_dim or heads < 1:
+            raise ValueError("RotaryPositionEmbedder: x must be [rows, heads, head_dim]")
+        at = _coords(coords, self.ctx, rows)
+        if out is None:
+            out = x.new_empty((rows, heads, d))
+        elif out.shape != x.shape:
+            raise ValueError("RotaryPositionEmbedder: out must have x's shape")
+        ldy = _heads3d(out, self.ctx, x.dtype, "RotaryPositionEmbedder: out")
+        if rows:
+            _on_torch_stream(self.ctx, x.device)
+            check(lib.t2sc_rope_apply_device(self.handle, at, x.data_ptr(), ldx, out.data_ptr(), ldy, rows, heads, code),
+                  self.ctx.handle)
+        return out
+
+    def __del__(self):
+        h = getattr(self, "handle", None)
+        if h and self.ctx.handle:
+            lib.t2sc_rope_destroy(h)
+            self.handle = None
+
+
+def qk_norm_rope_device(q, k, gain_q, gain_k, coords=None, rope=None, eps=1e-6, out_q=None, out_k=None, ctx=None):
+    """RMS norm of every head of q and k with its own gains, then the rotation
+    of `rope` (None: no rotation) at `coords`, in one pass. q, k [rows, heads,
+    head_dim] (rows may be strided), gains float32 [heads, head_dim]. k None:
+    q alone. out_q may be q and out_k k. Returns (out_q, out_k)."""
+    ctx = rope.ctx if ctx is None and rope is not None else _context(ctx, q)
+    code = _code(q.dtype)
+    if code is None:
+        raise ValueError("qk_norm_rope: q must be float32, float16 or bfloat16")
+    ldq = _heads3d(q, ctx, q.dtype, "qk_norm_rope: q")
+    rows, heads, d = q.shape
+    if heads < 1 or (rope is not None and rope.head_dim != d):
+        raise ValueError("qk_norm_rope: q must be [rows, heads, head_dim] with rope's head_dim")
+    if out_q is None:
+        out_q = q.new_empty((rows, heads, d))
+    elif out_q.shape != q.shape:
+        raise ValueError("qk_norm_rope: out_q must have q's shape")
+    ldqo = _heads3d(out_q, ctx, q.dtype, "qk_norm_rope: out_q")
+    gq = _f32(gain_q, ctx, (heads, d), "qk_norm_rope: gain_q")
+    ldk = ldko = 0
+    gk = kp = kop = None
+    if k is not None:
+        ldk = _heads3d(k, ctx, q.dtype, "qk_norm_rope: k")
+        if k.shape != q.shape:
+            raise ValueError("qk_norm_rope: k must have q's shape")
+        if out_k is None:
+            out_k = q.new_empty((rows, heads, d))
+        elif out_k.shape != q.shape:
+            raise ValueError("qk_norm_rope: out_k must have q's shape")
+        ldko = _heads3d(out_k, ctx, q.dtype, "qk_norm_rope: out_k")
+        gk = _f32(gain_k, ctx, (heads, d), "qk_norm_rope: gain_k")
+        kp, kop = k.data_ptr(), out_k.data_ptr()
+    elif out_k is not None:
+        raise ValueError("qk_norm_rope: out_k without k")
+    at = _coords(coords, ctx, rows) if rope is not None else None
+    if rows:
+        _on_torch_stream(ctx, q.device)
+        check(lib.t2sc_qk_norm_rope_device(ctx.handle, None if rope is None else rope.handle, at, q.data_ptr(), ldq, kp,
+                                           ldk, gq, gk, out_q.data_ptr(), ldqo, kop, ldko, rows, heads, d, float(eps),
+                                           code), ctx.handle)
+    return out_q, out_k
+
+
+class SequenceLayout:
+    """The sequences of a ragged batch: lengths of each one's queries and of
+    its keys (None: the same, self-attention). Built once for a set of
+    coordinates (`of` a SparseTensor: one sequence per batch entry) and
+    shared by every layer and step."""
+
+    def __init__(self, q_lens, kv_lens=None, ctx=None):
+        self.q_offsets = self._offsets(q_lens)
+        self.kv_offsets = self.q_offsets if kv_lens is None else self._offsets(kv_lens)
+        if len(self.q_offsets) != len(self.kv_offsets):
+            raise ValueError("SequenceLayout: as many key lengths as query lengths")
+        self.ctx = ctx or Context.default()
+        h = ctypes.c_void_p()
+        check(lib.t2sc_seqs_create(self.ctx.handle, self.q_offsets.ctypes.data, self.kv_offsets.ctypes.data,
+                                   len(self.q_offsets) - 1, ctypes.byref(h)), self.ctx.handle)
+        self.handle = h
+
+    @classmethod
+    def of(cls, x, kv_lens=None):
+        """One sequence for each batch entry of a SparseTensor."""
+        return cls(np.diff(x.offsets), kv_lens, ctx=x.ctx)
+
+    @staticmethod
+    def _offsets(lens):
+        lens = np.asarray(lens, dtype=np.int64).reshape(-1)
+        if len(lens) and lens.min() < 0:
+            raise ValueError("SequenceLayout: lengths must not be negative")
+        return np.concatenate([[0], np.cumsum(lens)]).astype(np.int64)
+
+    def attention_device(self, q, k, v, scale=None, out=None):
+        """softmax(scale * q k^T) v inside each sequence. q [rows, heads,
+        head_dim] with the layout's query rows, k and v with its key rows
+        (more rows may follow; they are left alone); rows may be strided.
+        scale defaults to head_dim ** -0.5. out must not overlap an input."""
+        ctx = self.ctx
+        code = _code(q.dtype)
+        if code is None:
+            raise ValueError("attention: q must be float32, float16 or bfloat16")
+        ldq = _heads3d(q, ctx, q.dtype, "attention: q")
+        ldk = _heads3d(k, ctx, q.dtype, "attention: k")
+        ldv = _heads3d(v, ctx, q.dtype, "attention: v")
+        rows, heads, d = q.shape
+        if tuple(k.shape[1:]) != (heads, d) or v.shape != k.shape or heads < 1 or d < 1:
+            raise ValueError("attention: k and v must be [rows, heads, head_dim] with q's heads and head_dim")
+        if rows < self.q_offsets[-1] or k.shape[0] < self.kv_offsets[-1]:
+            raise ValueError("attention: fewer rows than the layout has")
+        if out is None:
+            out = q.new_empty((rows, heads, d))
+        elif out.shape != q.shape:
+            raise ValueError("attention: out must have q's shape")
+        ldo = _heads3d(out, ctx, q.dtype, "attention: out")
+        _on_torch_stream(ctx, q.device)
+        check(lib.t2sc_attention_device(self.handle, q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv,
+                                        out.data_ptr(), ldo, heads, d, float(d ** -0.5 if scale is None else scale),
+                                        code), ctx.handle)
+        return out
+
+    def __del__(self):
+        h = getattr(self, "handle", None)
+        if h and self.ctx.handle:
+            lib.t2sc_seqs_destroy(h)
+            self.handle = None
+
+
+def _tensor(a, dtype, device):
+    import torch
+    return None if a is None else torch.from_numpy(np.array(a, np.float32)).to(device, dtype)
+
+
+def _torch_dtype(dtype):
+    import torch
+    return {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[dtype]
+
+
+class SparseMultiHeadAttention:
+    """Self- or cross-attention of a SparseTensor's rows, inside each batch
+    entry: projections, per-head RMS norm of q and k (qk_norm), rotary
+    positions of the voxels (rope, self-attention only), attention, output
+    projection (+ residual).
+
+    Self-attention: to_qkv = (weight [3C, C], bias [3C]). Cross-attention
+    (ctx_channels given): to_q = (weight [C, C], bias) and to_kv = (weight
+    [2C, ctx_channels], bias). to_out = (weight [C, C], bias). gains =
+    (gain_q, gain_k), each [heads, head_dim], or None for no norm (then no
+    rotation either)."""
+
+    def __init__(self, channels, heads, to_out, to_qkv=None, to_q=None, to_kv=None, gains=None, rope=None, eps=1e-6,
+                 dtype="bf16", ctx=None):
+        if channels % heads:
+            raise ValueError("SparseMultiHeadAttention: channels must be a multiple of heads")
+        if (to_qkv is None) == (to_q is None or to_kv is None):
+            raise ValueError("SparseMultiHeadAttention: either to_qkv, or to_q and to_kv")
+        if rope is not None and (gains is None or to_qkv is None):
+            raise ValueError("SparseMultiHeadAttention: rotary positions go with self-attention and q/k gains")
+        if dtype not in _DTYPES:
+            raise ValueError("SparseMultiHeadAttention: dtype must be f32, f16 or bf16")
+        self.ctx = ctx or Context.default()
+        self.channels, self.heads, self.head_dim = channels, heads, channels // heads
+        self.cross, self.rope, self.eps, self.dtype = to_qkv is None, rope, float(eps), dtype
+        dev, dt = f"cuda:{self.ctx.device}", _torch_dtype(dtype)
+        import torch
+
+        def pair(wb, co, ci=None):
+            w, b = _tensor(wb[0], dt, dev), _tensor(wb[1], torch.float32, dev)
+            if w.dim() != 2 or w.shape[0] != co or (ci is not None and w.shape[1] != ci) or \
+                    (b is not None and tuple(b.shape) != (co,)):
+                raise ValueError("SparseMultiHeadAttention: projection weights must be [out, in] with bias [out]")
+            return w, b
+
+        if self.cross:
+            self._q, self._kv = pair(to_q, channels, channels), pair(to_kv, 2 * channels)
+        else:
+            self._qkv = pair(to_qkv, 3 * channels, channels)
+        self._out = pair(to_out, channels, channels)
+        self._gains = None
+        if gains is not None:
+            self._gains = tuple(_tensor(g, torch.float32, dev).reshape(heads, self.head_dim) for g in gains)
+
+    def forward_device(self, x, layout, coords=None, context=None, residual=None):
+        """x [rows, C] on the device; layout: the SequenceLayout of its rows
+        (and the context's); coords int32 [rows, 4] where rope is set;
+        context [context rows, ctx_channels] for cross-attention. Rows behind
+        the layout's last are not given a meaning: pass none."""
+        h, d, c = self.heads, self.head_dim, self.channels
+        rows = x.shape[0]
+        if rows != layout.q_offsets[-1]:
+            raise ValueError("SparseMultiHeadAttention: x must have the layout's rows")
+        if self.cross:
+            if context is None:
+                raise ValueError("SparseMultiHeadAttention: cross-attention needs a context")
+            q = dense_linear_device(x, *self._q, ctx=self.ctx).view(rows, h, d)
+            kv = dense_linear_device(context, *self._kv, ctx=self.ctx).view(context.shape[0], 2, h, d)
+            k, v = kv[:, 0], kv[:, 1]
+            if self._gains:
+                qk_norm_rope_device(q, None, self._gains[0], None, eps=self.eps, out_q=q, ctx=self.ctx)
+                qk_norm_rope_device(k, None, self._gains[1], None, eps=self.eps, out_q=k, ctx=self.ctx)
+        else:
+            qkv = dense_linear_device(x, *self._qkv, ctx=self.ctx).view(rows, 3, h, d)
+            q, k, v = qkv[:, 0], qkv[:, 1], qkv[:, 2]
+            if self._gains:
+                qk_norm_rope_device(q, k, *self._gains, coords=coords, rope=self.rope, eps=self.eps, out_q=q, out_k=k,
+                                    ctx=self.ctx)
+        a = layout.attention_device(q, k, v)
+        return dense_linear_device(a.view(rows, c), *self._out, residual=residual, ctx=self.ctx)
+
+    def forward(self, x, context=None, context_lens=None, residual=False):
+        """x: SparseTensor; context: host f32 [rows, ctx_channels] with
+        context_lens rows of it for each batch entry. residual: add x."""
+        import torch
+        dev, dt = f"cuda:{self.ctx.device}", _torch_dtype(self.dtype)
+        xd = _tensor(x.feats, dt, dev)
+        if self.cross and context_lens is None:
+            raise ValueError("SparseMultiHeadAttention: cross-attention needs context_lens")
+        layout = SequenceLayout(np.diff(x.offsets), context_lens if self.cross else None, ctx=self.ctx)
+        coords = torch.from_numpy(x.coords).to(dev) if self.rope is not None else None
+        y = self.forward_device(xd, layout, coords, _tensor(context, dt, dev), xd if residual else None)
+        y = y.float().cpu().numpy()
+        self.ctx.synchronize()
+        return x.replace(y)
+
+    __call__ = forward
+
+
+class SparseFeedForwardNet:
+    """lin2(GELU(lin1(x))) (+ residual) over rows: lin1 = (weight [H, C], bias
+    [H]), lin2 = (weight [C, H], bias [C])."""
+
+    def __init__(self, lin1, lin2, activation="gelu", dtype="bf16", ctx=None):
+        import torch
+        if activation not in _ACTIVATIONS:
+            raise ValueError('SparseFeedForwardNet: activation must be None, "silu" or "gelu"')
+        if dtype not in _DTYPES:
+            raise ValueError("SparseFeedForwardNet: dtype must be f32, f16 or bf16")
+        self.ctx = ctx or Context.default()
+        self.activation, self.dtype = activation, dtype
+        dev, dt = f"cuda:{self.ctx.device}", _torch_dtype(dtype)
+        self._lin1 = _tensor(lin1[0], dt, dev), _tensor(lin1[1], torch.float32, dev)
+        self._lin2 = _tensor(lin2[0], dt, dev), _tensor(lin2[1], torch.float32, dev)
+
+    def forward_device(self, x, residual=None):
+        h = dense_linear_device(x, *self._lin1, activation=self.activation, ctx=self.ctx)
+        return dense_linear_device(h, *self._lin2, residual=residual, ctx=self.ctx)
+
+    def forward(self, x, residual=False):
+        """x: SparseTensor or host f32 [rows, C]; residual: add x."""
+        st = x if isinstance(x, SparseTensor) else None
+        xd = _tensor(st.feats if st is not None else x, _torch_dtype(self.dtype), f"cuda:{self.ctx.device}")
+        y = self.forward_device(xd, xd if residual else None).float().cpu().numpy()
+        self.ctx.synchronize()
+        return st.replace(y) if st is not None else y
+
+    __call__ = forward
