@@ -281,9 +281,8 @@ int t2sc_c2s_block_forward_device(t2sc_c2s_block *block, t2sc_coords *coords, co
  * (with residual [rows, co]). Unlike t2sc_linear_forward_device it takes the
  * weight as it lies on the device and keeps nothing. y may be residual
  * itself (same address and stride); any other overlap with an input is
- * refused. 16-bit rows that start on 16 bytes (addresses, strides and ci
- * multiples of 8 elements) run on the tensor cores, f32 and other 16-bit
- * rows on the CUDA cores. */
+ * refused. 16-bit x and w whose rows start on 16 bytes (address and stride)
+ * run on the tensor cores, f32 and other 16-bit rows on the CUDA cores. */
 int t2sc_dense_linear_device(t2sc_ctx *ctx, const void *x, int64_t x_stride, const void *w, int64_t w_stride,
                              const float *bias, const void *residual, int64_t residual_stride, void *y,
                              int64_t y_stride, int64_t rows, int co, int ci, int flags, int dtype);

@@ -34,6 +34,9 @@ __device__ __forceinline__ float activate(float v, int act) {
   return v;
 }
 
+// 16-bit rows that start on 16 bytes (what TMA needs of x and w).
+bool dense_tc_takes(const DenseArgs &a, int dtype);
+int dense_tc(t2sc_ctx *ctx, const DenseArgs &a, int dtype, std::string &err);
 int dense_simt(t2sc_ctx *ctx, const DenseArgs &a, int dtype, std::string &err);
 
 }  // namespace t2sc

@@ -1,0 +1,388 @@
+// Dense linear on the tensor cores: y = act(x @ w^T + bias) + residual for
+// 16-bit rows that start on 16 bytes.
+//
+// Output tiles of 128 rows x BN columns a CTA, the K axis in 128-byte steps:
+// TMA brings the x and w tiles into a ring of shared-memory stages (128-byte
+// swizzle, zeros outside the matrices), one warp issues tcgen05.mma into one
+// of two TMEM accumulators while four warps drain the other through the
+// epilogue. With a CTA pair (CG = 2) one MMA covers 256 rows and each CTA
+// stages only half of the w tile, which halves what shared memory has to
+// take in and feed for w. The CTAs are persistent; a CTA's tiles are `slots`
+// apart with the columns fastest, so that the tiles in flight share their x
+// rows and the whole of w in L2.
+//
+// The epilogue takes 64 columns at a time: a thread owns a row (TMEM lane),
+// and the block passes through a swizzled 4 KB of shared memory per warp so
+// that the residual is read and y written in whole 128-byte rows. y may be
+// the residual: each element is read before the same thread writes it.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "dense.h"
+#include "entry.h"
+#include "internal.h"
+#include "sm100.cuh"
+#include "tensormap.h"
+
+namespace t2sc {
+namespace {
+
+constexpr int kTileM = 128;         // rows of a CTA's tile
+constexpr int kBK = 64;             // K elements of a stage: one 128-byte swizzle row
+constexpr int kSmemMax = 232448;    // 227 KB: the sm_100 per-block limit
+constexpr int kThreads = 192;       // warps 0-3 epilogue, 4 TMA, 5 MMA
+constexpr int kStageBytes = 4 * 32 * 128;  // epilogue staging, 4 KB a warp
+constexpr long long kWaitLimit = 4000000000ll;  // ~2 s of SM clocks
+
+struct DenseTcArgs {
+  CUtensorMap map_x, map_w;
+  const char *res;
+  char *y;
+  const float *bias;
+  int64_t ldr, ldy;  // elements
+  int64_t rows;
+  int co, k_iters, act, m_tiles, n_tiles, slots;
+  int vec;  // y (and residual) rows start on 16 bytes
+  int *err;
+};
+
+template <int CG, int BN>
+struct Shape {
+  static constexpr int kWRows = BN / CG;  // w rows a CTA stages
+  static constexpr int kABytes = kTileM * 128, kBBytes = kWRows * 128;
+  static constexpr int kStage = kABytes + kBBytes;
+  static constexpr int kStages = (kSmemMax - 1024 - kStageBytes - 512) / kStage > 8 ? 8 : (kSmemMax - 1024 - kStageBytes - 512) / kStage;
+  static constexpr size_t kSmem = 1024 + (size_t)kStages * kStage + kStageBytes + 512;
+  static constexpr uint32_t kCols = 2 * BN;  // two accumulators
+};
+
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *abort, int *err) {
+  bool ok = sm100::mbar_test_wait(bar, parity);
+  if (__all_sync(0xffffffffu, ok)) return true;
+  if (!ok) ok = sm100::mbar_wait_bounded(bar, parity, abort, err, kDevErrTimeout, kWaitLimit);
+  return __all_sync(0xffffffffu, ok);
+}
+
+template <int DT>
+__device__ __forceinline__ float ld16(const char *p) {
+  if (DT == T2SC_DT_BF16) return __bfloat162float(*reinterpret_cast<const __nv_bfloat16 *>(p));
+  return __half2float(*reinterpret_cast<const __half *>(p));
+}
+
+template <int DT, int CG, int BN>
+__global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_constant__ DenseTcArgs a) {
+  using S = Shape<CG, BN>;
+  constexpr int NS = S::kStages;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t *staging = smem + (size_t)NS * S::kStage;
+  uint64_t *bars = reinterpret_cast<uint64_t *>(staging + kStageBytes);  // full[NS], empty[NS], tfull[2], tempty[2], done
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * NS + 5);
+  volatile int *abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
+  const uint32_t sbase = sm100::smem_u32(smem), full0 = sm100::smem_u32(bars), empty0 = full0 + 8 * NS;
+  const uint32_t tfull0 = empty0 + 8 * NS, tempty0 = tfull0 + 16, done = tempty0 + 16;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = CG == 2 ? sm100::cluster_rank() : 0;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < NS; s++) {
+      sm100::mbar_init(full0 + 8 * s, 1);
+      sm100::mbar_init(empty0 + 8 * s, 1);
+    }
+    for (int b = 0; b < 2; b++) {
+      sm100::mbar_init(tfull0 + 8 * b, 1);
+      sm100::mbar_init(tempty0 + 8 * b, 4 * CG);  // every epilogue warp of the pair
+    }
+    sm100::mbar_init(done, 1);
+    *abort = 0;
+    sm100::fence_mbar_init();
+  }
+  if (warp == 5) {
+    if (CG == 2) {
+      sm100::tmem_alloc_pair(sm100::smem_u32(tmem_slot), S::kCols);
+      sm100::tmem_relinquish_pair();
+    } else {
+      sm100::tmem_alloc(sm100::smem_u32(tmem_slot), S::kCols);
+      sm100::tmem_relinquish();
+    }
+  }
+  sm100::tc_fence_before();
+  __syncthreads();
+  if (CG == 2) sm100::cluster_sync();  // the other CTA's barriers are ready before anything arrives on them
+  sm100::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int64_t ntiles = (int64_t)a.m_tiles * a.n_tiles;
+  const int64_t slot = blockIdx.x / CG;
+
+  if (warp == 4) {
+    // ------------------------------- TMA --------------------------------
+    if (lane == 0) {
+      sm100::tma_prefetch(&a.map_x);
+      sm100::tma_prefetch(&a.map_w);
+    }
+    uint32_t s = 0, ph = 0, it = 0;
+    bool ok = true;
+    for (int64_t t = slot; t < ntiles && ok; t += a.slots) {
+      const int m0 = (int)(t / a.n_tiles) * kTileM * CG + (int)rank * kTileM;
+      const int n0 = (int)(t % a.n_tiles) * BN + (int)rank * S::kWRows;
+      for (int k = 0; k < a.k_iters; k++) {
+        if (!warp_wait(empty0 + 8 * s, ph ^ 1, abort, a.err)) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) {
+          const uint32_t dst = sbase + s * S::kStage;
+          if (CG == 2) {
+            const uint32_t bar = sm100::map_to_rank(full0 + 8 * s, 0);  // CTA 0 waits for both CTAs' tiles
+            if (rank == 0) sm100::mbar_arrive_expect_tx(full0 + 8 * s, 2 * S::kStage);
+            sm100::tma_load_2d_pair(dst, &a.map_x, k * kBK, m0, bar);
+            sm100::tma_load_2d_pair(dst + S::kABytes, &a.map_w, k * kBK, n0, bar);
+          } else {
+            sm100::mbar_arrive_expect_tx(full0 + 8 * s, S::kStage);
+            sm100::tma_load_2d(dst, &a.map_x, k * kBK, m0, full0 + 8 * s);
+            sm100::tma_load_2d(dst + S::kABytes, &a.map_w, k * kBK, n0, full0 + 8 * s);
+          }
+        }
+        __syncwarp();
+        it++;
+        if (++s == NS) s = 0, ph ^= 1;
+      }
+    }
+    // every copy asked for has landed before shared memory is given up (a
+    // pair's land on CTA 0's barriers, and CTA 1 stays until the cluster's end)
+    if (lane == 0 && rank == 0) {
+      const uint32_t first = it > (uint32_t)NS ? it - NS : 0;
+      for (uint32_t i = first; i < it; i++)
+        sm100::mbar_wait_cycles(full0 + 8 * (i % NS), (i / NS) & 1, kWaitLimit / 8);
+    }
+    __syncwarp();
+  } else if (warp == 5) {
+    // ------------------------------- MMA --------------------------------
+    if (rank == 0) {
+      const uint32_t idesc = sm100::instr_desc(DT == T2SC_DT_BF16 ? 1 : 0, BN) + (CG == 2 ? (128u >> 4) << 24 : 0u);
+      const uint64_t da0 = sm100::smem_desc(sbase, 128), db0 = sm100::smem_desc(sbase + S::kABytes, 128);
+      uint32_t s = 0, ph = 0, acc = 0;
+      bool ok = true;
+      for (int64_t t = slot; t < ntiles && ok; t += a.slots) {
+        const uint32_t b = acc & 1;
+        if (!warp_wait(tempty0 + 8 * b, ((acc >> 1) & 1) ^ 1, abort, a.err)) break;
+        if (CG == 2) asm volatile("fence.acq_rel.cluster;" ::: "memory");  // half of the arrivals are the other CTA's
+        sm100::tc_fence_after();
+        const uint32_t d = tmem + b * BN;
+        for (int k = 0; k < a.k_iters; k++) {
+          if (!warp_wait(full0 + 8 * s, ph, abort, a.err)) {
+            ok = false;
+            break;
+          }
+          sm100::tc_fence_after();
+          const uint64_t so = (uint64_t)(s * S::kStage) >> 4;
+#pragma unroll
+          for (int kk = 0; kk < kBK / 16; kk++) {
+            const uint64_t da = da0 + so + kk * 2, db = db0 + so + kk * 2;
+            if (CG == 2)
+              sm100::mma_f16_pair_elect(d, da, db, idesc, k + kk > 0);
+            else
+              sm100::mma_f16_elect(d, da, db, idesc, k + kk > 0);
+          }
+          if (CG == 2)
+            sm100::mma_commit_pair_elect(empty0 + 8 * s);
+          else
+            sm100::mma_commit_elect(empty0 + 8 * s);
+          if (++s == NS) s = 0, ph ^= 1;
+        }
+        if (!ok) break;
+        if (CG == 2)
+          sm100::mma_commit_pair_elect(tfull0 + 8 * b);
+        else
+          sm100::mma_commit_elect(tfull0 + 8 * b);
+        acc++;
+      }
+      // all issued MMAs retire before TMEM and shared memory are given up
+      if (CG == 2)
+        sm100::mma_commit_pair_elect(done);
+      else
+        sm100::mma_commit_elect(done);
+      if (lane == 0) sm100::mbar_wait_cycles(done, 0, kWaitLimit / 8);
+      __syncwarp();
+    }
+  } else {
+    // ----------------------------- epilogue -----------------------------
+    uint8_t *stage = staging + warp * 4096;
+    uint32_t acc = 0;
+    const int crow = lane >> 3, cch = lane & 7;  // this lane's place when whole rows move: 4 rows x 8 chunks
+    for (int64_t t = slot; t < ntiles; t += a.slots) {
+      const int64_t row0 = (t / a.n_tiles) * (kTileM * CG) + (int64_t)rank * kTileM + warp * 32;
+      const int n0 = (int)(t % a.n_tiles) * BN;
+      const uint32_t b = acc & 1;
+      if (!warp_wait(tfull0 + 8 * b, (acc >> 1) & 1, abort, a.err)) break;
+      sm100::tc_fence_after();
+      const uint32_t taddr = tmem + b * BN + ((uint32_t)(warp * 32) << 16);
+#pragma unroll 1
+      for (int c0 = 0; c0 < BN; c0 += 64) {
+        const int col0 = n0 + c0;
+        const bool any = col0 < a.co && row0 < a.rows;
+        float v[64];
+        sm100::tmem_ld32(taddr + c0, reinterpret_cast<uint32_t *>(v));
+        sm100::tmem_ld32(taddr + c0 + 32, reinterpret_cast<uint32_t *>(v) + 32);
+        if (a.res && any) {
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            const int r = i * 4 + crow, col = col0 + cch * 8;
+            uint4 u = make_uint4(0, 0, 0, 0);
+            if (row0 + r < a.rows && col < a.co) {
+              const char *p = a.res + ((row0 + r) * a.ldr + col) * 2;
+              if (a.vec && col + 8 <= a.co) {
+                u = *reinterpret_cast<const uint4 *>(p);
+              } else {
+                uint16_t e[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) e[j] = col + j < a.co ? *reinterpret_cast<const uint16_t *>(p + 2 * j) : 0;
+                u = *reinterpret_cast<uint4 *>(e);
+              }
+            }
+            *reinterpret_cast<uint4 *>(stage + r * 128 + ((cch ^ (r & 7)) << 4)) = u;
+          }
+          __syncwarp();
+        }
+        sm100::tmem_ld_wait();
+        if (c0 + 64 == BN) {  // the accumulator is read out: the next tile may use it
+          sm100::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if (CG == 2)
+              sm100::mbar_arrive_cluster(sm100::map_to_rank(tempty0 + 8 * b, 0));
+            else
+              sm100::mbar_arrive(tempty0 + 8 * b);
+          }
+        }
+        if (any) {
+#pragma unroll
+          for (int c = 0; c < 8; c++) {
+            float *z = v + c * 8;
+            const int col = col0 + c * 8;
+            if (a.bias) {
+#pragma unroll
+              for (int j = 0; j < 8; j++) z[j] += col + j < a.co ? __ldg(a.bias + col + j) : 0.f;
+            }
+            if (a.act) {
+#pragma unroll
+              for (int j = 0; j < 8; j++) z[j] = activate(z[j], a.act);
+            }
+            uint4 *sp = reinterpret_cast<uint4 *>(stage + lane * 128 + ((c ^ (lane & 7)) << 4));
+            if (a.res) {
+              const uint4 u = *sp;
+              const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+              for (int j = 0; j < 4; j++) {
+                const float2 f = unpack2<DT>(w[j]);
+                z[2 * j] += f.x, z[2 * j + 1] += f.y;
+              }
+            }
+            *sp = make_uint4(pack2<DT>(z[0], z[1]), pack2<DT>(z[2], z[3]), pack2<DT>(z[4], z[5]), pack2<DT>(z[6], z[7]));
+          }
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            const int r = i * 4 + crow, col = col0 + cch * 8;
+            if (row0 + r < a.rows && col < a.co) {
+              const uint4 u = *reinterpret_cast<const uint4 *>(stage + r * 128 + ((cch ^ (r & 7)) << 4));
+              char *p = a.y + ((row0 + r) * a.ldy + col) * 2;
+              if (a.vec && col + 8 <= a.co) {
+                *reinterpret_cast<uint4 *>(p) = u;
+              } else {
+                const uint16_t *e = reinterpret_cast<const uint16_t *>(&u);
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                  if (col + j < a.co) *reinterpret_cast<uint16_t *>(p + 2 * j) = e[j];
+              }
+            }
+          }
+          __syncwarp();
+        }
+      }
+      acc++;
+    }
+  }
+  sm100::tc_fence_before();
+  __syncthreads();
+  if (CG == 2) sm100::cluster_sync();  // no CTA leaves while the other may still signal it or read its tiles
+  if (warp == 5) {
+    sm100::tc_fence_after();
+    if (CG == 2)
+      sm100::tmem_dealloc_pair(tmem, S::kCols);
+    else
+      sm100::tmem_dealloc(tmem, S::kCols);
+  }
+}
+
+template <int DT, int CG, int BN>
+int launch(t2sc_ctx *ctx, const DenseArgs &a, std::string &err) {
+  using S = Shape<CG, BN>;
+  DenseTcArgs t;
+  const uint64_t dx[2] = {(uint64_t)a.ci, (uint64_t)a.rows}, dw[2] = {(uint64_t)a.ci, (uint64_t)a.co};
+  const uint64_t one = ((uint64_t)a.ci * 2 + 15) / 16 * 16;  // a stride that a single row never uses
+  const uint64_t sx[1] = {a.rows > 1 ? (uint64_t)a.ldx * 2 : one}, sw[1] = {a.co > 1 ? (uint64_t)a.ldw * 2 : one};
+  const uint32_t bx[2] = {kBK, kTileM}, bw[2] = {kBK, (uint32_t)S::kWRows};
+  T2SC_TRY(tensormap_16bit(&t.map_x, DT, 2, a.x, dx, sx, bx, err));
+  T2SC_TRY(tensormap_16bit(&t.map_w, DT, 2, a.w, dw, sw, bw, err));
+  t.res = a.res, t.y = a.y, t.bias = a.bias, t.ldr = a.ldr, t.ldy = a.ldy, t.rows = a.rows, t.co = a.co;
+  t.k_iters = (a.ci + kBK - 1) / kBK, t.act = a.act, t.err = ctx->d_err;
+  t.m_tiles = (int)((a.rows + kTileM * CG - 1) / (kTileM * CG)), t.n_tiles = (a.co + BN - 1) / BN;
+  auto on16 = [&](const void *p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (a.rows <= 1 || ld % 8 == 0); };
+  t.vec = on16(a.y, a.ldy) && (!a.res || on16(a.res, a.ldr));
+  const int64_t tiles = (int64_t)t.m_tiles * t.n_tiles, most = ctx->num_sms / CG;
+  t.slots = (int)(tiles < most ? tiles : most);
+  auto kernel = dense_tc_kernel<DT, CG, BN>;
+  T2SC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem), "dense_linear");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)t.slots * CG), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = S::kSmem, cfg.stream = ctx->stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = CG, at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at, cfg.numAttrs = 1;
+  T2SC_CUDA(cudaLaunchKernelEx(&cfg, kernel, t), "dense_linear");
+  T2SC_LAUNCHED(ctx, "dense_linear");
+  return T2SC_OK;
+}
+
+template <int DT>
+int launch_dt(t2sc_ctx *ctx, const DenseArgs &a, std::string &err) {
+  // The tile shape that finishes first: rounds of tiles x (clocks of a K step
+  // of that shape x K steps + a tile's fixed part).
+  struct Option {
+    int cg, bn;
+    double step;
+  };
+  constexpr Option options[] = {{2, 256, 520}, {2, 128, 300}, {1, 128, 330}, {1, 64, 220}};
+  const double k_iters = (a.ci + kBK - 1) / kBK;
+  int best = 0;
+  double least = 1e300;
+  for (int i = 0; i < 4; i++) {
+    const Option &o = options[i];
+    const double tiles = (double)((a.rows + kTileM * o.cg - 1) / (kTileM * o.cg)) * ((a.co + o.bn - 1) / o.bn);
+    const double slots = ctx->num_sms / o.cg, rounds = (double)(int64_t)((tiles + slots - 1) / slots);
+    const double clocks = rounds * (k_iters * o.step + 600) + 8 * o.bn;
+    if (clocks < least) least = clocks, best = i;
+  }
+  switch (best) {
+    case 0: return launch<DT, 2, 256>(ctx, a, err);
+    case 1: return launch<DT, 2, 128>(ctx, a, err);
+    case 2: return launch<DT, 1, 128>(ctx, a, err);
+    default: return launch<DT, 1, 64>(ctx, a, err);
+  }
+}
+
+}  // namespace
+
+bool dense_tc_takes(const DenseArgs &a, int dtype) {
+  auto on16 = [](const void *p, int64_t ld, int64_t rows) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (rows <= 1 || ld % 8 == 0);
+  };
+  return dtype != T2SC_DT_F32 && on16(a.x, a.ldx, a.rows) && on16(a.w, a.ldw, a.co);
+}
+
+int dense_tc(t2sc_ctx *ctx, const DenseArgs &a, int dtype, std::string &err) {
+  return dtype == T2SC_DT_BF16 ? launch_dt<T2SC_DT_BF16>(ctx, a, err) : launch_dt<T2SC_DT_F16>(ctx, a, err);
+}
+
+}  // namespace t2sc
