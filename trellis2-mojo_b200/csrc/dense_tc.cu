@@ -4,7 +4,7 @@
 // Output tiles of 128 rows x BN columns a CTA, the K axis in 128-byte steps:
 // TMA brings the x and w tiles into a ring of shared-memory stages (128-byte
 // swizzle, zeros outside the matrices), one warp issues tcgen05.mma into one
-// of two TMEM accumulators while four warps drain the other through the
+// of two TMEM accumulators while eight warps drain the other through the
 // epilogue. With a CTA pair (CG = 2) one MMA covers 256 rows and each CTA
 // stages only half of the w tile, which halves what shared memory has to
 // take in and feed for w. The CTAs are persistent; a CTA's tiles are `slots`
@@ -30,8 +30,9 @@ namespace {
 constexpr int kTileM = 128;         // rows of a CTA's tile
 constexpr int kBK = 64;             // K elements of a stage: one 128-byte swizzle row
 constexpr int kSmemMax = 232448;    // 227 KB: the sm_100 per-block limit
-constexpr int kThreads = 192;       // warps 0-3 epilogue, 4 TMA, 5 MMA
-constexpr int kStageBytes = 4 * 32 * 128;  // epilogue staging, 4 KB a warp
+constexpr int kEpiWarps = 8;        // two per TMEM lane quadrant, 64 columns at a time each
+constexpr int kTmaWarp = kEpiWarps, kMmaWarp = kEpiWarps + 1, kThreads = 32 * (kEpiWarps + 2);
+constexpr int kStageBytes = kEpiWarps * 32 * 128;  // epilogue staging, 4 KB a warp
 constexpr long long kWaitLimit = 4000000000ll;  // ~2 s of SM clocks
 
 struct DenseTcArgs {
@@ -50,9 +51,12 @@ template <int CG, int BN>
 struct Shape {
   static constexpr int kWRows = BN / CG;  // w rows a CTA stages
   static constexpr int kABytes = kTileM * 128, kBBytes = kWRows * 128;
+  static constexpr int kBiasBytes = kEpiWarps * 64 * 4;
   static constexpr int kStage = kABytes + kBBytes;
-  static constexpr int kStages = (kSmemMax - 1024 - kStageBytes - 512) / kStage > 8 ? 8 : (kSmemMax - 1024 - kStageBytes - 512) / kStage;
-  static constexpr size_t kSmem = 1024 + (size_t)kStages * kStage + kStageBytes + 512;
+  static constexpr int kStages = (kSmemMax - 1024 - kStageBytes - kBiasBytes - 512) / kStage > 8
+                                     ? 8
+                                     : (kSmemMax - 1024 - kStageBytes - kBiasBytes - 512) / kStage;
+  static constexpr size_t kSmem = 1024 + (size_t)kStages * kStage + kStageBytes + kBiasBytes + 512;
   static constexpr uint32_t kCols = 2 * BN;  // two accumulators
 };
 
@@ -76,7 +80,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t *staging = smem + (size_t)NS * S::kStage;
-  uint64_t *bars = reinterpret_cast<uint64_t *>(staging + kStageBytes);  // full[NS], empty[NS], tfull[2], tempty[2], done
+  uint64_t *bars = reinterpret_cast<uint64_t *>(staging + kStageBytes + S::kBiasBytes);  // full[NS], empty[NS], tfull[2], tempty[2], done
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * NS + 5);
   volatile int *abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
   const uint32_t sbase = sm100::smem_u32(smem), full0 = sm100::smem_u32(bars), empty0 = full0 + 8 * NS;
@@ -91,13 +95,13 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
     }
     for (int b = 0; b < 2; b++) {
       sm100::mbar_init(tfull0 + 8 * b, 1);
-      sm100::mbar_init(tempty0 + 8 * b, 4 * CG);  // every epilogue warp of the pair
+      sm100::mbar_init(tempty0 + 8 * b, kEpiWarps * CG);  // every epilogue warp of the pair
     }
     sm100::mbar_init(done, 1);
     *abort = 0;
     sm100::fence_mbar_init();
   }
-  if (warp == 5) {
+  if (warp == kMmaWarp) {
     if (CG == 2) {
       sm100::tmem_alloc_pair(sm100::smem_u32(tmem_slot), S::kCols);
       sm100::tmem_relinquish_pair();
@@ -114,7 +118,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
   const int64_t ntiles = (int64_t)a.m_tiles * a.n_tiles;
   const int64_t slot = blockIdx.x / CG;
 
-  if (warp == 4) {
+  if (warp == kTmaWarp) {
     // ------------------------------- TMA --------------------------------
     if (lane == 0) {
       sm100::tma_prefetch(&a.map_x);
@@ -156,7 +160,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
         sm100::mbar_wait_cycles(full0 + 8 * (i % NS), (i / NS) & 1, kWaitLimit / 8);
     }
     __syncwarp();
-  } else if (warp == 5) {
+  } else if (warp == kMmaWarp) {
     // ------------------------------- MMA --------------------------------
     if (rank == 0) {
       const uint32_t idesc = sm100::instr_desc(DT == T2SC_DT_BF16 ? 1 : 0, BN) + (CG == 2 ? (128u >> 4) << 24 : 0u);
@@ -207,45 +211,68 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
     }
   } else {
     // ----------------------------- epilogue -----------------------------
+    // Warp w reads TMEM lanes 32 (w % 4)..; the two warps of a quadrant take
+    // turns at blocks of 64 columns.
+    const int quad = warp & 3, half = warp >> 2;
     uint8_t *stage = staging + warp * 4096;
+    float *bias = reinterpret_cast<float *>(staging + kStageBytes) + warp * 64;  // of the block at hand
     uint32_t acc = 0;
     const int crow = lane >> 3, cch = lane & 7;  // this lane's place when whole rows move: 4 rows x 8 chunks
     for (int64_t t = slot; t < ntiles; t += a.slots) {
-      const int64_t row0 = (t / a.n_tiles) * (kTileM * CG) + (int64_t)rank * kTileM + warp * 32;
+      const int64_t row0 = (t / a.n_tiles) * (kTileM * CG) + (int64_t)rank * kTileM + quad * 32;
       const int n0 = (int)(t % a.n_tiles) * BN;
       const uint32_t b = acc & 1;
+      // the first block's bias and residual come in while the tile is still computed
+      float bias0, bias1;
+      auto load_bias = [&](int col0) {
+        const int col = col0 + lane;
+        bias0 = a.bias && col < a.co ? __ldg(a.bias + col) : 0.f;
+        bias1 = a.bias && col + 32 < a.co ? __ldg(a.bias + col + 32) : 0.f;
+      };
+      uint4 res[8];
+      auto load_residual = [&](int col0) {
+        const bool whole = a.vec && col0 + 64 <= a.co;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const int64_t r = row0 + i * 4 + crow;
+          const int col = col0 + cch * 8;
+          res[i] = make_uint4(0, 0, 0, 0);
+          if (r >= a.rows) continue;
+          const char *p = a.res + (r * a.ldr + col) * 2;
+          if (whole) {
+            res[i] = *reinterpret_cast<const uint4 *>(p);
+          } else {
+            uint16_t e[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) e[j] = col + j < a.co ? *reinterpret_cast<const uint16_t *>(p + 2 * j) : 0;
+            res[i] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+          }
+        }
+      };
+      load_bias(n0 + half * 64);
+      if (a.res) load_residual(n0 + half * 64);
       if (!warp_wait(tfull0 + 8 * b, (acc >> 1) & 1, abort, a.err)) break;
       sm100::tc_fence_after();
-      const uint32_t taddr = tmem + b * BN + ((uint32_t)(warp * 32) << 16);
+      const uint32_t taddr = tmem + b * BN + ((uint32_t)(quad * 32) << 16);
 #pragma unroll 1
-      for (int c0 = 0; c0 < BN; c0 += 64) {
+      for (int c0 = half * 64; c0 < BN; c0 += 128) {
         const int col0 = n0 + c0;
-        const bool any = col0 < a.co && row0 < a.rows;
         float v[64];
         sm100::tmem_ld32(taddr + c0, reinterpret_cast<uint32_t *>(v));
         sm100::tmem_ld32(taddr + c0 + 32, reinterpret_cast<uint32_t *>(v) + 32);
-        if (a.res && any) {
+        if (a.res) {
 #pragma unroll
           for (int i = 0; i < 8; i++) {
-            const int r = i * 4 + crow, col = col0 + cch * 8;
-            uint4 u = make_uint4(0, 0, 0, 0);
-            if (row0 + r < a.rows && col < a.co) {
-              const char *p = a.res + ((row0 + r) * a.ldr + col) * 2;
-              if (a.vec && col + 8 <= a.co) {
-                u = *reinterpret_cast<const uint4 *>(p);
-              } else {
-                uint16_t e[8];
-#pragma unroll
-                for (int j = 0; j < 8; j++) e[j] = col + j < a.co ? *reinterpret_cast<const uint16_t *>(p + 2 * j) : 0;
-                u = *reinterpret_cast<uint4 *>(e);
-              }
-            }
-            *reinterpret_cast<uint4 *>(stage + r * 128 + ((cch ^ (r & 7)) << 4)) = u;
+            const int r = i * 4 + crow;
+            *reinterpret_cast<uint4 *>(stage + r * 128 + ((cch ^ (r & 7)) << 4)) = res[i];
           }
-          __syncwarp();
+          if (c0 + 128 < BN) load_residual(col0 + 128);
         }
+        bias[lane] = bias0, bias[lane + 32] = bias1;
+        if (c0 + 128 < BN) load_bias(col0 + 128);
+        __syncwarp();
         sm100::tmem_ld_wait();
-        if (c0 + 64 == BN) {  // the accumulator is read out: the next tile may use it
+        if (c0 + 128 >= BN) {  // this warp's part of the accumulator is read out
           sm100::tc_fence_before();
           __syncwarp();
           if (lane == 0) {
@@ -255,49 +282,62 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
               sm100::mbar_arrive(tempty0 + 8 * b);
           }
         }
-        if (any) {
-#pragma unroll
-          for (int c = 0; c < 8; c++) {
-            float *z = v + c * 8;
-            const int col = col0 + c * 8;
-            if (a.bias) {
-#pragma unroll
-              for (int j = 0; j < 8; j++) z[j] += col + j < a.co ? __ldg(a.bias + col + j) : 0.f;
-            }
-            if (a.act) {
-#pragma unroll
-              for (int j = 0; j < 8; j++) z[j] = activate(z[j], a.act);
-            }
-            uint4 *sp = reinterpret_cast<uint4 *>(stage + lane * 128 + ((c ^ (lane & 7)) << 4));
-            if (a.res) {
-              const uint4 u = *sp;
-              const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-              for (int j = 0; j < 4; j++) {
-                const float2 f = unpack2<DT>(w[j]);
-                z[2 * j] += f.x, z[2 * j + 1] += f.y;
-              }
-            }
-            *sp = make_uint4(pack2<DT>(z[0], z[1]), pack2<DT>(z[2], z[3]), pack2<DT>(z[4], z[5]), pack2<DT>(z[6], z[7]));
-          }
+        if (col0 >= a.co || row0 >= a.rows) {
           __syncwarp();
+          continue;
+        }
 #pragma unroll
-          for (int i = 0; i < 8; i++) {
-            const int r = i * 4 + crow, col = col0 + cch * 8;
-            if (row0 + r < a.rows && col < a.co) {
-              const uint4 u = *reinterpret_cast<const uint4 *>(stage + r * 128 + ((cch ^ (r & 7)) << 4));
-              char *p = a.y + ((row0 + r) * a.ldy + col) * 2;
-              if (a.vec && col + 8 <= a.co) {
-                *reinterpret_cast<uint4 *>(p) = u;
-              } else {
-                const uint16_t *e = reinterpret_cast<const uint16_t *>(&u);
+        for (int c = 0; c < 16; c++) {
+          const float4 w = *reinterpret_cast<const float4 *>(bias + c * 4);
+          v[4 * c] += w.x, v[4 * c + 1] += w.y, v[4 * c + 2] += w.z, v[4 * c + 3] += w.w;
+        }
+        if (a.act & T2SC_SILU) {
 #pragma unroll
-                for (int j = 0; j < 8; j++)
-                  if (col + j < a.co) *reinterpret_cast<uint16_t *>(p + 2 * j) = e[j];
-              }
+          for (int j = 0; j < 64; j++) v[j] = silu(v[j]);
+        } else if (a.act & T2SC_GELU) {
+#pragma unroll
+          for (int j = 0; j < 64; j++) v[j] = gelu_tanh(v[j]);
+        }
+#pragma unroll
+        for (int c = 0; c < 8; c++) {
+          float *z = v + c * 8;
+          uint4 *sp = reinterpret_cast<uint4 *>(stage + lane * 128 + ((c ^ (lane & 7)) << 4));
+          if (a.res) {
+            const uint4 u = *sp;
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+              const float2 f = unpack2<DT>(w[j]);
+              z[2 * j] += f.x, z[2 * j + 1] += f.y;
             }
           }
-          __syncwarp();
+          *sp = make_uint4(pack2<DT>(z[0], z[1]), pack2<DT>(z[2], z[3]), pack2<DT>(z[4], z[5]), pack2<DT>(z[6], z[7]));
+        }
+        __syncwarp();
+        const bool whole = a.vec && col0 + 64 <= a.co;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const int r = i * 4 + crow, col = col0 + cch * 8;
+          if (row0 + r >= a.rows) continue;
+          const uint4 u = *reinterpret_cast<const uint4 *>(stage + r * 128 + ((cch ^ (r & 7)) << 4));
+          char *p = a.y + ((row0 + r) * a.ldy + col) * 2;
+          if (whole) {
+            *reinterpret_cast<uint4 *>(p) = u;
+          } else {
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+              if (col + j < a.co) *reinterpret_cast<uint16_t *>(p + 2 * j) = (uint16_t)(w[j >> 1] >> (j & 1) * 16);
+          }
+        }
+        __syncwarp();
+      }
+      if (half * 64 >= BN) {  // a tile of one block: the second warps have nothing to read
+        if (lane == 0) {
+          if (CG == 2)
+            sm100::mbar_arrive_cluster(sm100::map_to_rank(tempty0 + 8 * b, 0));
+          else
+            sm100::mbar_arrive(tempty0 + 8 * b);
         }
       }
       acc++;
@@ -306,7 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
   sm100::tc_fence_before();
   __syncthreads();
   if (CG == 2) sm100::cluster_sync();  // no CTA leaves while the other may still signal it or read its tiles
-  if (warp == 5) {
+  if (warp == kMmaWarp) {
     sm100::tc_fence_after();
     if (CG == 2)
       sm100::tmem_dealloc_pair(tmem, S::kCols);
