@@ -354,6 +354,18 @@ def test_attention_many_sequences(t2sc):
     ref.assert_close(y, *ref.attention(q, k, v, lens, lens, 0.125))
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("d", [128, 96, 64, 40])
+def test_attention_two_blocks_a_cta(t2sc, dtype, d):
+    """Enough heads that a CTA takes 256 queries: with one block, two blocks
+    and a part of the second, keys from none to many blocks."""
+    g = _gen(60 + d)
+    q_lens, kv_lens = [700, 1, 0, 257, 128, 30], [650, 700, 90, 3, 129, 0]
+    q, k, v = (_normal(g, n, 40, d, dtype=dtype) for n in (sum(q_lens), sum(kv_lens), sum(kv_lens)))
+    y = t2sc.SequenceLayout(q_lens, kv_lens).attention_device(q, k, v)
+    ref.assert_close(y, *ref.attention(q, k, v, q_lens, kv_lens, d ** -0.5))
+
+
 # ---- how they are called ----
 
 def _block(t2sc, dtype, c=128, heads=2, hidden=384, cross=None, seed=50, ctx=None):

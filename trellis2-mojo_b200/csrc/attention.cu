@@ -8,6 +8,9 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <string.h>
+
+#include <algorithm>
 #include <cmath>
 
 #include "attention.h"
@@ -181,8 +184,26 @@ int t2sc_seqs_create(t2sc_ctx *ctx, const int64_t *q_offsets, const int64_t *kv_
     for (int64_t b = 0; b < batch; b++)
       h[b] = make_int4((int)s->q_off[b], (int)(s->q_off[b + 1] - s->q_off[b]), (int)s->kv_off[b],
                        (int)(s->kv_off[b + 1] - s->kv_off[b]));
-    T2SC_CUDA(cudaMalloc((void **)&s->d_seqs, h.size() * sizeof(int4)), "seqs");
-    T2SC_CUDA(cudaMemcpy(s->d_seqs, h.data(), h.size() * sizeof(int4), cudaMemcpyHostToDevice), "seqs");
+    std::vector<int4> sorted(h.begin(), h.begin() + batch);
+    std::stable_sort(sorted.begin(), sorted.end(), [](const int4 &x, const int4 &y) { return x.w > y.w; });
+    std::vector<int64_t> blocks(2 * (size_t)(batch + 1), 0);
+    for (int64_t b = 0; b < batch; b++) {
+      blocks[b + 1] = blocks[b] + ((int64_t)sorted[b].y + 255) / 256;
+      blocks[batch + 1 + b + 1] = blocks[batch + 1 + b] + ((int64_t)sorted[b].y + 127) / 128;
+      s->max_kv = std::max<int64_t>(s->max_kv, sorted[b].w);
+    }
+    s->blocks256 = blocks[batch], s->blocks128 = blocks[2 * batch + 1];
+    // one allocation: sequences in order, sorted, block counts
+    const size_t nb = (size_t)batch + 1, bytes = 2 * nb * sizeof(int4) + blocks.size() * sizeof(int64_t);
+    T2SC_CUDA(cudaMalloc((void **)&s->d_seqs, bytes), "seqs");
+    s->d_sorted = s->d_seqs + nb;
+    s->d_blocks = reinterpret_cast<int64_t *>(s->d_sorted + nb);
+    sorted.resize(nb);
+    std::vector<char> image(bytes);
+    memcpy(image.data(), h.data(), nb * sizeof(int4));
+    memcpy(image.data() + nb * sizeof(int4), sorted.data(), nb * sizeof(int4));
+    memcpy(image.data() + 2 * nb * sizeof(int4), blocks.data(), blocks.size() * sizeof(int64_t));
+    T2SC_CUDA(cudaMemcpy(s->d_seqs, image.data(), bytes, cudaMemcpyHostToDevice), "seqs");
     *out = s.release();
     return T2SC_OK;
   });
@@ -225,7 +246,8 @@ int t2sc_attention_device(t2sc_seqs *seqs, const void *q, int64_t q_stride, cons
     a.ldq = q_stride, a.ldk = k_stride, a.ldv = v_stride, a.ldo = out_stride;
     a.seqs = seqs->d_seqs, a.batch = (int)seqs->batch, a.heads = heads, a.head_dim = head_dim, a.scale = scale;
     DeviceGuard g(ctx->device);
-    return attention_simt(seqs, a, dtype, ctx->last_error);
+    return attention_tc_takes(seqs, a, dtype) ? attention_tc(seqs, a, dtype, ctx->last_error)
+                                              : attention_simt(seqs, a, dtype, ctx->last_error);
   });
 }
 
