@@ -63,7 +63,7 @@ struct Shape {
   static constexpr size_t kSmem = 1024 + (size_t)(NT + kSlots) * kTile + kExtra;
   static constexpr int kThreads = 128 * (NT + 1);
   // registers a thread of the softmax warpgroups and of the other one; launched with their mean
-  static constexpr int kSoftmaxRegs = NT == 2 ? 232 : 200, kOtherRegs = NT == 2 ? 40 : 56;
+  static constexpr int kSoftmaxRegs = NT == 2 ? 224 : 192, kOtherRegs = NT == 2 ? 56 : 64;
   static constexpr uint32_t kCols = NT == 2 ? 512 : 256;
 };
 
@@ -72,6 +72,11 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
   if (__all_sync(0xffffffffu, ok)) return true;
   if (!ok) ok = sm100::mbar_wait_bounded(bar, parity, abort, err, kDevErrTimeout, kWaitLimit);
   return __all_sync(0xffffffffu, ok);
+}
+
+template <class T>
+__device__ __forceinline__ T uniform(T v) {
+  return __shfl_sync(0xffffffffu, v, 0);
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -102,14 +107,15 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
   uint8_t *ring = smem + NT * S::kTile;
   float *row_m = reinterpret_cast<float *>(ring + NS * S::kTile), *row_l = row_m + 128;  // split sums
   uint64_t *bars = reinterpret_cast<uint64_t *>(row_l + 128);
-  // bars: q_full[NT], s_full[NT], p_full[NT], o_full[NT], full[NS], empty[NS]
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 4 * NT + 2 * NS);
+  // bars: q_full[NT], s_full[NT], p_full[NT], o_full[NT], full[NS], empty[NS], v_dirty, v_clean
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 4 * NT + 2 * NS + 2);
   volatile int *abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
   int *where = reinterpret_cast<int *>(tmem_slot + 2);  // the CTA's work
   const uint32_t qsm = sm100::smem_u32(smem), rsm = sm100::smem_u32(ring), bar0 = sm100::smem_u32(bars);
   const uint32_t q_full = bar0, s_full = q_full + 8 * NT, p_full = s_full + 8 * NT, o_full = p_full + 8 * NT;
-  const uint32_t full0 = o_full + 8 * NT, empty0 = full0 + 8 * NS;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wg = warp >> 2;
+  const uint32_t full0 = o_full + 8 * NT, empty0 = full0 + 8 * NS, v_dirty = empty0 + 8 * NS, v_clean = v_dirty + 8;
+  // lane 0's value is every lane's: the compiler may keep it in uniform registers
+  const int warp = uniform((int)threadIdx.x >> 5), lane = threadIdx.x & 31, wg = warp >> 2;
   constexpr int kTmaWarp = 4 * NT, kMmaWarp = 4 * NT + 1;
 
   if (threadIdx.x == 0) {
@@ -123,6 +129,8 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
       sm100::mbar_init(full0 + 8 * s, 1);
       sm100::mbar_init(empty0 + 8 * s, 1);
     }
+    sm100::mbar_init(v_dirty, 1);
+    sm100::mbar_init(v_clean, 1);
     *abort = 0;
     sm100::fence_mbar_init();
     // the CTA's sequence, head and query block: blocks of a head are neighbours, heads of a sequence follow
@@ -151,14 +159,16 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
   sm100::tc_fence_before();
   __syncthreads();
   sm100::tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
-  const int head = where[0], q0 = where[1], here = min(where[2], NT * kBQ), kv0 = where[3], kv_len = where[4];
-  const int split = a.splits > 1 ? (int)sm100::cluster_rank() : 0;
+  const uint32_t tmem = uniform(*tmem_slot);
+  const int head = uniform(where[0]), q0 = uniform(where[1]), here = min(uniform(where[2]), NT * kBQ), kv0 = uniform(where[3]),
+            kv_len = uniform(where[4]);
+  const int split = a.splits > 1 ? uniform((int)sm100::cluster_rank()) : 0;
   const int all_tiles = (kv_len + kBK - 1) / kBK, per = (all_tiles + a.splits - 1) / a.splits;
   const int t0 = min(split * per, all_tiles), n = min(t0 + per, all_tiles) - t0;  // this CTA's key blocks
   const int nt = NT == 2 && here > kBQ ? 2 : 1;                                     // query blocks with rows
   const uint32_t s_tmem = tmem, o_tmem = tmem + NT * 128;
   const int ksteps = (a.head_dim + 15) / 16;
+  const bool tail = n > 0 && t0 + n == all_tiles && kv_len % 16 != 0;  // the last block's keys end inside a product step
 
   if (wg == NT) {
     sm100::regs_down<S::kOtherRegs>();
@@ -196,77 +206,85 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
       __syncwarp();
     } else if (warp == kMmaWarp && n > 0) {
       // ------------------------------- MMA --------------------------------
-      constexpr uint32_t fmt = DT == T2SC_DT_BF16 ? 1 : 0;
-      const uint32_t idesc_s = sm100::instr_desc(fmt, kBK);
-      const uint32_t idesc_o = sm100::instr_desc(fmt, ksteps * 16) | sm100::kInstrBMnMajor;
-      uint32_t it = 0;  // ring position of the next block to consume
-      bool ok = true;
-      auto wait_slot = [&]() {
-        ok = ok && warp_wait(full0 + 8 * (it % NS), (it / NS) & 1, abort, a.err);
-        sm100::tc_fence_after();
-      };
-      auto scores = [&](int i, uint32_t slot) {
-        const uint64_t dq = sm100::smem_desc(qsm + i * S::kTile, 128), dk = sm100::smem_desc(rsm + slot * S::kTile, 128);
-#pragma unroll
-        for (int kk = 0; kk < DP / 16; kk++) {
-          if (kk < ksteps) {
-            const uint64_t off = (uint64_t)((kk >> 2) * 16384 + (kk & 3) * 32) >> 4;
-            sm100::mma_f16_elect(s_tmem + i * 128, dq + off, dk + off, idesc_s, kk > 0);
-          }
-        }
-        sm100::mma_commit_elect(s_full + 8 * i);
-      };
-      for (int i = 0; i < nt && ok; i++) {
-        ok = warp_wait(q_full + 8 * i, 0, abort, a.err);
-        if (i == 0) wait_slot();
-        if (ok) scores(i, 0);
-      }
-      if (ok) sm100::mma_commit_elect(empty0);
-      it = 1;
-      for (int j = 0; j < n && ok; j++) {
-        wait_slot();  // V of block j
-        const uint32_t vslot = it % NS, kslot = (it + 1) % NS;
-        const int valid = min(kv_len - (t0 + j) * kBK, kBK), steps = (valid + 15) / 16;
-        if (ok && valid < steps * 16) {
-          uint8_t *v = ring + vslot * S::kTile;
-          for (int i = lane; i < (steps * 16 - valid) * 8 * kSub; i += 32) {
-            const int h = i % kSub, r = i / kSub;
-            *reinterpret_cast<uint4 *>(v + h * 16384 + valid * 128 + r * 16) = make_uint4(0, 0, 0, 0);
-          }
-          sm100::fence_proxy_async_smem();
-          __syncwarp();
-        }
-        for (int i = 0; i < nt && ok; i++) {
-          ok = warp_wait(p_full + 8 * i, j & 1, abort, a.err);
-          if (!ok) break;
+      // One thread waits and issues: this role is what everything waits for,
+      // and a whole warp's waits and votes, or an election at every
+      // instruction, cost it ~100 clocks each (measured per block of keys and
+      // two query blocks, head_dim 128: 5000 clocks with elections, 4000
+      // with one issuing lane between warp-wide waits).
+      if (sm100::elect_one()) {
+        constexpr uint32_t fmt = DT == T2SC_DT_BF16 ? 1 : 0;
+        const uint32_t idesc_s = sm100::instr_desc(fmt, kBK);
+        const uint32_t idesc_o = sm100::instr_desc(fmt, ksteps * 16) | sm100::kInstrBMnMajor;
+        const uint64_t dq0 = sm100::smem_desc(qsm, 128), dk0 = sm100::smem_desc(rsm, 128), dv0 = sm100::smem_desc_mn(rsm, 16384);
+        uint32_t slot = 0, phase = 0;  // ring position of the next block to consume
+        bool ok = true;
+        auto wait = [&](uint32_t bar, uint32_t parity) {
+          ok = ok && sm100::mbar_wait_bounded(bar, parity, abort, a.err, kDevErrTimeout, kWaitLimit);
           sm100::tc_fence_after();
-          const uint64_t dv = sm100::smem_desc_mn(rsm + vslot * S::kTile, 16384);
-#pragma unroll
-          for (int kk = 0; kk < kBK / 16; kk++)
-            if (kk < steps)
-              sm100::mma_f16_ts_elect(o_tmem + i * DP, s_tmem + i * 128 + kk * 8, dv + (uint64_t)(kk * 2048 >> 4), idesc_o,
-                                      j + kk > 0);
-          if (i == nt - 1) sm100::mma_commit_elect(empty0 + 8 * vslot);
-          if (j + 1 < n) {
-            if (i == 0) {  // K of block j + 1
-              it++;
-              wait_slot();
-            }
-            if (!ok) break;
-            scores(i, kslot);
-            if (i == nt - 1) sm100::mma_commit_elect(empty0 + 8 * kslot);
-          } else {
-            sm100::mma_commit_elect(o_full + 8 * i);
+        };
+        auto next = [&]() {
+          if (++slot == NS) slot = 0, phase ^= 1;
+        };
+        auto scores = [&](int i, uint32_t at) {
+          const uint64_t dq = dq0 + (uint64_t)(i * S::kTile >> 4), dk = dk0 + (uint64_t)(at * S::kTile >> 4);
+#pragma unroll 1
+          for (int kk = 0; kk < ksteps; kk++) {
+            const uint64_t off = (uint64_t)((kk >> 2) * 16384 + (kk & 3) * 32) >> 4;
+            sm100::mma_f16(s_tmem + i * 128, dq + off, dk + off, idesc_s, kk > 0);
           }
+          sm100::mma_commit(s_full + 8 * i);
+        };
+        wait(full0, 0);
+        for (int i = 0; i < nt && ok; i++) {
+          wait(q_full + 8 * i, 0);
+          if (ok) scores(i, 0);
         }
-        it++;
+        if (ok) sm100::mma_commit(empty0);
+        next();
+        for (int j = 0; j < n && ok; j++) {
+          const uint32_t vslot = slot;
+          wait(full0 + 8 * vslot, phase);
+          if (tail && j == n - 1) sm100::mbar_arrive(v_dirty);
+          next();
+          const uint32_t kslot = slot;
+          const int steps = min((kv_len - (t0 + j) * kBK + 15) / 16, kBK / 16);
+          const uint64_t dv = dv0 + (uint64_t)(vslot * S::kTile >> 4);
+          for (int i = 0; i < nt && ok; i++) {
+            wait(p_full + 8 * i, j & 1);
+            if (i == 0 && tail && j == n - 1) wait(v_clean, 0);
+            if (!ok) break;
+#pragma unroll 1
+            for (int kk = 0; kk < steps; kk++)
+              sm100::mma_f16_ts(o_tmem + i * DP, s_tmem + i * 128 + kk * 8, dv + (uint64_t)(kk * 2048 >> 4), idesc_o, j + kk > 0);
+            if (i == nt - 1) sm100::mma_commit(empty0 + 8 * vslot);
+            if (j + 1 < n) {
+              if (i == 0) wait(full0 + 8 * kslot, phase);  // K of block j + 1
+              if (!ok) break;
+              scores(i, kslot);
+              if (i == nt - 1) sm100::mma_commit(empty0 + 8 * kslot);
+            } else {
+              sm100::mma_commit(o_full + 8 * i);
+            }
+          }
+          next();
+        }
+        // all issued MMAs retire before TMEM and shared memory are given up: in
+        // the regular case o_full told so; after an abort wait for a last commit
+        if (!ok) {
+          sm100::mma_commit(o_full);
+          sm100::mbar_wait_cycles(o_full, 0, kWaitLimit / 8);
+        }
       }
-      // all issued MMAs retire before TMEM and shared memory are given up: in
-      // the regular case o_full told so; after an abort wait for a last commit
-      if (!ok) {
-        sm100::mma_commit_elect(o_full);
-        if (lane == 0) sm100::mbar_wait_cycles(o_full, 0, kWaitLimit / 8);
+    } else if (warp == kMmaWarp + 1 && tail) {
+      // zeros the V rows behind the last key, up to the 16 that a product step takes, once the MMA thread has seen the block
+      const int valid = kv_len % kBK;
+      if (warp_wait(v_dirty, 0, abort, a.err)) {
+        uint8_t *v = ring + (2 * n - 1) % NS * S::kTile + valid * 128;
+        for (int x = lane; x < ((valid + 15) / 16 * 16 - valid) * 8 * kSub; x += 32)
+          *reinterpret_cast<uint4 *>(v + x % kSub * 16384 + x / kSub * 16) = make_uint4(0, 0, 0, 0);
+        sm100::fence_proxy_async_smem();
         __syncwarp();
+        if (lane == 0) sm100::mbar_arrive(v_clean);
       }
     }
     __syncwarp();
@@ -326,19 +344,25 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
             }
           }
           const float base = kLift - (m == -INFINITY ? 0.f : m * a.c);
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          const uint64_t c2 = sm100::pack_f32x2(a.c, a.c), base2 = sm100::pack_f32x2(base, base);
+          uint64_t sum[2] = {0, 0};
 #pragma unroll
           for (int q = 0; q < 128; q += 32) {
             uint32_t p[16];
 #pragma unroll
             for (int z = 0; z < 32; z += 2) {
-              const float p0 = ex2(fmaf(s[q + z], a.c, base)), p1 = ex2(fmaf(s[q + z + 1], a.c, base));
-              sum[z & 2] += p0, sum[(z & 2) + 1] += p1;
+              const uint64_t x = sm100::fma_f32x2(sm100::pack_f32x2(s[q + z], s[q + z + 1]), c2, base2);
+              float p0, p1;
+              sm100::unpack_f32x2(x, p0, p1);
+              p0 = ex2(p0), p1 = ex2(p1);
+              sum[z >> 1 & 1] = sm100::add_f32x2(sum[z >> 1 & 1], sm100::pack_f32x2(p0, p1));
               p[z / 2] = pack2<DT>(p0, p1);
             }
             sm100::tmem_st16(st + q / 2, p);
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          float l0, l1;
+          sm100::unpack_f32x2(sm100::add_f32x2(sum[0], sum[1]), l0, l1);
+          l += l0 + l1;
           sm100::tmem_st_wait();
         }
         sm100::tc_fence_before();
