@@ -2,17 +2,25 @@
 // 16 bytes and head dims that are multiples of 8 up to 128.
 //
 // A CTA owns NT blocks of 128 queries of one head and walks its sequence's
-// keys 128 at a time. TMA brings the query blocks once and the K and V blocks
+// keys. TMA brings the query blocks once and blocks of 128 K and V rows
 // through a ring of shared-memory slots (heads are a dimension of the tensor
-// map: channels past head_dim read as zero). One warp issues the products:
+// map: channels past head_dim read as zero). One thread issues the
+// products, for a unit of 64 keys at a time:
 //   S = Q K^T   tcgen05.mma, both operands from shared memory, f32 S in TMEM
 //   O += P V    A = P from TMEM, B = V as it lies (channels contiguous:
 //               MN-major), f32 O in TMEM
 // and a warpgroup per query block, one thread a row, turns S into P in
 // between: p = 2^(s c - m c), c = scale log2(e), m the running maximum, P
-// rounded to the 16-bit type and written over S. With two blocks (NT = 2) one
-// block's softmax runs under the other's products, and K and V are read for
-// 256 queries; with one, two CTAs share an SM to the same end.
+// rounded to the 16-bit type and written over S.
+//
+// A query block has two S buffers of 64 columns, so that the scores of the
+// next unit are there when the softmax of this one is done: O takes up to 128
+// columns, two blocks fill the 512 of an SM. (With one buffer of 128 keys a
+// block waits for P V and the next Q K^T after every softmax: 3650 clocks a
+// block of 128 keys and two query blocks at head_dim 128, of which the
+// softmax takes 1850.) With two blocks (NT = 2) one's softmax also runs under
+// the other's products, and K and V are read for 256 queries; with one, two
+// CTAs share an SM to the same end.
 //
 // The running maximum that P is relative to is only raised when a row's
 // maximum has grown by more than a factor 2^kSlack (then l and O are
@@ -41,7 +49,7 @@
 namespace t2sc {
 namespace {
 
-constexpr int kBQ = 128, kBK = 128;
+constexpr int kBQ = 128, kBK = 128, kUnit = 64;
 constexpr long long kWaitLimit = 4000000000ll;  // ~2 s of SM clocks
 
 struct TcArgs {
@@ -62,9 +70,12 @@ struct Shape {
   static constexpr int kExtra = 2048;         // barriers, m and l of the rows
   static constexpr size_t kSmem = 1024 + (size_t)(NT + kSlots) * kTile + kExtra;
   static constexpr int kThreads = 128 * (NT + 1);
-  // registers a thread of the softmax warpgroups and of the other one; launched with their mean
-  static constexpr int kSoftmaxRegs = NT == 2 ? 224 : 192, kOtherRegs = NT == 2 ? 56 : 64;
   static constexpr uint32_t kCols = NT == 2 ? 512 : 256;
+  // Query blocks whose units join one barrier. At head_dim 128 the products
+  // bound the kernel and every wait of their thread counts: both blocks join
+  // one. Below, the exponentials do, and the two blocks' softmaxes should not
+  // want them at the same time: one each (23024 tokens, 16 x 64: JOINED ms).
+  static constexpr int kGroups = DP == 128 ? 1 : NT;
 };
 
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *abort, int *err) {
@@ -107,32 +118,24 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
   uint8_t *ring = smem + NT * S::kTile;
   float *row_m = reinterpret_cast<float *>(ring + NS * S::kTile), *row_l = row_m + 128;  // split sums
   uint64_t *bars = reinterpret_cast<uint64_t *>(row_l + 128);
-  // bars: q_full[NT], s_full[NT], p_full[NT], o_full[NT], full[NS], empty[NS], v_dirty, v_clean
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 4 * NT + 2 * NS + 2);
+  // bars: q_full[NT], s_full[NT][2], o_prev[NT], o_full[NT], ready[kGroups][2], full[NS], empty[NS]
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 5 * NT + 2 * S::kGroups + 2 * NS);
   volatile int *abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
   int *where = reinterpret_cast<int *>(tmem_slot + 2);  // the CTA's work
   const uint32_t qsm = sm100::smem_u32(smem), rsm = sm100::smem_u32(ring), bar0 = sm100::smem_u32(bars);
-  const uint32_t q_full = bar0, s_full = q_full + 8 * NT, p_full = s_full + 8 * NT, o_full = p_full + 8 * NT;
-  const uint32_t full0 = o_full + 8 * NT, empty0 = full0 + 8 * NS, v_dirty = empty0 + 8 * NS, v_clean = v_dirty + 8;
+  const uint32_t q_full = bar0, s_full = q_full + 8 * NT, o_prev = s_full + 16 * NT, o_full = o_prev + 8 * NT;
+  const uint32_t ready = o_full + 8 * NT, full0 = ready + 16 * S::kGroups, empty0 = full0 + 8 * NS;
   // lane 0's value is every lane's: the compiler may keep it in uniform registers
   const int warp = uniform((int)threadIdx.x >> 5), lane = threadIdx.x & 31, wg = warp >> 2;
-  constexpr int kTmaWarp = 4 * NT, kMmaWarp = 4 * NT + 1;
+  constexpr int kTmaWarp = 4 * NT, kMmaWarp = 4 * NT + 1, kFeedWarp = 4 * NT + 2;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < NT; i++) {
       sm100::mbar_init(q_full + 8 * i, 1);
-      sm100::mbar_init(s_full + 8 * i, 1);
-      sm100::mbar_init(p_full + 8 * i, 4);
+      for (int b = 0; b < 2; b++) sm100::mbar_init(s_full + 16 * i + 8 * b, 1);
+      sm100::mbar_init(o_prev + 8 * i, 1);
       sm100::mbar_init(o_full + 8 * i, 1);
     }
-    for (int s = 0; s < NS; s++) {
-      sm100::mbar_init(full0 + 8 * s, 1);
-      sm100::mbar_init(empty0 + 8 * s, 1);
-    }
-    sm100::mbar_init(v_dirty, 1);
-    sm100::mbar_init(v_clean, 1);
-    *abort = 0;
-    sm100::fence_mbar_init();
     // the CTA's sequence, head and query block: blocks of a head are neighbours, heads of a sequence follow
     const int64_t id = blockIdx.x / a.splits;
     int lo = 0, hi = a.batch - 1;
@@ -151,6 +154,16 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
     where[2] = seq.y - block * (NT * kBQ);          // query rows left
     where[3] = seq.z;
     where[4] = seq.w;
+    for (int s = 0; s < NS; s++) {
+      sm100::mbar_init(full0 + 8 * s, 1);
+      sm100::mbar_init(empty0 + 8 * s, 1);
+    }
+    // a unit's P (4 warps a query block), and its V and the next K
+    const bool second = NT == 2 && where[2] > kBQ;
+    for (int g = 0; g < S::kGroups; g++)
+      for (int b = 0; b < 2; b++) sm100::mbar_init(ready + 16 * g + 8 * b, (second && S::kGroups == 1 ? 8 : 4) + 1);
+    *abort = 0;
+    sm100::fence_mbar_init();
   }
   if (warp == kMmaWarp) {
     sm100::tmem_alloc(sm100::smem_u32(tmem_slot), S::kCols);
@@ -165,13 +178,12 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
   const int split = a.splits > 1 ? uniform((int)sm100::cluster_rank()) : 0;
   const int all_tiles = (kv_len + kBK - 1) / kBK, per = (all_tiles + a.splits - 1) / a.splits;
   const int t0 = min(split * per, all_tiles), n = min(t0 + per, all_tiles) - t0;  // this CTA's key blocks
+  const int keys = min(kv_len - t0 * kBK, n * kBK), units = (keys + kUnit - 1) / kUnit;
   const int nt = NT == 2 && here > kBQ ? 2 : 1;                                     // query blocks with rows
   const uint32_t s_tmem = tmem, o_tmem = tmem + NT * 128;
   const int ksteps = (a.head_dim + 15) / 16;
-  const bool tail = n > 0 && t0 + n == all_tiles && kv_len % 16 != 0;  // the last block's keys end inside a product step
 
   if (wg == NT) {
-    sm100::regs_down<S::kOtherRegs>();
     if (warp == kTmaWarp && n > 0) {
       // ------------------------------- TMA --------------------------------
       bool ok = true;
@@ -206,67 +218,79 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
       __syncwarp();
     } else if (warp == kMmaWarp && n > 0) {
       // ------------------------------- MMA --------------------------------
-      // One thread waits and issues: this role is what everything waits for,
-      // and a whole warp's waits and votes, or an election at every
-      // instruction, cost it ~100 clocks each (measured per block of keys and
-      // two query blocks, head_dim 128: 5000 clocks with elections, 4000
-      // with one issuing lane between warp-wide waits).
+      // One thread waits and issues. A wait, even on a phase that has
+      // completed, stands behind the thread's own products in the queue (~150
+      // clocks), so there is one a unit: the barrier that counts the warps
+      // that have written P and the feeding warp that has seen the loads. (A
+      // thread for each query block hides its waits under the other's
+      // products, but the exponentials of the softmax warps on its part of
+      // the SM wait behind the products in the same queue: 1250 clocks later
+      // than the others.)
       if (sm100::elect_one()) {
         constexpr uint32_t fmt = DT == T2SC_DT_BF16 ? 1 : 0;
-        const uint32_t idesc_s = sm100::instr_desc(fmt, kBK);
+        const uint32_t idesc_s = sm100::instr_desc(fmt, kUnit);
         const uint32_t idesc_o = sm100::instr_desc(fmt, ksteps * 16) | sm100::kInstrBMnMajor;
-        const uint64_t dq0 = sm100::smem_desc(qsm, 128), dk0 = sm100::smem_desc(rsm, 128), dv0 = sm100::smem_desc_mn(rsm, 16384);
-        uint32_t slot = 0, phase = 0;  // ring position of the next block to consume
+        // descriptors: both operands' high words are the same (1024 bytes between 8-row atoms, 128-byte swizzle)
+        const uint64_t dq0 = sm100::smem_desc(qsm, 128);
+        const uint32_t hi = (uint32_t)(dq0 >> 32), q_lo = (uint32_t)dq0, k_lo = (uint32_t)sm100::smem_desc(rsm, 128),
+                       v_lo = (uint32_t)sm100::smem_desc_mn(rsm, 16384);
+        constexpr uint32_t kTile16 = S::kTile >> 4, kUnit16 = kUnit * 128 >> 4;
         bool ok = true;
         auto wait = [&](uint32_t bar, uint32_t parity) {
           ok = ok && sm100::mbar_wait_bounded(bar, parity, abort, a.err, kDevErrTimeout, kWaitLimit);
           sm100::tc_fence_after();
         };
-        auto next = [&]() {
-          if (++slot == NS) slot = 0, phase ^= 1;
-        };
-        auto scores = [&](int i, uint32_t at) {
-          const uint64_t dq = dq0 + (uint64_t)(i * S::kTile >> 4), dk = dk0 + (uint64_t)(at * S::kTile >> 4);
+        auto scores = [&](int i, int b, uint32_t kslot, bool done) {  // S into buffer b = the unit's half of its block
+          const uint32_t dq = q_lo + i * kTile16, dk = k_lo + kslot * kTile16 + b * kUnit16, d = s_tmem + i * 128 + b * kUnit;
+          if (ksteps == DP / 16) {
+#pragma unroll
+            for (int kk = 0; kk < DP / 16; kk++)
+              sm100::mma_f16_lo(d, dq + (kk >> 2) * 1024 + (kk & 3) * 2, dk + (kk >> 2) * 1024 + (kk & 3) * 2, hi, idesc_s, kk > 0);
+          } else {
 #pragma unroll 1
-          for (int kk = 0; kk < ksteps; kk++) {
-            const uint64_t off = (uint64_t)((kk >> 2) * 16384 + (kk & 3) * 32) >> 4;
-            sm100::mma_f16(s_tmem + i * 128, dq + off, dk + off, idesc_s, kk > 0);
+            for (int kk = 0; kk < ksteps; kk++)
+              sm100::mma_f16_lo(d, dq + (kk >> 2) * 1024 + (kk & 3) * 2, dk + (kk >> 2) * 1024 + (kk & 3) * 2, hi, idesc_s, kk > 0);
           }
-          sm100::mma_commit(s_full + 8 * i);
+          sm100::mma_commit(s_full + 16 * i + 8 * b);
+          if (done && i == nt - 1) sm100::mma_commit(empty0 + 8 * kslot);  // the block's last unit, for the last query block
+        };
+        // ring position of the V block at hand, and of the K block behind it
+        uint32_t vslot = 1 % NS, kslot = 2 % NS;
+        auto unit = [&](int u, int b, bool last) {
+          const uint32_t dv = v_lo + vslot * kTile16 + b * kUnit16;
+#pragma unroll
+          for (int i = 0; i < NT; i++) {
+            if (i >= nt) break;
+            if (i < S::kGroups) wait(ready + 16 * i + 8 * b, (u >> 1) & 1);
+            if (!ok) break;
+            const uint32_t o = o_tmem + i * DP, p = s_tmem + i * 128 + b * kUnit;
+            if (!last) {
+#pragma unroll
+              for (int kk = 0; kk < kUnit / 16; kk++) sm100::mma_f16_ts_lo(o, p + kk * 8, dv + kk * 128, hi, idesc_o, u + kk > 0);
+            } else {
+              const int steps = (keys - u * kUnit + 15) / 16;
+#pragma unroll 1
+              for (int kk = 0; kk < steps; kk++) sm100::mma_f16_ts_lo(o, p + kk * 8, dv + kk * 128, hi, idesc_o, u + kk > 0);
+            }
+            if (i == nt - 1 && (b == 1 || last)) sm100::mma_commit(empty0 + 8 * vslot);
+            if (u + 2 < units)
+              scores(i, b, kslot, b == 1 || u + 2 == units - 1);
+            else
+              sm100::mma_commit((last ? o_full : o_prev) + 8 * i);
+          }
         };
         wait(full0, 0);
-        for (int i = 0; i < nt && ok; i++) {
-          wait(q_full + 8 * i, 0);
-          if (ok) scores(i, 0);
-        }
-        if (ok) sm100::mma_commit(empty0);
-        next();
-        for (int j = 0; j < n && ok; j++) {
-          const uint32_t vslot = slot;
-          wait(full0 + 8 * vslot, phase);
-          if (tail && j == n - 1) sm100::mbar_arrive(v_dirty);
-          next();
-          const uint32_t kslot = slot;
-          const int steps = min((kv_len - (t0 + j) * kBK + 15) / 16, kBK / 16);
-          const uint64_t dv = dv0 + (uint64_t)(vslot * S::kTile >> 4);
-          for (int i = 0; i < nt && ok; i++) {
-            wait(p_full + 8 * i, j & 1);
-            if (i == 0 && tail && j == n - 1) wait(v_clean, 0);
-            if (!ok) break;
-#pragma unroll 1
-            for (int kk = 0; kk < steps; kk++)
-              sm100::mma_f16_ts(o_tmem + i * DP, s_tmem + i * 128 + kk * 8, dv + (uint64_t)(kk * 2048 >> 4), idesc_o, j + kk > 0);
-            if (i == nt - 1) sm100::mma_commit(empty0 + 8 * vslot);
-            if (j + 1 < n) {
-              if (i == 0) wait(full0 + 8 * kslot, phase);  // K of block j + 1
-              if (!ok) break;
-              scores(i, kslot);
-              if (i == nt - 1) sm100::mma_commit(empty0 + 8 * kslot);
-            } else {
-              sm100::mma_commit(o_full + 8 * i);
-            }
+        for (int u = 0; u < min(units, 2); u++)
+          for (int i = 0; i < nt; i++) {
+            if (u == 0) wait(q_full + 8 * i, 0);
+            if (ok) scores(i, u, 0, u == 1 || units == 1);
           }
-          next();
+#pragma unroll 1
+        for (int u = 0; u < units && ok; u += 2) {
+          unit(u, 0, u + 1 >= units);
+          if (u + 1 < units && ok) unit(u + 1, 1, u + 2 >= units);
+          vslot = kslot + 1 == NS ? 0 : kslot + 1;
+          kslot = vslot + 1 == NS ? 0 : vslot + 1;
         }
         // all issued MMAs retire before TMEM and shared memory are given up: in
         // the regular case o_full told so; after an abort wait for a last commit
@@ -275,16 +299,34 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
           sm100::mbar_wait_cycles(o_full, 0, kWaitLimit / 8);
         }
       }
-    } else if (warp == kMmaWarp + 1 && tail) {
-      // zeros the V rows behind the last key, up to the 16 that a product step takes, once the MMA thread has seen the block
-      const int valid = kv_len % kBK;
-      if (warp_wait(v_dirty, 0, abort, a.err)) {
-        uint8_t *v = ring + (2 * n - 1) % NS * S::kTile + valid * 128;
-        for (int x = lane; x < ((valid + 15) / 16 * 16 - valid) * 8 * kSub; x += 32)
-          *reinterpret_cast<uint4 *>(v + x % kSub * 16384 + x / kSub * 16) = make_uint4(0, 0, 0, 0);
-        sm100::fence_proxy_async_smem();
+    } else if (warp == kFeedWarp && n > 0) {
+      // ------------------------------- feed -------------------------------
+      // Joins a unit's barrier once its V block and the K block of two units
+      // on are there, and zeros the V rows behind the last key, up to the 16
+      // that a product step takes.
+      // Every load is waited for in turn, the first K too: a wait for a slot's
+      // next phase is only good once the one before it has completed.
+      const bool first = warp_wait(full0, 0, abort, a.err);
+      for (int u = 0; u < units && first; u++) {
+        bool over = true;  // the barrier's last use, two units ago
+        for (int g = 0; g < min(S::kGroups, nt); g++)
+          over = over && (u < 2 || warp_wait(ready + 16 * g + 8 * (u & 1), ((u - 2) >> 1) & 1, abort, a.err));
+        if (!over) break;
+        if (!(u & 1)) {
+          const uint32_t v = u + 1, k = u + 2;  // loads: block j's K is number 2 j, its V 2 j + 1
+          if (!warp_wait(full0 + 8 * (v % NS), (v / NS) & 1, abort, a.err)) break;
+          if (u + 2 < units && !warp_wait(full0 + 8 * (k % NS), (k / NS) & 1, abort, a.err)) break;
+          const int valid = keys - u * kUnit;  // of this block's
+          if (valid < kBK && valid % 16) {
+            uint8_t *rows = ring + v % NS * S::kTile + valid * 128;
+            for (int x = lane; x < (16 - valid % 16) * 8 * kSub; x += 32)
+              *reinterpret_cast<uint4 *>(rows + x % kSub * 16384 + x / kSub * 16) = make_uint4(0, 0, 0, 0);
+            sm100::fence_proxy_async_smem();
+          }
+        }
         __syncwarp();
-        if (lane == 0) sm100::mbar_arrive(v_clean);
+        if (lane == 0)
+          for (int g = 0; g < min(S::kGroups, nt); g++) sm100::mbar_arrive(ready + 16 * g + 8 * (u & 1));
       }
     }
     __syncwarp();
@@ -294,7 +336,6 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
     }
   } else {
     // ----------------------------- softmax ------------------------------
-    sm100::regs_up<S::kSoftmaxRegs>();
     const int i = wg, quad = warp & 3;
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
     const uint32_t st = s_tmem + i * 128 + lanes, ot = o_tmem + i * DP + lanes;
@@ -302,27 +343,28 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     if (i < nt) {
-      for (int j = 0; j < n; j++) {
-        if (!warp_wait(s_full + 8 * i, j & 1, abort, a.err)) {
+      for (int u = 0; u < units; u++) {
+        const uint32_t b = u & 1, su = st + b * kUnit;
+        if (!warp_wait(s_full + 16 * i + 8 * b, (u >> 1) & 1, abort, a.err)) {
           ok = false;
           break;
         }
         sm100::tc_fence_after();
         if (live) {
-          float s[128];
-#pragma unroll
-          for (int q = 0; q < 4; q++) sm100::tmem_ld32(st + q * 32, reinterpret_cast<uint32_t *>(s) + q * 32);
+          float s[kUnit];
+          sm100::tmem_ld32(su, reinterpret_cast<uint32_t *>(s));
+          sm100::tmem_ld32(su + 32, reinterpret_cast<uint32_t *>(s) + 32);
           sm100::tmem_ld_wait();
-          const int valid = kv_len - (t0 + j) * kBK;
-          if (valid < kBK) {
+          const int valid = keys - u * kUnit;
+          if (valid < kUnit) {
 #pragma unroll
-            for (int q = 0; q < 128; q++) s[q] = q < valid ? s[q] : -INFINITY;
+            for (int q = 0; q < kUnit; q++) s[q] = q < valid ? s[q] : -INFINITY;
           }
           float top[4];
 #pragma unroll
           for (int q = 0; q < 4; q++) top[q] = fmaxf(s[q], s[q + 4]);
 #pragma unroll
-          for (int q = 8; q < 128; q += 4)
+          for (int q = 8; q < kUnit; q += 4)
 #pragma unroll
             for (int z = 0; z < 4; z++) top[z] = fmaxf(top[z], s[q + z]);
           const float mn = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), m);
@@ -330,8 +372,15 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
             const float f = mn > m ? ex2((m - mn) * a.c) : 1.f;
             m = mn;
             l *= f;
-            if (j > 0) {  // S of this block was committed after the last P V: O is complete
-#pragma unroll
+            if (u > 0) {
+              // O is complete once P V of the last unit is: the next unit's scores were issued behind it
+              if (u + 1 < units)
+                ok = warp_wait(s_full + 16 * i + 8 * (b ^ 1), ((u + 1) >> 1) & 1, abort, a.err);
+              else
+                ok = warp_wait(o_prev + 8 * i, 0, abort, a.err);
+              if (!ok) break;
+              sm100::tc_fence_after();
+#pragma unroll 1
               for (int q = 0; q < DP; q += 32) {
                 uint32_t o[32];
                 sm100::tmem_ld32(ot + q, o);
@@ -347,18 +396,17 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
           const uint64_t c2 = sm100::pack_f32x2(a.c, a.c), base2 = sm100::pack_f32x2(base, base);
           uint64_t sum[2] = {0, 0};
 #pragma unroll
-          for (int q = 0; q < 128; q += 32) {
+          for (int q = 0; q < kUnit; q += 32) {
             uint32_t p[16];
 #pragma unroll
             for (int z = 0; z < 32; z += 2) {
-              const uint64_t x = sm100::fma_f32x2(sm100::pack_f32x2(s[q + z], s[q + z + 1]), c2, base2);
               float p0, p1;
-              sm100::unpack_f32x2(x, p0, p1);
+              sm100::unpack_f32x2(sm100::fma_f32x2(sm100::pack_f32x2(s[q + z], s[q + z + 1]), c2, base2), p0, p1);
               p0 = ex2(p0), p1 = ex2(p1);
               sum[z >> 1 & 1] = sm100::add_f32x2(sum[z >> 1 & 1], sm100::pack_f32x2(p0, p1));
               p[z / 2] = pack2<DT>(p0, p1);
             }
-            sm100::tmem_st16(st + q / 2, p);
+            sm100::tmem_st16(su + q / 2, p);
           }
           float l0, l1;
           sm100::unpack_f32x2(sm100::add_f32x2(sum[0], sum[1]), l0, l1);
@@ -367,7 +415,7 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
         }
         sm100::tc_fence_before();
         __syncwarp();
-        if (lane == 0) sm100::mbar_arrive(p_full + 8 * i);
+        if (lane == 0) sm100::mbar_arrive(ready + (S::kGroups == 1 ? 0 : 16 * i) + 8 * b);
       }
       if (n > 0 && ok) ok = warp_wait(o_full + 8 * i, 0, abort, a.err);
       sm100::tc_fence_after();
@@ -464,16 +512,6 @@ int launch(t2sc_seqs *s, const AttnArgs &a, int splits, std::string &err) {
   using S = Shape<DP, NT>;
   t2sc_ctx *ctx = s->ctx;
   auto kernel = attention_tc_kernel<DT, DP, NT>;
-  static int regs = 0;  // registers a thread the kernel is launched with: what its warpgroups share
-  if (!regs) {
-    cudaFuncAttributes fa;
-    T2SC_CUDA(cudaFuncGetAttributes(&fa, kernel), "attention");
-    regs = fa.numRegs;
-  }
-  if (regs * (NT + 1) < NT * S::kSoftmaxRegs + S::kOtherRegs) {
-    err = "attention: the kernel was built with fewer registers than its warpgroups share";
-    return T2SC_ERR_UNSUPPORTED;
-  }
   TcArgs t;
   const uint64_t D = a.head_dim, H = a.heads;
   auto encode = [&](CUtensorMap *m, const char *p, int64_t ld, int64_t rows) -> int {
