@@ -360,15 +360,32 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
 #pragma unroll
             for (int q = 0; q < kUnit; q++) s[q] = q < valid ? s[q] : -INFINITY;
           }
-          float top[4];
+          // P is computed relative to the maximum so far while this unit's is
+          // still being found, and once more if that turns out to be too low
+          // (always in the first unit, hardly ever later).
+          float l0, l1;
+          for (;;) {
+            const float base = kLift - (m == -INFINITY ? 0.f : m * a.c);
+            const uint64_t c2 = sm100::pack_f32x2(a.c, a.c), base2 = sm100::pack_f32x2(base, base);
+            uint64_t sum[2] = {0, 0};
+            float top[4] = {m, m, m, m};
 #pragma unroll
-          for (int q = 0; q < 4; q++) top[q] = fmaxf(s[q], s[q + 4]);
+            for (int q = 0; q < kUnit; q += 32) {
+              uint32_t p[16];
 #pragma unroll
-          for (int q = 8; q < kUnit; q += 4)
-#pragma unroll
-            for (int z = 0; z < 4; z++) top[z] = fmaxf(top[z], s[q + z]);
-          const float mn = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), m);
-          if (__any_sync(0xffffffffu, (mn - m) * a.c > kSlack)) {
+              for (int z = 0; z < 32; z += 2) {
+                float p0, p1;
+                sm100::unpack_f32x2(sm100::fma_f32x2(sm100::pack_f32x2(s[q + z], s[q + z + 1]), c2, base2), p0, p1);
+                p0 = ex2(p0), p1 = ex2(p1);
+                sum[z >> 1 & 1] = sm100::add_f32x2(sum[z >> 1 & 1], sm100::pack_f32x2(p0, p1));
+                p[z / 2] = pack2<DT>(p0, p1);
+                top[z >> 1 & 3] = fmaxf(fmaxf(top[z >> 1 & 3], s[q + z]), s[q + z + 1]);
+              }
+              sm100::tmem_st16(su + q / 2, p);
+            }
+            sm100::unpack_f32x2(sm100::add_f32x2(sum[0], sum[1]), l0, l1);
+            const float mn = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+            if (!__any_sync(0xffffffffu, (mn - m) * a.c > kSlack)) break;
             const float f = mn > m ? ex2((m - mn) * a.c) : 1.f;
             m = mn;
             l *= f;
@@ -392,24 +409,7 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
               }
             }
           }
-          const float base = kLift - (m == -INFINITY ? 0.f : m * a.c);
-          const uint64_t c2 = sm100::pack_f32x2(a.c, a.c), base2 = sm100::pack_f32x2(base, base);
-          uint64_t sum[2] = {0, 0};
-#pragma unroll
-          for (int q = 0; q < kUnit; q += 32) {
-            uint32_t p[16];
-#pragma unroll
-            for (int z = 0; z < 32; z += 2) {
-              float p0, p1;
-              sm100::unpack_f32x2(sm100::fma_f32x2(sm100::pack_f32x2(s[q + z], s[q + z + 1]), c2, base2), p0, p1);
-              p0 = ex2(p0), p1 = ex2(p1);
-              sum[z >> 1 & 1] = sm100::add_f32x2(sum[z >> 1 & 1], sm100::pack_f32x2(p0, p1));
-              p[z / 2] = pack2<DT>(p0, p1);
-            }
-            sm100::tmem_st16(su + q / 2, p);
-          }
-          float l0, l1;
-          sm100::unpack_f32x2(sm100::add_f32x2(sum[0], sum[1]), l0, l1);
+          if (!ok) break;
           l += l0 + l1;
           sm100::tmem_st_wait();
         }
