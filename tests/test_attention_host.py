@@ -33,7 +33,7 @@ def test_host_tensors_are_refused(t2sc):
         with pytest.raises(ValueError):
             t2sc.qk_norm_rope_device(x.view(4, 2, 8), None, torch.ones(2, 8), None, ctx=ctx)
     layout = object.__new__(t2sc.SequenceLayout)
-    layout.ctx, layout.q_offsets, layout.kv_offsets = _fake_ctx(), np.array([0, 4]), np.array([0, 4])
+    layout.ctx, layout.q_rows, layout.kv_rows = _fake_ctx(), 4, 4
     q = x.view(4, 2, 8)
     with pytest.raises(ValueError):
         layout.attention_device(q, q, q)

@@ -531,7 +531,8 @@ int launch(t2sc_seqs *s, const AttnArgs &a, int splits, std::string &err) {
   t.c = a.scale * 1.4426950408889634f, t.err = ctx->d_err;
   const int64_t grid = (NT == 2 ? s->blocks256 : s->blocks128) * a.heads * splits;
   if (grid > INT32_MAX) return fail(ctx, T2SC_ERR_UNSUPPORTED, "attention: too many query blocks in one call");
-  T2SC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem), "attention");
+  static std::atomic<uint64_t> allowed{0};
+  T2SC_TRY(allow_smem(ctx, kernel, (int)S::kSmem, allowed, err));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid), cfg.blockDim = dim3(S::kThreads), cfg.dynamicSmemBytes = S::kSmem, cfg.stream = ctx->stream;
   cudaLaunchAttribute at[1];

@@ -373,7 +373,8 @@ int launch(t2sc_ctx *ctx, const DenseArgs &a, std::string &err) {
   const int64_t tiles = (int64_t)t.m_tiles * t.n_tiles, most = ctx->num_sms / CG;
   t.slots = (int)(tiles < most ? tiles : most);
   auto kernel = dense_tc_kernel<DT, CG, BN>;
-  T2SC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem), "dense_linear");
+  static std::atomic<uint64_t> allowed{0};
+  T2SC_TRY(allow_smem(ctx, kernel, (int)S::kSmem, allowed, err));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)t.slots * CG), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = S::kSmem, cfg.stream = ctx->stream;
   cudaLaunchAttribute at[1];

@@ -1,6 +1,7 @@
 // Helpers shared by the C-ABI entry points: the device guard, the error
 // path, the exception barrier and the checks of strided device buffers.
 #pragma once
+#include <atomic>
 #include <new>
 #include <string>
 
@@ -43,6 +44,16 @@ int guarded(t2sc_ctx *ctx, F &&body) {
   } catch (...) {
     return fail(ctx, T2SC_ERR_INVALID, "unexpected exception");
   }
+}
+
+// Lets `kernel` use `bytes` of dynamic shared memory, once per device.
+template <class K>
+int allow_smem(t2sc_ctx *ctx, K kernel, int bytes, std::atomic<uint64_t> &done, std::string &err) {
+  const uint64_t bit = ctx->device < 64 ? uint64_t(1) << ctx->device : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return T2SC_OK;
+  T2SC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "shared memory size");
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return T2SC_OK;
 }
 
 inline bool dtype_known(int dtype) { return dtype == T2SC_DT_F32 || dtype == T2SC_DT_F16 || dtype == T2SC_DT_BF16; }

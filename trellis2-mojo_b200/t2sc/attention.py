@@ -13,78 +13,96 @@ import ctypes
 
 import numpy as np
 
+import torch
+
 from . import _lib
 from ._lib import check, lib
-from .decoder import _on_torch_stream
-from .sparse import _DTYPES, Context, SparseTensor, _check_on_ctx_device
+from .sparse import _DTYPES, Context, SparseTensor
 
 _ACTIVATIONS = {None: 0, "silu": _lib.SILU, "gelu": _lib.GELU}
 _LAYOUTS = {"pairs": _lib.ROPE_PAIRS, "halves": _lib.ROPE_HALVES}
-_CODES = None
+_CODES = {torch.float32: _lib.DT_F32, torch.float16: _lib.DT_F16, torch.bfloat16: _lib.DT_BF16}
+_linear, _rope_apply = lib.t2sc_dense_linear_device, lib.t2sc_rope_apply_device
+_qk_norm_rope, _attention = lib.t2sc_qk_norm_rope_device, lib.t2sc_attention_device
 
 
-def _code(dtype):
-    global _CODES
-    if _CODES is None:
-        import torch
-        _CODES = {torch.float32: _lib.DT_F32, torch.float16: _lib.DT_F16, torch.bfloat16: _lib.DT_BF16}
-    return _CODES.get(dtype)
+def _code(t, what):
+    code = _CODES.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{what} must be float32, float16 or bfloat16")
+    return code
 
 
-def _rows2d(t, ctx, dtype, what):
-    """Row stride of a [rows, width] tensor whose rows are contiguous."""
-    _check_on_ctx_device(t, ctx, what)
-    if t.dtype != dtype:
-        raise ValueError(f"{what} must be {dtype}")
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise ValueError(f"{what} must be [rows, width] with contiguous rows")
-    return _row_stride(t, t.shape[1], what)
+def _rows2d(t, device, dtype, what):
+    """(rows, width, row stride) of a [rows, width] tensor whose rows are contiguous."""
+    if not isinstance(t, torch.Tensor) or t.get_device() != device:
+        raise ValueError(f"{what} must be a CUDA tensor on cuda:{device}")
+    if t.dtype is not dtype or t.dim() != 2:
+        raise ValueError(f"{what} must be [rows, width] of {dtype}")
+    rows, width = t.shape
+    if t.is_contiguous():
+        return rows, width, width
+    stride, inner = t.stride()
+    if width > 1 and inner != 1:
+        raise ValueError(f"{what} must have contiguous rows")
+    return rows, width, _row_stride(rows, width, stride, what)
 
 
-def _heads3d(t, ctx, dtype, what):
-    """Row stride of a [rows, heads, head_dim] tensor whose rows are contiguous."""
-    _check_on_ctx_device(t, ctx, what)
-    if t.dtype != dtype:
-        raise ValueError(f"{what} must be {dtype}")
-    if t.dim() != 3:
-        raise ValueError(f"{what} must be [rows, heads, head_dim]")
-    _, h, d = t.shape
-    if (d > 1 and t.stride(2) != 1) or (h > 1 and t.stride(1) != d):
-        raise ValueError(f"{what} must be [rows, heads, head_dim] with contiguous rows")
-    return _row_stride(t, h * d, what)
+def _heads3d(t, device, dtype, what):
+    """(rows, heads, head_dim, row stride) of a [rows, heads, head_dim] tensor whose rows are contiguous."""
+    if not isinstance(t, torch.Tensor) or t.get_device() != device:
+        raise ValueError(f"{what} must be a CUDA tensor on cuda:{device}")
+    if t.dtype is not dtype or t.dim() != 3:
+        raise ValueError(f"{what} must be [rows, heads, head_dim] of {dtype}")
+    rows, h, d = t.shape
+    if t.is_contiguous():
+        return rows, h, d, h * d
+    stride, per_head, inner = t.stride()
+    if (d > 1 and inner != 1) or (h > 1 and per_head != d):
+        raise ValueError(f"{what} must have contiguous rows")
+    return rows, h, d, _row_stride(rows, h * d, stride, what)
 
 
-def _row_stride(t, width, what):
-    if t.shape[0] <= 1:
+def _row_stride(rows, width, stride, what):
+    if rows <= 1:
         return width
-    s = t.stride(0)
-    if s < width:
+    if stride < width:
         raise ValueError(f"{what}: rows overlap")
-    return s
+    return stride
 
 
-def _f32(t, ctx, shape, what):
-    import torch
-    _check_on_ctx_device(t, ctx, what)
-    if t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous():
-        raise ValueError(f"{what} must be contiguous float32 {list(shape)}")
+def _f32(t, device, shape, what):
+    if not isinstance(t, torch.Tensor) or t.get_device() != device or t.dtype is not torch.float32 or \
+            t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{what} must be contiguous float32 {list(shape)} on cuda:{device}")
     return t.data_ptr()
 
 
-def _coords(t, ctx, rows):
-    import torch
-    _check_on_ctx_device(t, ctx, "coords")
-    if t.dtype != torch.int32 or tuple(t.shape) != (rows, 4) or not t.is_contiguous():
-        raise ValueError("coords must be contiguous int32 [rows, 4]")
+def _coords(t, device, rows):
+    if not isinstance(t, torch.Tensor) or t.get_device() != device or t.dtype is not torch.int32 or \
+            t.shape != (rows, 4) or not t.is_contiguous():
+        raise ValueError(f"coords must be contiguous int32 [rows, 4] on cuda:{device}")
     return t.data_ptr()
 
 
 def _context(ctx, t):
     if ctx is not None:
         return ctx
-    if not getattr(t, "is_cuda", False):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError("the operator takes CUDA tensors")
-    return Context.default(t.device.index)
+    return Context.default(t.get_device())
+
+
+def _on_torch_stream(ctx):
+    """The context's work goes to torch's current stream of its device."""
+    stream = torch.cuda.current_stream(ctx.device).cuda_stream if _raw_stream is None else _raw_stream(ctx.device)
+    stream = stream or 1    # handle 0 would name the context's own stream, 1 is cudaStreamLegacy
+    if ctx.stream_ptr != stream:
+        ctx.set_stream(stream)
+
+
+# the handle alone, without a Stream object around it (2 us less a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def dense_linear_device(x, weight, bias=None, activation=None, residual=None, out=None, ctx=None):
@@ -93,36 +111,33 @@ def dense_linear_device(x, weight, bias=None, activation=None, residual=None, ou
     strided; bias float32 [co]; activation None, "silu" or "gelu" (tanh
     form); residual and out [rows, co] of x's type, out may be residual."""
     ctx = _context(ctx, x)
+    device, dtype = ctx.device, x.dtype
     if activation not in _ACTIVATIONS:
         raise ValueError('dense_linear: activation must be None, "silu" or "gelu"')
-    code = _code(x.dtype)
-    if code is None:
-        raise ValueError("dense_linear: x must be float32, float16 or bfloat16")
-    ldx = _rows2d(x, ctx, x.dtype, "dense_linear: x")
-    ldw = _rows2d(weight, ctx, x.dtype, "dense_linear: weight")
-    rows, ci = x.shape
-    co = weight.shape[0]
-    if weight.shape[1] != ci or ci < 1 or co < 1:
+    code, flags = _code(x, "dense_linear: x"), _ACTIVATIONS[activation]
+    rows, ci, ldx = _rows2d(x, device, dtype, "dense_linear: x")
+    co, wi, ldw = _rows2d(weight, device, dtype, "dense_linear: weight")
+    if wi != ci or ci < 1 or co < 1:
         raise ValueError("dense_linear: weight must be [co, ci] with x's ci")
-    flags = _ACTIVATIONS[activation]
-    ldr = 0
+    res, ldr = None, 0
     if residual is not None:
-        ldr = _rows2d(residual, ctx, x.dtype, "dense_linear: residual")
-        if tuple(residual.shape) != (rows, co):
+        r, w, ldr = _rows2d(residual, device, dtype, "dense_linear: residual")
+        if r != rows or w != co:
             raise ValueError("dense_linear: residual must be [rows, co]")
-        flags |= _lib.RESIDUAL
+        res, flags = residual.data_ptr(), flags | _lib.RESIDUAL
     if out is None:
-        out = x.new_empty((rows, co))
-    elif tuple(out.shape) != (rows, co):
-        raise ValueError("dense_linear: out must be [rows, co]")
-    ldy = _rows2d(out, ctx, x.dtype, "dense_linear: out")
-    if rows == 0:
-        return out
-    _on_torch_stream(ctx, x.device)
-    check(lib.t2sc_dense_linear_device(ctx.handle, x.data_ptr(), ldx, weight.data_ptr(), ldw,
-                                       None if bias is None else _f32(bias, ctx, (co,), "dense_linear: bias"),
-                                       None if residual is None else residual.data_ptr(), ldr, out.data_ptr(), ldy,
-                                       rows, co, ci, flags, code), ctx.handle)
+        out, ldy = x.new_empty((rows, co)), co
+    else:
+        r, w, ldy = _rows2d(out, device, dtype, "dense_linear: out")
+        if r != rows or w != co:
+            raise ValueError("dense_linear: out must be [rows, co]")
+    b = None if bias is None else _f32(bias, device, (co,), "dense_linear: bias")
+    if rows:
+        _on_torch_stream(ctx)
+        rc = _linear(ctx.handle, x.data_ptr(), ldx, weight.data_ptr(), ldw, b, res, ldr, out.data_ptr(), ldy, rows, co, ci,
+                     flags, code)
+        if rc:
+            check(rc, ctx.handle)
     return out
 
 
@@ -148,28 +163,29 @@ class RotaryPositionEmbedder:
 
     def forward_device(self, x, coords, out=None):
         """x [rows, heads, head_dim] (rows may be strided), coords int32 [rows, 4]; out may be x."""
-        code = _code(x.dtype)
-        if code is None:
-            raise ValueError("RotaryPositionEmbedder: x must be float32, float16 or bfloat16")
-        ldx = _heads3d(x, self.ctx, x.dtype, "RotaryPositionEmbedder: x")
-        rows, heads, d = x.shape
+        ctx = self.ctx
+        device, dtype = ctx.device, x.dtype
+        code = _code(x, "RotaryPositionEmbedder: x")
+        rows, heads, d, ldx = _heads3d(x, device, dtype, "RotaryPositionEmbedder: x")
         if d != self.head_dim or heads < 1:
             raise ValueError("RotaryPositionEmbedder: x must be [rows, heads, head_dim]")
-        at = _coords(coords, self.ctx, rows)
+        at = _coords(coords, device, rows)
         if out is None:
-            out = x.new_empty((rows, heads, d))
-        elif out.shape != x.shape:
-            raise ValueError("RotaryPositionEmbedder: out must have x's shape")
-        ldy = _heads3d(out, self.ctx, x.dtype, "RotaryPositionEmbedder: out")
+            out, ldy = x.new_empty((rows, heads, d)), heads * d
+        else:
+            r, h, e, ldy = _heads3d(out, device, dtype, "RotaryPositionEmbedder: out")
+            if (r, h, e) != (rows, heads, d):
+                raise ValueError("RotaryPositionEmbedder: out must have x's shape")
         if rows:
-            _on_torch_stream(self.ctx, x.device)
-            check(lib.t2sc_rope_apply_device(self.handle, at, x.data_ptr(), ldx, out.data_ptr(), ldy, rows, heads, code),
-                  self.ctx.handle)
+            _on_torch_stream(ctx)
+            rc = _rope_apply(self.handle, at, x.data_ptr(), ldx, out.data_ptr(), ldy, rows, heads, code)
+            if rc:
+                check(rc, ctx.handle)
         return out
 
     def __del__(self):
         h = getattr(self, "handle", None)
-        if h and self.ctx.handle:
+        if h and lib is not None and self.ctx.handle:   # None: the interpreter is shutting down
             lib.t2sc_rope_destroy(h)
             self.handle = None
 
@@ -180,40 +196,42 @@ def qk_norm_rope_device(q, k, gain_q, gain_k, coords=None, rope=None, eps=1e-6, 
     head_dim] (rows may be strided), gains float32 [heads, head_dim]. k None:
     q alone. out_q may be q and out_k k. Returns (out_q, out_k)."""
     ctx = rope.ctx if ctx is None and rope is not None else _context(ctx, q)
-    code = _code(q.dtype)
-    if code is None:
-        raise ValueError("qk_norm_rope: q must be float32, float16 or bfloat16")
-    ldq = _heads3d(q, ctx, q.dtype, "qk_norm_rope: q")
-    rows, heads, d = q.shape
+    device, dtype = ctx.device, q.dtype
+    code = _code(q, "qk_norm_rope: q")
+    rows, heads, d, ldq = _heads3d(q, device, dtype, "qk_norm_rope: q")
     if heads < 1 or (rope is not None and rope.head_dim != d):
         raise ValueError("qk_norm_rope: q must be [rows, heads, head_dim] with rope's head_dim")
+    shape = (rows, heads, d)
     if out_q is None:
-        out_q = q.new_empty((rows, heads, d))
-    elif out_q.shape != q.shape:
-        raise ValueError("qk_norm_rope: out_q must have q's shape")
-    ldqo = _heads3d(out_q, ctx, q.dtype, "qk_norm_rope: out_q")
-    gq = _f32(gain_q, ctx, (heads, d), "qk_norm_rope: gain_q")
+        out_q, ldqo = q.new_empty(shape), heads * d
+    else:
+        *got, ldqo = _heads3d(out_q, device, dtype, "qk_norm_rope: out_q")
+        if tuple(got) != shape:
+            raise ValueError("qk_norm_rope: out_q must have q's shape")
+    gq = _f32(gain_q, device, (heads, d), "qk_norm_rope: gain_q")
     ldk = ldko = 0
     gk = kp = kop = None
     if k is not None:
-        ldk = _heads3d(k, ctx, q.dtype, "qk_norm_rope: k")
-        if k.shape != q.shape:
+        *got, ldk = _heads3d(k, device, dtype, "qk_norm_rope: k")
+        if tuple(got) != shape:
             raise ValueError("qk_norm_rope: k must have q's shape")
         if out_k is None:
-            out_k = q.new_empty((rows, heads, d))
-        elif out_k.shape != q.shape:
-            raise ValueError("qk_norm_rope: out_k must have q's shape")
-        ldko = _heads3d(out_k, ctx, q.dtype, "qk_norm_rope: out_k")
-        gk = _f32(gain_k, ctx, (heads, d), "qk_norm_rope: gain_k")
+            out_k, ldko = q.new_empty(shape), heads * d
+        else:
+            *got, ldko = _heads3d(out_k, device, dtype, "qk_norm_rope: out_k")
+            if tuple(got) != shape:
+                raise ValueError("qk_norm_rope: out_k must have q's shape")
+        gk = _f32(gain_k, device, (heads, d), "qk_norm_rope: gain_k")
         kp, kop = k.data_ptr(), out_k.data_ptr()
     elif out_k is not None:
         raise ValueError("qk_norm_rope: out_k without k")
-    at = _coords(coords, ctx, rows) if rope is not None else None
+    at = _coords(coords, device, rows) if rope is not None else None
     if rows:
-        _on_torch_stream(ctx, q.device)
-        check(lib.t2sc_qk_norm_rope_device(ctx.handle, None if rope is None else rope.handle, at, q.data_ptr(), ldq, kp,
-                                           ldk, gq, gk, out_q.data_ptr(), ldqo, kop, ldko, rows, heads, d, float(eps),
-                                           code), ctx.handle)
+        _on_torch_stream(ctx)
+        rc = _qk_norm_rope(ctx.handle, None if rope is None else rope.handle, at, q.data_ptr(), ldq, kp, ldk, gq, gk,
+                           out_q.data_ptr(), ldqo, kop, ldko, rows, heads, d, eps, code)
+        if rc:
+            check(rc, ctx.handle)
     return out_q, out_k
 
 
@@ -228,6 +246,7 @@ class SequenceLayout:
         self.kv_offsets = self.q_offsets if kv_lens is None else self._offsets(kv_lens)
         if len(self.q_offsets) != len(self.kv_offsets):
             raise ValueError("SequenceLayout: as many key lengths as query lengths")
+        self.q_rows, self.kv_rows = int(self.q_offsets[-1]), int(self.kv_offsets[-1])
         self.ctx = ctx or Context.default()
         h = ctypes.c_void_p()
         check(lib.t2sc_seqs_create(self.ctx.handle, self.q_offsets.ctypes.data, self.kv_offsets.ctypes.data,
@@ -252,42 +271,40 @@ class SequenceLayout:
         (more rows may follow; they are left alone); rows may be strided.
         scale defaults to head_dim ** -0.5. out must not overlap an input."""
         ctx = self.ctx
-        code = _code(q.dtype)
-        if code is None:
-            raise ValueError("attention: q must be float32, float16 or bfloat16")
-        ldq = _heads3d(q, ctx, q.dtype, "attention: q")
-        ldk = _heads3d(k, ctx, q.dtype, "attention: k")
-        ldv = _heads3d(v, ctx, q.dtype, "attention: v")
-        rows, heads, d = q.shape
-        if tuple(k.shape[1:]) != (heads, d) or v.shape != k.shape or heads < 1 or d < 1:
+        device, dtype = ctx.device, q.dtype
+        code = _code(q, "attention: q")
+        rows, heads, d, ldq = _heads3d(q, device, dtype, "attention: q")
+        kv_rows, kh, kd, ldk = _heads3d(k, device, dtype, "attention: k")
+        v_rows, vh, vd, ldv = _heads3d(v, device, dtype, "attention: v")
+        if kh != heads or kd != d or (v_rows, vh, vd) != (kv_rows, kh, kd) or heads < 1 or d < 1:
             raise ValueError("attention: k and v must be [rows, heads, head_dim] with q's heads and head_dim")
-        if rows < self.q_offsets[-1] or k.shape[0] < self.kv_offsets[-1]:
+        if rows < self.q_rows or kv_rows < self.kv_rows:
             raise ValueError("attention: fewer rows than the layout has")
         if out is None:
-            out = q.new_empty((rows, heads, d))
-        elif out.shape != q.shape:
-            raise ValueError("attention: out must have q's shape")
-        ldo = _heads3d(out, ctx, q.dtype, "attention: out")
-        _on_torch_stream(ctx, q.device)
-        check(lib.t2sc_attention_device(self.handle, q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv,
-                                        out.data_ptr(), ldo, heads, d, float(d ** -0.5 if scale is None else scale),
-                                        code), ctx.handle)
+            out, ldo = q.new_empty((rows, heads, d)), heads * d
+        else:
+            r, h, e, ldo = _heads3d(out, device, dtype, "attention: out")
+            if (r, h, e) != (rows, heads, d):
+                raise ValueError("attention: out must have q's shape")
+        _on_torch_stream(ctx)
+        rc = _attention(self.handle, q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, out.data_ptr(), ldo, heads, d,
+                        d ** -0.5 if scale is None else scale, code)
+        if rc:
+            check(rc, ctx.handle)
         return out
 
     def __del__(self):
         h = getattr(self, "handle", None)
-        if h and self.ctx.handle:
+        if h and lib is not None and self.ctx.handle:   # None: the interpreter is shutting down
             lib.t2sc_seqs_destroy(h)
             self.handle = None
 
 
 def _tensor(a, dtype, device):
-    import torch
     return None if a is None else torch.from_numpy(np.array(a, np.float32)).to(device, dtype)
 
 
 def _torch_dtype(dtype):
-    import torch
     return {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[dtype]
 
 
@@ -317,8 +334,7 @@ class SparseMultiHeadAttention:
         self.channels, self.heads, self.head_dim = channels, heads, channels // heads
         self.cross, self.rope, self.eps, self.dtype = to_qkv is None, rope, float(eps), dtype
         dev, dt = f"cuda:{self.ctx.device}", _torch_dtype(dtype)
-        import torch
-
+    
         def pair(wb, co, ci=None):
             w, b = _tensor(wb[0], dt, dev), _tensor(wb[1], torch.float32, dev)
             if w.dim() != 2 or w.shape[0] != co or (ci is not None and w.shape[1] != ci) or \
@@ -342,7 +358,7 @@ class SparseMultiHeadAttention:
         the layout's last are not given a meaning: pass none."""
         h, d, c = self.heads, self.head_dim, self.channels
         rows = x.shape[0]
-        if rows != layout.q_offsets[-1]:
+        if rows != layout.q_rows:
             raise ValueError("SparseMultiHeadAttention: x must have the layout's rows")
         if self.cross:
             if context is None:
@@ -365,7 +381,6 @@ class SparseMultiHeadAttention:
     def forward(self, x, context=None, context_lens=None, residual=False):
         """x: SparseTensor; context: host f32 [rows, ctx_channels] with
         context_lens rows of it for each batch entry. residual: add x."""
-        import torch
         dev, dt = f"cuda:{self.ctx.device}", _torch_dtype(self.dtype)
         xd = _tensor(x.feats, dt, dev)
         if self.cross and context_lens is None:
@@ -385,7 +400,6 @@ class SparseFeedForwardNet:
     [H]), lin2 = (weight [C, H], bias [C])."""
 
     def __init__(self, lin1, lin2, activation="gelu", dtype="bf16", ctx=None):
-        import torch
         if activation not in _ACTIVATIONS:
             raise ValueError('SparseFeedForwardNet: activation must be None, "silu" or "gelu"')
         if dtype not in _DTYPES:

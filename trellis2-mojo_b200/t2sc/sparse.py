@@ -40,6 +40,7 @@ class Context:
         check(rc)
         self.handle = h
         self.device = device
+        self.stream_ptr = None    # as last set; None: the context's own stream
 
     @classmethod
     def default(cls, device=0):
@@ -62,6 +63,7 @@ class Context:
     def set_stream(self, stream_ptr):
         check(lib.t2sc_ctx_set_stream(self.handle, ctypes.c_void_p(stream_ptr) if stream_ptr else None),
               self.handle)
+        self.stream_ptr = stream_ptr or None
 
     def close(self):
         if self.handle:
