@@ -210,7 +210,7 @@ def test_qk_norm_rope(t2sc, dtype, layout, rows, heads, d):
 
 # ---- attention ----
 
-LENGTHS = [([1], [1]), ([1], [300]), ([3], [2048]), ([17], [0]), ([64], [64]), ([127], [129]), ([128], [128]), ([129], [127]),
+LENGTHS = [([2, 1, 0, 2], [700, 0, 5, 129]), ([4, 3, 1], [9000, 1, 64]), ([1, 1], [5000, 20000]), ([8, 5], [2100, 77]), ([1], [1]), ([1], [300]), ([3], [2048]), ([17], [0]), ([64], [64]), ([127], [129]), ([128], [128]), ([129], [127]),
            ([255, 1, 0, 300], [255, 1, 0, 300]), ([5, 0, 200, 40], [0, 77, 1, 513]), ([700], [1029]), ([256, 257], [1, 640])]
 
 

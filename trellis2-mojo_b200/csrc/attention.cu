@@ -190,6 +190,7 @@ int t2sc_seqs_create(t2sc_ctx *ctx, const int64_t *q_offsets, const int64_t *kv_
     for (int64_t b = 0; b < batch; b++) {
       blocks[b + 1] = blocks[b] + ((int64_t)sorted[b].y + 255) / 256;
       blocks[batch + 1 + b + 1] = blocks[batch + 1 + b] + ((int64_t)sorted[b].y + 127) / 128;
+      s->max_q = std::max<int64_t>(s->max_q, sorted[b].y);
       s->max_kv = std::max<int64_t>(s->max_kv, sorted[b].w);
     }
     s->blocks256 = blocks[batch], s->blocks128 = blocks[2 * batch + 1];
@@ -246,6 +247,7 @@ int t2sc_attention_device(t2sc_seqs *seqs, const void *q, int64_t q_stride, cons
     a.ldq = q_stride, a.ldk = k_stride, a.ldv = v_stride, a.ldo = out_stride;
     a.seqs = seqs->d_seqs, a.batch = (int)seqs->batch, a.heads = heads, a.head_dim = head_dim, a.scale = scale;
     DeviceGuard g(ctx->device);
+    if (attention_rows_takes(seqs, a, dtype)) return attention_rows(seqs, a, dtype, ctx->last_error);
     return attention_tc_takes(seqs, a, dtype) ? attention_tc(seqs, a, dtype, ctx->last_error)
                                               : attention_simt(seqs, a, dtype, ctx->last_error);
   });

@@ -13,7 +13,7 @@ struct t2sc_seqs {
   std::vector<int64_t> q_off, kv_off;  // [batch + 1]
   int64_t q_rows = 0, kv_rows = 0;     // rows up to the last offset
   int64_t q_total = 0;                 // query rows inside sequences
-  int64_t max_kv = 0;                  // keys of the longest sequence
+  int64_t max_q = 0, max_kv = 0;       // queries, keys of the longest sequence
   int64_t blocks128 = 0, blocks256 = 0;  // blocks of 128 / 256 query rows, sequence by sequence
   int4 *d_sorted = nullptr;            // as d_seqs, most keys first
   int64_t *d_blocks = nullptr;         // [2][batch + 1] blocks of 256 / 128 rows before each sequence of d_sorted
@@ -34,6 +34,9 @@ struct AttnArgs {
 // 16-bit rows that start on 16 bytes, head_dim a multiple of 8 up to 128, scale > 0.
 bool attention_tc_takes(const t2sc_seqs *s, const AttnArgs &a, int dtype);
 int attention_tc(t2sc_seqs *s, const AttnArgs &a, int dtype, std::string &err);
+// As attention_tc, for at most 4 queries a sequence.
+bool attention_rows_takes(const t2sc_seqs *s, const AttnArgs &a, int dtype);
+int attention_rows(t2sc_seqs *s, const AttnArgs &a, int dtype, std::string &err);
 int attention_simt(t2sc_seqs *s, const AttnArgs &a, int dtype, std::string &err);
 
 }  // namespace t2sc
