@@ -2,7 +2,7 @@
 // 16 bytes and head dims that are multiples of 8 up to 128.
 //
 // A CTA owns NT blocks of 128 queries of one head and walks its sequence's
-// keys. TMA brings the query blocks once and blocks of 128 K and V rows
+// keys. TMA brings the query blocks once and blocks of K and V rows
 // through a ring of shared-memory slots (heads are a dimension of the tensor
 // map: channels past head_dim read as zero). One thread issues the
 // products, for a unit of 64 keys at a time:
@@ -49,7 +49,7 @@
 namespace t2sc {
 namespace {
 
-constexpr int kBQ = 128, kBK = 128, kUnit = 64;
+constexpr int kBQ = 128, kUnit = 64;
 constexpr long long kWaitLimit = 4000000000ll;  // ~2 s of SM clocks
 
 struct TcArgs {
@@ -65,10 +65,15 @@ struct TcArgs {
 
 template <int DP, int NT>
 struct Shape {
-  static constexpr int kTile = 128 * DP * 2;  // bytes of a 128-row block
-  static constexpr int kSlots = NT == 2 ? (DP == 128 ? 5 : 8) : (DP == 128 ? 2 : 4);
+  static constexpr int kTile = kBQ * DP * 2;  // bytes of a query block
+  // Keys of a K or V block: two units, or one where two CTAs' shared memory
+  // would leave a ring of only two slots (300 queries over 20000 keys,
+  // 12 x 128: RINGT us).
+  static constexpr int kBK = NT == 1 && DP == 128 ? 64 : 128, kUB = kBK / kUnit;
+  static constexpr int kSlot = kBK * DP * 2, kHalf = kBK * 128;  // bytes of a slot, of its 64-channel half
+  static constexpr int kSlots = NT == 2 ? (DP == 128 ? 5 : 8) : 4;
   static constexpr int kExtra = 2048;         // barriers, m and l of the rows
-  static constexpr size_t kSmem = 1024 + (size_t)(NT + kSlots) * kTile + kExtra;
+  static constexpr size_t kSmem = 1024 + (size_t)NT * kTile + (size_t)kSlots * kSlot + kExtra;
   static constexpr int kThreads = 128 * (NT + 1);
   static constexpr uint32_t kCols = NT == 2 ? 512 : 256;
   // Query blocks whose units join one barrier. At head_dim 128 the products
@@ -78,10 +83,9 @@ struct Shape {
   static constexpr int kGroups = DP == 128 ? 1 : NT;
 };
 
+// Bounded wait of a whole warp, its verdict the same in every lane.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *abort, int *err) {
-  bool ok = sm100::mbar_test_wait(bar, parity);
-  if (__all_sync(0xffffffffu, ok)) return true;
-  if (!ok) ok = sm100::mbar_wait_bounded(bar, parity, abort, err, kDevErrTimeout, kWaitLimit);
+  const bool ok = sm100::mbar_wait_bounded(bar, parity, abort, err, kDevErrTimeout, kWaitLimit);
   return __all_sync(0xffffffffu, ok);
 }
 
@@ -111,12 +115,12 @@ __device__ __forceinline__ float ld_cluster1(uint32_t addr) {
 template <int DT, int DP, int NT>
 __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) attention_tc_kernel(const __grid_constant__ TcArgs a) {
   using S = Shape<DP, NT>;
-  constexpr int NS = S::kSlots, kSub = DP / 64;
+  constexpr int NS = S::kSlots, kSub = DP / 64, kBK = S::kBK, kUB = S::kUB;
   constexpr float kSlack = DT == T2SC_DT_F16 ? 7.f : 8.f, kLift = DT == T2SC_DT_F16 ? 8.f : 0.f;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t *ring = smem + NT * S::kTile;
-  float *row_m = reinterpret_cast<float *>(ring + NS * S::kTile), *row_l = row_m + 128;  // split sums
+  float *row_m = reinterpret_cast<float *>(ring + NS * S::kSlot), *row_l = row_m + 128;  // split sums
   uint64_t *bars = reinterpret_cast<uint64_t *>(row_l + 128);
   // bars: q_full[NT], s_full[NT][2], o_prev[NT], o_full[NT], ready[kGroups][2], full[NS], empty[NS]
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 5 * NT + 2 * S::kGroups + 2 * NS);
@@ -202,10 +206,10 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
           break;
         }
         if (lane == 0) {
-          sm100::mbar_arrive_expect_tx(full0 + 8 * s, S::kTile);
+          sm100::mbar_arrive_expect_tx(full0 + 8 * s, S::kSlot);
           const void *map = j & 1 ? &a.map_v : &a.map_k;
           for (int h = 0; h < kSub; h++)
-            sm100::tma_load_3d(rsm + s * S::kTile + h * 16384, map, h * 64, head, kv0 + (t0 + (j >> 1)) * kBK, full0 + 8 * s);
+            sm100::tma_load_3d(rsm + s * S::kSlot + h * S::kHalf, map, h * 64, head, kv0 + (t0 + (j >> 1)) * kBK, full0 + 8 * s);
         }
         __syncwarp();
         it++;
@@ -233,31 +237,36 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
         // descriptors: both operands' high words are the same (1024 bytes between 8-row atoms, 128-byte swizzle)
         const uint64_t dq0 = sm100::smem_desc(qsm, 128);
         const uint32_t hi = (uint32_t)(dq0 >> 32), q_lo = (uint32_t)dq0, k_lo = (uint32_t)sm100::smem_desc(rsm, 128),
-                       v_lo = (uint32_t)sm100::smem_desc_mn(rsm, 16384);
-        constexpr uint32_t kTile16 = S::kTile >> 4, kUnit16 = kUnit * 128 >> 4;
+                       v_lo = (uint32_t)sm100::smem_desc_mn(rsm, S::kHalf);
+        constexpr uint32_t kTile16 = S::kTile >> 4, kSlot16 = S::kSlot >> 4, kHalf16 = S::kHalf >> 4, kUnit16 = kUnit * 128 >> 4;
         bool ok = true;
         auto wait = [&](uint32_t bar, uint32_t parity) {
           ok = ok && sm100::mbar_wait_bounded(bar, parity, abort, a.err, kDevErrTimeout, kWaitLimit);
           sm100::tc_fence_after();
         };
-        auto scores = [&](int i, int b, uint32_t kslot, bool done) {  // S into buffer b = the unit's half of its block
-          const uint32_t dq = q_lo + i * kTile16, dk = k_lo + kslot * kTile16 + b * kUnit16, d = s_tmem + i * 128 + b * kUnit;
+        auto scores = [&](int i, int b, uint32_t kslot, bool done) {  // S into buffer b; b is the unit's place in a block of two
+          const uint32_t dq = q_lo + i * kTile16, dk = k_lo + kslot * kSlot16 + (kUB == 2 ? b * kUnit16 : 0),
+                         d = s_tmem + i * 128 + b * kUnit;
           if (ksteps == DP / 16) {
 #pragma unroll
             for (int kk = 0; kk < DP / 16; kk++)
-              sm100::mma_f16_lo(d, dq + (kk >> 2) * 1024 + (kk & 3) * 2, dk + (kk >> 2) * 1024 + (kk & 3) * 2, hi, idesc_s, kk > 0);
+              sm100::mma_f16_lo(d, dq + (kk >> 2) * 1024 + (kk & 3) * 2, dk + (kk >> 2) * kHalf16 + (kk & 3) * 2, hi, idesc_s, kk > 0);
           } else {
 #pragma unroll 1
             for (int kk = 0; kk < ksteps; kk++)
-              sm100::mma_f16_lo(d, dq + (kk >> 2) * 1024 + (kk & 3) * 2, dk + (kk >> 2) * 1024 + (kk & 3) * 2, hi, idesc_s, kk > 0);
+              sm100::mma_f16_lo(d, dq + (kk >> 2) * 1024 + (kk & 3) * 2, dk + (kk >> 2) * kHalf16 + (kk & 3) * 2, hi, idesc_s, kk > 0);
           }
           sm100::mma_commit(s_full + 16 * i + 8 * b);
           if (done && i == nt - 1) sm100::mma_commit(empty0 + 8 * kslot);  // the block's last unit, for the last query block
         };
-        // ring position of the V block at hand, and of the K block behind it
-        uint32_t vslot = 1 % NS, kslot = 2 % NS;
+        // ring position of the V block at hand, and of the K block of two units on (block j's loads are 2 j and 2 j + 1)
+        uint32_t vslot = 1, kslot = kUB == 2 ? 2 : 4 % NS;
+        auto next_block = [&]() {
+          vslot = vslot + 2 >= NS ? vslot + 2 - NS : vslot + 2;
+          kslot = kslot + 2 >= NS ? kslot + 2 - NS : kslot + 2;
+        };
         auto unit = [&](int u, int b, bool last) {
-          const uint32_t dv = v_lo + vslot * kTile16 + b * kUnit16;
+          const uint32_t dv = v_lo + vslot * kSlot16 + (kUB == 2 ? b * kUnit16 : 0);
 #pragma unroll
           for (int i = 0; i < NT; i++) {
             if (i >= nt) break;
@@ -272,9 +281,9 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
 #pragma unroll 1
               for (int kk = 0; kk < steps; kk++) sm100::mma_f16_ts_lo(o, p + kk * 8, dv + kk * 128, hi, idesc_o, u + kk > 0);
             }
-            if (i == nt - 1 && (b == 1 || last)) sm100::mma_commit(empty0 + 8 * vslot);
+            if (i == nt - 1 && (kUB == 1 || b == 1 || last)) sm100::mma_commit(empty0 + 8 * vslot);
             if (u + 2 < units)
-              scores(i, b, kslot, b == 1 || u + 2 == units - 1);
+              scores(i, b, kslot, kUB == 1 || b == 1 || u + 2 == units - 1);
             else
               sm100::mma_commit((last ? o_full : o_prev) + 8 * i);
           }
@@ -283,14 +292,15 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
         for (int u = 0; u < min(units, 2); u++)
           for (int i = 0; i < nt; i++) {
             if (u == 0) wait(q_full + 8 * i, 0);
-            if (ok) scores(i, u, 0, u == 1 || units == 1);
+            if (u == 1 && kUB == 1 && i == 0) wait(full0 + 16, 0);
+            if (ok) scores(i, u, kUB == 2 ? 0 : 2 * u, kUB == 1 || u == 1 || units == 1);
           }
 #pragma unroll 1
         for (int u = 0; u < units && ok; u += 2) {
           unit(u, 0, u + 1 >= units);
+          if (kUB == 1) next_block();
           if (u + 1 < units && ok) unit(u + 1, 1, u + 2 >= units);
-          vslot = kslot + 1 == NS ? 0 : kslot + 1;
-          kslot = vslot + 1 == NS ? 0 : vslot + 1;
+          next_block();
         }
         // all issued MMAs retire before TMEM and shared memory are given up: in
         // the regular case o_full told so; after an abort wait for a last commit
@@ -304,23 +314,24 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
       // Joins a unit's barrier once its V block and the K block of two units
       // on are there, and zeros the V rows behind the last key, up to the 16
       // that a product step takes.
-      // Every load is waited for in turn, the first K too: a wait for a slot's
+      // Every load is waited for, the first units' K too: a wait for a slot's
       // next phase is only good once the one before it has completed.
-      const bool first = warp_wait(full0, 0, abort, a.err);
+      bool first = warp_wait(full0, 0, abort, a.err);
+      if (kUB == 1 && units > 1) first = first && warp_wait(full0 + 16, 0, abort, a.err);
       for (int u = 0; u < units && first; u++) {
         bool over = true;  // the barrier's last use, two units ago
         for (int g = 0; g < min(S::kGroups, nt); g++)
           over = over && (u < 2 || warp_wait(ready + 16 * g + 8 * (u & 1), ((u - 2) >> 1) & 1, abort, a.err));
         if (!over) break;
-        if (!(u & 1)) {
-          const uint32_t v = u + 1, k = u + 2;  // loads: block j's K is number 2 j, its V 2 j + 1
+        if (u % kUB == 0) {
+          const uint32_t v = 2 * (u / kUB) + 1, k = 2 * ((u + 2) / kUB);  // loads: block j's K is number 2 j, its V 2 j + 1
           if (!warp_wait(full0 + 8 * (v % NS), (v / NS) & 1, abort, a.err)) break;
           if (u + 2 < units && !warp_wait(full0 + 8 * (k % NS), (k / NS) & 1, abort, a.err)) break;
           const int valid = keys - u * kUnit;  // of this block's
           if (valid < kBK && valid % 16) {
-            uint8_t *rows = ring + v % NS * S::kTile + valid * 128;
+            uint8_t *rows = ring + v % NS * S::kSlot + valid * 128;
             for (int x = lane; x < (16 - valid % 16) * 8 * kSub; x += 32)
-              *reinterpret_cast<uint4 *>(rows + x % kSub * 16384 + x / kSub * 16) = make_uint4(0, 0, 0, 0);
+              *reinterpret_cast<uint4 *>(rows + x % kSub * S::kHalf + x / kSub * 16) = make_uint4(0, 0, 0, 0);
             sm100::fence_proxy_async_smem();
           }
         }
@@ -514,16 +525,16 @@ int launch(t2sc_seqs *s, const AttnArgs &a, int splits, std::string &err) {
   auto kernel = attention_tc_kernel<DT, DP, NT>;
   TcArgs t;
   const uint64_t D = a.head_dim, H = a.heads;
-  auto encode = [&](CUtensorMap *m, const char *p, int64_t ld, int64_t rows) -> int {
+  auto encode = [&](CUtensorMap *m, const char *p, int64_t ld, int64_t rows, uint32_t box_rows) -> int {
     const uint64_t dims[3] = {D, H, (uint64_t)std::max<int64_t>(rows, 1)};
     const uint64_t strides[2] = {D * 2, rows > 1 ? (uint64_t)ld * 2 : D * H * 2};
-    const uint32_t box[3] = {64, 1, 128};
+    const uint32_t box[3] = {64, 1, box_rows};
     return tensormap_16bit(m, DT, 3, p, dims, strides, box, err);
   };
-  T2SC_TRY(encode(&t.map_q, a.q, a.ldq, s->q_rows));
+  T2SC_TRY(encode(&t.map_q, a.q, a.ldq, s->q_rows, kBQ));
   const bool keys = s->kv_off[s->batch] > s->kv_off[0];
-  T2SC_TRY(encode(&t.map_k, keys ? a.k : a.q, keys ? a.ldk : a.ldq, keys ? s->kv_rows : 1));  // never read without keys
-  T2SC_TRY(encode(&t.map_v, keys ? a.v : a.q, keys ? a.ldv : a.ldq, keys ? s->kv_rows : 1));
+  T2SC_TRY(encode(&t.map_k, keys ? a.k : a.q, keys ? a.ldk : a.ldq, keys ? s->kv_rows : 1, S::kBK));  // never read without keys
+  T2SC_TRY(encode(&t.map_v, keys ? a.v : a.q, keys ? a.ldv : a.ldq, keys ? s->kv_rows : 1, S::kBK));
   t.out = a.out, t.ldo = a.ldo;
   t.seqs = s->d_sorted;
   t.blocks = s->d_blocks + (NT == 2 ? 0 : s->batch + 1);
@@ -552,7 +563,7 @@ int launch_dp(t2sc_seqs *s, const AttnArgs &a, std::string &err) {
   // part keeps at least two key blocks.
   if (pairs >= sms) return launch<DT, DP, 2>(s, a, 1, err);
   int splits = 1;
-  while (splits < 8 && singles * splits * 2 <= 2 * sms && s->max_kv >= (int64_t)4 * splits * kBK) splits *= 2;
+  while (splits < 8 && singles * splits * 2 <= 2 * sms && s->max_kv >= (int64_t)512 * splits) splits *= 2;
   return launch<DT, DP, 1>(s, a, splits, err);
 }
 

@@ -8,21 +8,25 @@
 // off by 3e-5, and any int32 position is allowed here.
 //
 // The operators move their rows once in and once out and do ~10 operations a
-// value, so HBM bounds them if enough bytes are in flight. A CTA takes T
-// rows; a group of g lanes (a power of two) owns one head, every lane the
-// two 16-byte chunks at the same place of the head's two halves, which holds
-// whole pairs in either layout. All loads of up to R heads a group are issued
-// before the CTA's T x pairs sines and cosines are computed into shared
-// memory, so that their latency hides behind them, and one angle serves all
-// heads of q and k.
+// value, so HBM bounds them if enough bytes are in flight and the
+// instructions stay few. A CTA takes T rows; a group of lanes (a power of
+// two) takes up to R heads of one row, every lane two 16-byte chunks at the
+// same place of a head's two halves, which hold whole pairs in either layout.
+// All loads are issued before the CTA's T x pairs sines and cosines are
+// computed into shared memory, so that their latency hides behind them; a
+// lane reads its pairs' once for its R heads. The arithmetic is in packed
+// pairs of f32, one instruction for two values.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <cmath>
+#include <type_traits>
 #include <vector>
 
 #include "entry.h"
 #include "internal.h"
+#include "sm100.cuh"
 
 struct t2sc_rope {
   t2sc_ctx *ctx = nullptr;
@@ -34,7 +38,7 @@ struct t2sc_rope {
 namespace t2sc {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 constexpr int kMaxHeadDim = 256;
 
 struct RopeArgs {
@@ -60,34 +64,41 @@ __device__ __forceinline__ float2 turn_of(const RopeArgs &a, int64_t row, int p)
   return make_float2(c, s);
 }
 
+// 16 bytes <-> packed pairs of f32.
 template <int DT>
-struct Chunk {  // 16 bytes
+struct Chunk {
   static constexpr int kElems = DT == T2SC_DT_F32 ? 4 : 8;
-  __device__ __forceinline__ static void unpack(const uint4 &u, float *f) {
+  __device__ __forceinline__ static void unpack(const uint4 &u, uint64_t *f) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    if (DT == T2SC_DT_F32) {
+      f[0] = sm100::pack_f32x2(__uint_as_float(w[0]), __uint_as_float(w[1]));
+      f[1] = sm100::pack_f32x2(__uint_as_float(w[2]), __uint_as_float(w[3]));
+    } else {
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      if (DT == T2SC_DT_F32) {
-        f[j] = __uint_as_float(w[j]);
-      } else if (DT == T2SC_DT_BF16) {
-        f[2 * j] = __uint_as_float(w[j] << 16), f[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-      } else {
-        const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&w[j]));
-        f[2 * j] = h.x, f[2 * j + 1] = h.y;
+      for (int j = 0; j < 4; j++) {
+        if (DT == T2SC_DT_BF16) {
+          f[j % (kElems / 2)] = sm100::pack_f32x2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u));
+        } else {
+          const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&w[j]));
+          f[j % (kElems / 2)] = sm100::pack_f32x2(h.x, h.y);
+        }
       }
     }
   }
-  __device__ __forceinline__ static uint4 pack(const float *f) {
+  __device__ __forceinline__ static uint4 pack(const uint64_t *f) {
+    float v[kElems];
+#pragma unroll
+    for (int j = 0; j < kElems / 2; j++) sm100::unpack_f32x2(f[j], v[2 * j], v[2 * j + 1]);
     uint32_t w[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
       if (DT == T2SC_DT_F32) {
-        w[j] = __float_as_uint(f[j]);
+        w[j] = __float_as_uint(v[j]);
       } else if (DT == T2SC_DT_BF16) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * j], f[2 * j + 1]);
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j % kElems], v[(2 * j + 1) % kElems]);
         w[j] = *reinterpret_cast<const uint32_t *>(&h);
       } else {
-        const __half2 h = __floats2half2_rn(f[2 * j], f[2 * j + 1]);
+        const __half2 h = __floats2half2_rn(v[2 * j % kElems], v[(2 * j + 1) % kElems]);
         w[j] = *reinterpret_cast<const uint32_t *>(&h);
       }
     }
@@ -96,89 +107,118 @@ struct Chunk {  // 16 bytes
 };
 
 // NORM: RMS norm and gains first. PAIRS: adjacent channels are a pair, else
-// channels j and j + head_dim / 2. R: heads a group holds at once.
+// channels j and j + head_dim / 2. R: heads of a row that a group holds at
+// once; `slots` groups share a row.
 template <int DT, bool NORM, bool PAIRS, int R>
-__global__ void __launch_bounds__(kThreads) rope_vec_kernel(const RopeArgs a, int t_rows, int lanes, int chunks) {
-  constexpr int E = Chunk<DT>::kElems;
-  extern __shared__ float2 turn[];  // [t_rows][rotated]
-  const int groups = kThreads / lanes, gid = (int)threadIdx.x / lanes, sub = (int)threadIdx.x % lanes;
+__global__ void __launch_bounds__(kThreads) rope_vec_kernel(const RopeArgs a, int t_rows, int lanes, int chunks, int slots) {
+  constexpr int E = Chunk<DT>::kElems, H = E / 2;  // values of a chunk, packed pairs of them
+  extern __shared__ float2 turn[];                 // [t_rows][pairs]
+  const int groups = (int)blockDim.x / lanes, gid = (int)threadIdx.x / lanes, sub = (int)threadIdx.x % lanes;
   const int64_t row0 = (int64_t)blockIdx.x * t_rows;
   const int here = (int)min((int64_t)t_rows, a.rows - row0);
-  const int total = here * a.per_row;
-  const int half_bytes = a.head_dim / 2 * (16 / E);
+  const int total = here * slots, pairs = a.head_dim / 2, half = pairs * (16 / E);
   const bool lane_live = sub < chunks;
-  for (int base = 0; base < total; base += groups * R) {
+  // the lane's pairs: H in each half of the head where adjacent channels are pairs, else E
+  const int p0 = PAIRS ? sub * H : sub * E, p1 = PAIRS ? pairs / 2 + p0 : p0 + H;
+  for (int base = 0; base < total; base += groups) {
+    const int w = base + gid, row = w / slots, h0 = (w - row * slots) * R;
+    const bool live = w < total && lane_live;
     uint4 raw[R][2];
-    int vrow[R], vhead[R], vt[R];
 #pragma unroll
     for (int r = 0; r < R; r++) {
-      const int v = base + r * groups + gid;
-      vrow[r] = v < total ? v / a.per_row : -1;
-      const int h = v - vrow[r] * a.per_row;
-      vt[r] = h >= a.heads, vhead[r] = h - vt[r] * a.heads;
-      if (vrow[r] >= 0 && lane_live) {
-        const char *p = a.in[vt[r]] + (row0 + vrow[r]) * a.in_stride[vt[r]] + vhead[r] * 2 * half_bytes + sub * 16;
+      const int t = h0 + r >= a.heads, h = h0 + r - t * a.heads;
+      raw[r][0] = raw[r][1] = make_uint4(0, 0, 0, 0);
+      if (live && h0 + r < a.per_row) {
+        const char *p = a.in[t] + (row0 + row) * a.in_stride[t] + h * 2 * half + sub * 16;
         raw[r][0] = __ldcs(reinterpret_cast<const uint4 *>(p));
-        raw[r][1] = __ldcs(reinterpret_cast<const uint4 *>(p + half_bytes));
-      } else {
-        raw[r][0] = raw[r][1] = make_uint4(0, 0, 0, 0);
+        raw[r][1] = __ldcs(reinterpret_cast<const uint4 *>(p + half));
       }
     }
     if (base == 0) {
-      for (int i = threadIdx.x; i < here * a.rotated; i += kThreads) turn[i] = turn_of(a, row0 + i / a.rotated, i % a.rotated);
+      for (int i = threadIdx.x; i < here * a.rotated; i += blockDim.x)
+        turn[i / a.rotated * pairs + i % a.rotated] = turn_of(a, row0 + i / a.rotated, i % a.rotated);
       __syncthreads();
+    }
+    // Factors of the lane's pairs. PAIRS: (u, v) (c, c) + (v, u) (-s, s), a
+    // pair to a packed value; else u (c) + v (-s) and u (s) + v (c), two pairs
+    // to a packed value. Pairs that do not turn are selected away below.
+    uint64_t f0[E], f1[E];
+    {
+      const float2 *t0 = turn + (live ? row * pairs : 0);
+      float2 cs[E];
+#pragma unroll
+      for (int p = 0; p < E; p++) {
+        const int at = p < H ? p0 + p : p1 + p - H;
+        cs[p] = live && at < a.rotated ? t0[at] : make_float2(1.f, 0.f);
+      }
+      if (PAIRS) {
+#pragma unroll
+        for (int p = 0; p < E; p++) f0[p] = sm100::pack_f32x2(cs[p].x, cs[p].x), f1[p] = sm100::pack_f32x2(-cs[p].y, cs[p].y);
+      } else {
+#pragma unroll
+        for (int p = 0; p < H; p++) {
+          f0[p] = sm100::pack_f32x2(cs[2 * p].x, cs[2 * p + 1].x);
+          f1[p] = sm100::pack_f32x2(cs[2 * p].y, cs[2 * p + 1].y);
+          f1[H + p] = sm100::pack_f32x2(-cs[2 * p].y, -cs[2 * p + 1].y);
+        }
+      }
     }
 #pragma unroll
     for (int r = 0; r < R; r++) {
-      float x[2 * E];
+      const int t = h0 + r >= a.heads, h = h0 + r - t * a.heads;
+      const bool there = live && h0 + r < a.per_row;
+      uint64_t x[E];  // H of the first chunk, H of the second
       Chunk<DT>::unpack(raw[r][0], x);
-      Chunk<DT>::unpack(raw[r][1], x + E);
+      Chunk<DT>::unpack(raw[r][1], x + H);
       if (NORM) {
-        float ss = 0.f;
+        uint64_t ss2 = 0;
 #pragma unroll
-        for (int e = 0; e < 2 * E; e++) ss += x[e] * x[e];
+        for (int e = 0; e < E; e++) ss2 = sm100::fma_f32x2(x[e], x[e], ss2);
+        float ss, s1;
+        sm100::unpack_f32x2(ss2, ss, s1);
+        ss += s1;
         for (int d = lanes >> 1; d > 0; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
         const float inv = rsqrtf(ss * a.inv_dim + a.eps);
-        if (vrow[r] >= 0 && lane_live) {
-          const float *g = a.gain[vt[r]] + vhead[r] * a.head_dim + sub * E;
+        const uint64_t inv2 = sm100::pack_f32x2(inv, inv);
+        if (there) {
+          const float *g = a.gain[t] + h * a.head_dim + sub * E;
 #pragma unroll
           for (int q = 0; q < 2; q++)
 #pragma unroll
             for (int e4 = 0; e4 < E / 4; e4++) {
-              const float4 w = __ldg(reinterpret_cast<const float4 *>(g + q * (a.head_dim / 2)) + e4);
-              float *z = x + q * E + e4 * 4;
-              z[0] *= inv * w.x, z[1] *= inv * w.y, z[2] *= inv * w.z, z[3] *= inv * w.w;
+              const ulonglong2 m = __ldg(reinterpret_cast<const ulonglong2 *>(g + q * pairs) + e4);
+              uint64_t *z = x + q * H + e4 * 2;
+              z[0] = sm100::mul_f32x2(z[0], sm100::mul_f32x2(m.x, inv2));
+              z[1] = sm100::mul_f32x2(z[1], sm100::mul_f32x2(m.y, inv2));
             }
         }
       }
-      if (vrow[r] < 0 || !lane_live) continue;
-      const float2 *t = turn + vrow[r] * a.rotated;
+      if (!there) continue;
+      // pairs that do not turn pass through untouched, infinities and NaN too
       if (PAIRS) {
 #pragma unroll
-        for (int q = 0; q < 2; q++)
-#pragma unroll
-          for (int e = 0; e < E; e += 2) {
-            const int p = (q * (a.head_dim / 2) + sub * E + e) / 2;
-            if (p < a.rotated) {
-              const float2 cs = t[p];
-              const float u = x[q * E + e], v = x[q * E + e + 1];
-              x[q * E + e] = u * cs.x - v * cs.y, x[q * E + e + 1] = u * cs.y + v * cs.x;
-            }
-          }
+        for (int p = 0; p < E; p++) {
+          float u, v;
+          sm100::unpack_f32x2(x[p], u, v);
+          const uint64_t y = sm100::fma_f32x2(x[p], f0[p], sm100::mul_f32x2(sm100::pack_f32x2(v, u), f1[p]));
+          x[p] = (p < H ? p0 + p : p1 + p - H) < a.rotated ? y : x[p];
+        }
       } else {
 #pragma unroll
-        for (int e = 0; e < E; e++) {
-          const int p = sub * E + e;
-          if (p < a.rotated) {
-            const float2 cs = t[p];
-            const float u = x[e], v = x[E + e];
-            x[e] = u * cs.x - v * cs.y, x[E + e] = u * cs.y + v * cs.x;
-          }
+        for (int p = 0; p < H; p++) {
+          const uint64_t u = sm100::fma_f32x2(x[p], f0[p], sm100::mul_f32x2(x[H + p], f1[H + p]));
+          const uint64_t v = sm100::fma_f32x2(x[p], f1[p], sm100::mul_f32x2(x[H + p], f0[p]));
+          float u0, u1, v0, v1, k0, k1, m0, m1;
+          sm100::unpack_f32x2(u, u0, u1), sm100::unpack_f32x2(v, v0, v1);
+          sm100::unpack_f32x2(x[p], k0, k1), sm100::unpack_f32x2(x[H + p], m0, m1);
+          const bool a0 = p0 + 2 * p < a.rotated, a1 = p0 + 2 * p + 1 < a.rotated;
+          x[p] = sm100::pack_f32x2(a0 ? u0 : k0, a1 ? u1 : k1);
+          x[H + p] = sm100::pack_f32x2(a0 ? v0 : m0, a1 ? v1 : m1);
         }
       }
-      char *p = a.out[vt[r]] + (row0 + vrow[r]) * a.out_stride[vt[r]] + vhead[r] * 2 * half_bytes + sub * 16;
+      char *p = a.out[t] + (row0 + row) * a.out_stride[t] + h * 2 * half + sub * 16;
       __stcs(reinterpret_cast<uint4 *>(p), Chunk<DT>::pack(x));
-      __stcs(reinterpret_cast<uint4 *>(p + half_bytes), Chunk<DT>::pack(x + E));
+      __stcs(reinterpret_cast<uint4 *>(p + half), Chunk<DT>::pack(x + H));
     }
   }
 }
@@ -247,7 +287,6 @@ __global__ void __launch_bounds__(kThreads) rope_scalar_kernel(const RopeArgs a)
 
 template <int DT, bool NORM, bool PAIRS>
 int launch(t2sc_ctx *ctx, const RopeArgs &a, std::string &err) {
-  const int es = DT == T2SC_DT_F32 ? 4 : 2;
   constexpr int E = Chunk<DT>::kElems;
   bool vec = a.head_dim % (2 * E) == 0;
   for (int t = 0; t < (a.per_row > a.heads ? 2 : 1); t++) {
@@ -255,28 +294,35 @@ int launch(t2sc_ctx *ctx, const RopeArgs &a, std::string &err) {
     if (off(a.in[t]) || off(a.out[t]) || a.in_stride[t] % 16 || a.out_stride[t] % 16 || (NORM && off(a.gain[t]))) vec = false;
   }
   if (vec) {
-    constexpr int R = 4;
     const int chunks = a.head_dim / 2 / E;
     int lanes = 1;
     while (lanes < chunks) lanes <<= 1;
-    // Rows a CTA takes: as many as its groups hold at once (R heads each), so
-    // that one angle serves all heads; fewer when that would leave SMs idle.
-    const int held = kThreads / lanes * R;
-    int64_t t_rows = held / a.per_row;
-    if (t_rows > 16) t_rows = 16;
-    while (t_rows > 1 && (a.rows + t_rows - 1) / t_rows < 2 * ctx->num_sms) t_rows--;
-    if (t_rows < 1) t_rows = 1;
-    const int64_t grid = (a.rows + t_rows - 1) / t_rows;
-    if (grid <= INT32_MAX) {
-      const size_t smem = (size_t)t_rows * a.rotated * sizeof(float2);  // <= 16 x 128 x 8 bytes
-      rope_vec_kernel<DT, NORM, PAIRS, R><<<(unsigned)grid, kThreads, smem, ctx->stream>>>(a, (int)t_rows, lanes, chunks);
+    auto go = [&](auto rc) -> int {
+      constexpr int R = decltype(rc)::value;
+      // Rows a CTA takes: as many as its groups hold at once; fewer when that
+      // would leave SMs idle. No more threads than these rows have groups for
+      // (12 heads of 128, q and k: 2 rows on 96 threads).
+      const int slots = (a.per_row + R - 1) / R, row_threads = slots * lanes;
+      int64_t t_rows = std::max(1, std::min(16, kThreads / row_threads));
+      while (t_rows > 1 && (a.rows + t_rows - 1) / t_rows < 2 * ctx->num_sms) t_rows--;
+      const int threads = (int)std::min<int64_t>(kThreads, (t_rows * row_threads + 31) / 32 * 32);
+      const int64_t grid = (a.rows + t_rows - 1) / t_rows;
+      const size_t smem = (size_t)t_rows * (a.head_dim / 2) * sizeof(float2);  // <= 16 x 128 x 8 bytes
+      rope_vec_kernel<DT, NORM, PAIRS, R><<<(unsigned)grid, threads, smem, ctx->stream>>>(a, (int)t_rows, lanes, chunks, slots);
       T2SC_LAUNCHED(ctx, "rope");
       return T2SC_OK;
-    }
+    };
+    // Heads a group holds: four (bf16 [100003, 12, 128] q and k 266 us, with
+    // two 282, one 286) while that leaves threads for every SM; with fewer
+    // rows fewer ([1941, 12, 128]: 12.4 us with four, 9.9 with two).
+    const int64_t enough = (int64_t)1024 * ctx->num_sms;
+    auto threads_with = [&](int r) { return a.rows * ((a.per_row + r - 1) / r) * lanes; };
+    if (a.per_row >= 4 && threads_with(4) >= enough) return go(std::integral_constant<int, 4>());
+    if (a.per_row >= 2 && threads_with(2) >= enough) return go(std::integral_constant<int, 2>());
+    return go(std::integral_constant<int, 1>());
   }
   const int64_t warps = a.rows * a.per_row, grid = (warps + kThreads / 32 - 1) / (kThreads / 32);
   if (grid > INT32_MAX) return fail(ctx, T2SC_ERR_UNSUPPORTED, "rope: too many heads in one call");
-  (void)es;
   rope_scalar_kernel<DT, NORM, PAIRS><<<(unsigned)grid, kThreads, 0, ctx->stream>>>(a);
   T2SC_LAUNCHED(ctx, "rope");
   return T2SC_OK;
