@@ -109,7 +109,8 @@ def test_linear_unaligned(t2sc, shift_x, shift_w, shift_y, ci, rows):
     ref.assert_close(t2sc.dense_linear_device(x, w, out=out), *ref.linear(x, w))
 
 
-@pytest.mark.parametrize("rows,ci,co", [(1, 4096, 1024), (4, 1024, 4608), (40, 4096, 1024), (1941, 1536, 768), (2500, 512, 2304)])
+@pytest.mark.parametrize("rows,ci,co", [(1, 4096, 1024), (2, 1000, 517), (3, 4096, 1024), (4, 1024, 4608), (17, 2000, 300), (40, 4096, 1024),
+                                        (64, 4096, 130), (100, 1040, 777), (128, 8192, 128), (1941, 1536, 768), (2500, 512, 2304)])
 def test_linear_larger(t2sc, rows, ci, co):
     g = _gen(9)
     x, w, b = _normal(g, rows, ci, dtype="bfloat16"), _normal(g, co, ci, std=ci ** -0.5, dtype="bfloat16"), _normal(g, co)

@@ -11,7 +11,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "build")
 OUT = os.path.join(HERE, "t2sc", "libt2sc.so")
-SOURCES = ["api.cu", "hashmap.cu", "scan.cu", "conv_tc.cu", "conv_simt.cu", "convert.cu", "subdiv.cu", "selftest.cu", "norm.cu", "dist.cu", "block.cu", "pipeline.cu", "dense.cu", "dense_tc.cu", "dense_rows.cu",
+SOURCES = ["api.cu", "hashmap.cu", "scan.cu", "conv_tc.cu", "conv_simt.cu", "convert.cu", "subdiv.cu", "selftest.cu", "norm.cu", "dist.cu", "block.cu", "pipeline.cu", "dense.cu", "dense_tc.cu", "dense_rows.cu", "dense_skinny.cu",
            "rope.cu", "attention.cu", "attention_tc.cu", "attention_rows.cu", "synth.cpp"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 

@@ -37,7 +37,10 @@ __device__ __forceinline__ float activate(float v, int act) {
 // 16-bit rows that start on 16 bytes (what TMA needs of x and w).
 bool dense_tc_takes(const DenseArgs &a, int dtype);
 int dense_tc(t2sc_ctx *ctx, const DenseArgs &a, int dtype, std::string &err);
-// At most 8 such rows, ci a multiple of 8.
+// Such rows, few of them.
+bool dense_skinny_takes(t2sc_ctx *ctx, const DenseArgs &a, int dtype);
+int dense_skinny(t2sc_ctx *ctx, const DenseArgs &a, int dtype, std::string &err);
+// At most 2 such rows, ci a multiple of 8.
 bool dense_rows_takes(const DenseArgs &a, int dtype);
 int dense_rows(t2sc_ctx *ctx, const DenseArgs &a, int dtype, std::string &err);
 int dense_simt(t2sc_ctx *ctx, const DenseArgs &a, int dtype, std::string &err);

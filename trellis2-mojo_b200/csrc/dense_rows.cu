@@ -19,7 +19,7 @@
 namespace t2sc {
 namespace {
 
-constexpr int kWarps = 8, kOut = 4;
+constexpr int kMaxRows = 2, kWarps = 8, kOut = 4;
 
 template <int DT>
 __device__ __forceinline__ void unpack8(const uint4 &u, float (&f)[8]) {
@@ -117,19 +117,15 @@ int launch(t2sc_ctx *ctx, const DenseArgs &a, std::string &err) {
   const unsigned grid = (unsigned)((out_groups + kWarps / slices - 1) / (kWarps / slices));
   if (a.rows == 1)
     dense_rows_kernel<DT, 1, 3><<<grid, 32 * kWarps, 0, ctx->stream>>>(a, slices);
-  else if (a.rows == 2)
-    dense_rows_kernel<DT, 2, 2><<<grid, 32 * kWarps, 0, ctx->stream>>>(a, slices);
-  else if (a.rows <= 4)
-    dense_rows_kernel<DT, 4, 2><<<grid, 32 * kWarps, 0, ctx->stream>>>(a, slices);
   else
-    dense_rows_kernel<DT, 8, 2><<<grid, 32 * kWarps, 0, ctx->stream>>>(a, slices);
+    dense_rows_kernel<DT, 2, 2><<<grid, 32 * kWarps, 0, ctx->stream>>>(a, slices);
   T2SC_LAUNCHED(ctx, "dense_linear");
   return T2SC_OK;
 }
 
 }  // namespace
 
-bool dense_rows_takes(const DenseArgs &a, int dtype) { return dense_tc_takes(a, dtype) && a.rows <= 8 && a.ci % 8 == 0; }
+bool dense_rows_takes(const DenseArgs &a, int dtype) { return dense_tc_takes(a, dtype) && a.rows <= kMaxRows && a.ci % 8 == 0; }
 
 int dense_rows(t2sc_ctx *ctx, const DenseArgs &a, int dtype, std::string &err) {
   return dtype == T2SC_DT_BF16 ? launch<T2SC_DT_BF16>(ctx, a, err) : launch<T2SC_DT_F16>(ctx, a, err);
