@@ -9,7 +9,7 @@
 // stages only half of the w tile, which halves what shared memory has to
 // take in and feed for w. The CTAs are persistent; a CTA's tiles are `slots`
 // apart with the columns fastest, so that the tiles in flight share their x
-// rows and the whole of w in L2.
+// rows and a band of w in L2.
 //
 // The epilogue takes 64 columns at a time: a thread owns a row (TMEM lane),
 // and the block passes through a swizzled 4 KB of shared memory per warp so
@@ -17,6 +17,8 @@
 // the residual: each element is read before the same thread writes it.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <algorithm>
 
 #include "dense.h"
 #include "entry.h"
@@ -42,7 +44,7 @@ struct DenseTcArgs {
   const float *bias;
   int64_t ldr, ldy;  // elements
   int64_t rows;
-  int co, k_iters, act, m_tiles, n_tiles, slots;
+  int co, k_iters, act, m_tiles, n_tiles, band, slots;
   int vec;  // y (and residual) rows start on 16 bytes
   int *err;
 };
@@ -117,24 +119,29 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
   const uint32_t tmem = *tmem_slot;
   const int64_t ntiles = (int64_t)a.m_tiles * a.n_tiles;
   const int64_t slot = blockIdx.x / CG;
+  // Tile t: blocks of `band` column tiles (what of w stays in L2 beside x),
+  // rows by rows inside a band, the columns fastest.
+  auto place = [&](int64_t t, int &m, int &n) {
+    const int64_t per_band = (int64_t)a.band * a.m_tiles;
+    const int first = (int)(t / per_band) * a.band, width = min(a.band, a.n_tiles - first);
+    const int64_t i = t % per_band;
+    m = (int)(i / width), n = first + (int)(i % width);
+  };
 
   if (warp == kTmaWarp) {
     // ------------------------------- TMA --------------------------------
     if (lane == 0) {
       sm100::tma_prefetch(&a.map_x);
       sm100::tma_prefetch(&a.map_w);
-    }
-    uint32_t s = 0, ph = 0, it = 0;
-    bool ok = true;
-    for (int64_t t = slot; t < ntiles && ok; t += a.slots) {
-      const int m0 = (int)(t / a.n_tiles) * kTileM * CG + (int)rank * kTileM;
-      const int n0 = (int)(t % a.n_tiles) * BN + (int)rank * S::kWRows;
-      for (int k = 0; k < a.k_iters; k++) {
-        if (!warp_wait(empty0 + 8 * s, ph ^ 1, abort, a.err)) {
-          ok = false;
-          break;
-        }
-        if (lane == 0) {
+      uint32_t s = 0, ph = 0, it = 0;
+      bool ok = true;
+      for (int64_t t = slot; t < ntiles && ok; t += a.slots) {
+        int m, nt;
+        place(t, m, nt);
+        const int m0 = m * kTileM * CG + (int)rank * kTileM, n0 = nt * BN + (int)rank * S::kWRows;
+        for (int k = 0; k < a.k_iters; k++) {
+          ok = sm100::mbar_wait_bounded(empty0 + 8 * s, ph ^ 1, abort, a.err, kDevErrTimeout, kWaitLimit);
+          if (!ok) break;
           const uint32_t dst = sbase + s * S::kStage;
           if (CG == 2) {
             const uint32_t bar = sm100::map_to_rank(full0 + 8 * s, 0);  // CTA 0 waits for both CTAs' tiles
@@ -146,69 +153,64 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
             sm100::tma_load_2d(dst, &a.map_x, k * kBK, m0, full0 + 8 * s);
             sm100::tma_load_2d(dst + S::kABytes, &a.map_w, k * kBK, n0, full0 + 8 * s);
           }
+          it++;
+          if (++s == NS) s = 0, ph ^= 1;
         }
-        __syncwarp();
-        it++;
-        if (++s == NS) s = 0, ph ^= 1;
       }
-    }
-    // every copy asked for has landed before shared memory is given up (a
-    // pair's land on CTA 0's barriers, and CTA 1 stays until the cluster's end)
-    if (lane == 0 && rank == 0) {
-      const uint32_t first = it > (uint32_t)NS ? it - NS : 0;
-      for (uint32_t i = first; i < it; i++)
-        sm100::mbar_wait_cycles(full0 + 8 * (i % NS), (i / NS) & 1, kWaitLimit / 8);
+      // every copy asked for has landed before shared memory is given up (a
+      // pair's land on CTA 0's barriers, and CTA 1 stays until the cluster's end)
+      if (rank == 0)
+        for (uint32_t i = it > (uint32_t)NS ? it - NS : 0; i < it; i++)
+          sm100::mbar_wait_cycles(full0 + 8 * (i % NS), (i / NS) & 1, kWaitLimit / 8);
     }
     __syncwarp();
   } else if (warp == kMmaWarp) {
     // ------------------------------- MMA --------------------------------
-    if (rank == 0) {
-      const uint32_t idesc = sm100::instr_desc(DT == T2SC_DT_BF16 ? 1 : 0, BN) + (CG == 2 ? (128u >> 4) << 24 : 0u);
-      const uint64_t da0 = sm100::smem_desc(sbase, 128), db0 = sm100::smem_desc(sbase + S::kABytes, 128);
+    if (rank == 0 && sm100::elect_one()) {
+      constexpr uint32_t idesc = sm100::instr_desc(DT == T2SC_DT_BF16 ? 1 : 0, BN) + (CG == 2 ? (128u >> 4) << 24 : 0u);
+      const uint64_t da0 = sm100::smem_desc(sbase, 128);
+      const uint32_t hi = (uint32_t)(da0 >> 32), a_lo = (uint32_t)da0, b_lo = a_lo + (S::kABytes >> 4);
       uint32_t s = 0, ph = 0, acc = 0;
       bool ok = true;
+      auto wait = [&](uint32_t bar, uint32_t parity) {
+        ok = ok && sm100::mbar_wait_bounded(bar, parity, abort, a.err, kDevErrTimeout, kWaitLimit);
+      };
+      auto commit = [&](uint32_t bar) {
+        if (CG == 2)
+          sm100::mma_commit_pair(bar);
+        else
+          sm100::mma_commit(bar);
+      };
       for (int64_t t = slot; t < ntiles && ok; t += a.slots) {
         const uint32_t b = acc & 1;
-        if (!warp_wait(tempty0 + 8 * b, ((acc >> 1) & 1) ^ 1, abort, a.err)) break;
+        wait(tempty0 + 8 * b, ((acc >> 1) & 1) ^ 1);
         if (CG == 2) asm volatile("fence.acq_rel.cluster;" ::: "memory");  // half of the arrivals are the other CTA's
         sm100::tc_fence_after();
         const uint32_t d = tmem + b * BN;
-        for (int k = 0; k < a.k_iters; k++) {
-          if (!warp_wait(full0 + 8 * s, ph, abort, a.err)) {
-            ok = false;
-            break;
-          }
+        for (int k = 0; k < a.k_iters && ok; k++) {
+          wait(full0 + 8 * s, ph);
+          if (!ok) break;
           sm100::tc_fence_after();
-          const uint64_t so = (uint64_t)(s * S::kStage) >> 4;
+          const uint32_t at = s * (S::kStage >> 4);
 #pragma unroll
           for (int kk = 0; kk < kBK / 16; kk++) {
-            const uint64_t da = da0 + so + kk * 2, db = db0 + so + kk * 2;
             if (CG == 2)
-              sm100::mma_f16_pair_elect(d, da, db, idesc, k + kk > 0);
+              sm100::mma_f16_pair_lo(d, a_lo + at + kk * 2, b_lo + at + kk * 2, hi, idesc, k + kk > 0);
             else
-              sm100::mma_f16_elect(d, da, db, idesc, k + kk > 0);
+              sm100::mma_f16_lo(d, a_lo + at + kk * 2, b_lo + at + kk * 2, hi, idesc, k + kk > 0);
           }
-          if (CG == 2)
-            sm100::mma_commit_pair_elect(empty0 + 8 * s);
-          else
-            sm100::mma_commit_elect(empty0 + 8 * s);
+          commit(empty0 + 8 * s);
           if (++s == NS) s = 0, ph ^= 1;
         }
         if (!ok) break;
-        if (CG == 2)
-          sm100::mma_commit_pair_elect(tfull0 + 8 * b);
-        else
-          sm100::mma_commit_elect(tfull0 + 8 * b);
+        commit(tfull0 + 8 * b);
         acc++;
       }
       // all issued MMAs retire before TMEM and shared memory are given up
-      if (CG == 2)
-        sm100::mma_commit_pair_elect(done);
-      else
-        sm100::mma_commit_elect(done);
-      if (lane == 0) sm100::mbar_wait_cycles(done, 0, kWaitLimit / 8);
-      __syncwarp();
+      commit(done);
+      sm100::mbar_wait_cycles(done, 0, kWaitLimit / 8);
     }
+    __syncwarp();
   } else {
     // ----------------------------- epilogue -----------------------------
     // Warp w reads TMEM lanes 32 (w % 4)..; the two warps of a quadrant take
@@ -219,8 +221,10 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
     uint32_t acc = 0;
     const int crow = lane >> 3, cch = lane & 7;  // this lane's place when whole rows move: 4 rows x 8 chunks
     for (int64_t t = slot; t < ntiles; t += a.slots) {
-      const int64_t row0 = (t / a.n_tiles) * (kTileM * CG) + (int64_t)rank * kTileM + quad * 32;
-      const int n0 = (int)(t % a.n_tiles) * BN;
+      int m, nt;
+      place(t, m, nt);
+      const int64_t row0 = (int64_t)m * (kTileM * CG) + (int64_t)rank * kTileM + quad * 32;
+      const int n0 = nt * BN;
       const uint32_t b = acc & 1;
       // the first block's bias and residual come in while the tile is still computed
       float bias0, bias1;
@@ -370,6 +374,9 @@ int launch(t2sc_ctx *ctx, const DenseArgs &a, std::string &err) {
   t.m_tiles = (int)((a.rows + kTileM * CG - 1) / (kTileM * CG)), t.n_tiles = (a.co + BN - 1) / BN;
   auto on16 = [&](const void *p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (a.rows <= 1 || ld % 8 == 0); };
   t.vec = on16(a.y, a.ldy) && (!a.res || on16(a.res, a.ldr));
+  // 32 MB of w a band
+  const int64_t column_tile = (int64_t)BN * a.ci * 2;
+  t.band = (int)std::min<int64_t>(t.n_tiles, std::max<int64_t>(1, ((int64_t)32 << 20) / column_tile));
   const int64_t tiles = (int64_t)t.m_tiles * t.n_tiles, most = ctx->num_sms / CG;
   t.slots = (int)(tiles < most ? tiles : most);
   auto kernel = dense_tc_kernel<DT, CG, BN>;
