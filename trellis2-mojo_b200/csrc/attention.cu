@@ -193,6 +193,10 @@ int t2sc_seqs_create(t2sc_ctx *ctx, const int64_t *q_offsets, const int64_t *kv_
       s->max_q = std::max<int64_t>(s->max_q, sorted[b].y);
       s->max_kv = std::max<int64_t>(s->max_kv, sorted[b].w);
     }
+    for (int64_t b = 0; b <= 8; b++) {
+      s->few_blocks256[b] = b <= batch ? blocks[b] : 0, s->few_blocks128[b] = b <= batch ? blocks[batch + 1 + b] : 0;
+      if (b < 8) s->few_seqs[b] = b < batch ? sorted[b] : make_int4(0, 0, 0, 0);
+    }
     s->blocks256 = blocks[batch], s->blocks128 = blocks[2 * batch + 1];
     // one allocation: sequences in order, sorted, block counts
     const size_t nb = (size_t)batch + 1, bytes = 2 * nb * sizeof(int4) + blocks.size() * sizeof(int64_t);

@@ -17,6 +17,9 @@ struct t2sc_seqs {
   int64_t blocks128 = 0, blocks256 = 0;  // blocks of 128 / 256 query rows, sequence by sequence
   int4 *d_sorted = nullptr;            // as d_seqs, most keys first
   int64_t *d_blocks = nullptr;         // [2][batch + 1] blocks of 256 / 128 rows before each sequence of d_sorted
+  // the first sequences of d_sorted and d_blocks, for kernels to carry in their arguments
+  int4 few_seqs[8];
+  int64_t few_blocks256[9], few_blocks128[9];
   int4 *d_seqs = nullptr;              // [batch] first query row, query rows, first key row, key rows
 };
 

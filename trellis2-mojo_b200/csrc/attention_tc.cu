@@ -2,7 +2,7 @@
 // 16 bytes and head dims that are multiples of 8 up to 128.
 //
 // A CTA owns NT blocks of 128 queries of one head and walks its sequence's
-// keys. TMA brings the query blocks once and blocks of K and V rows
+// keys. TMA brings the query blocks once and blocks of 128 K and V rows
 // through a ring of shared-memory slots (heads are a dimension of the tensor
 // map: channels past head_dim read as zero). One thread issues the
 // products, for a unit of 64 keys at a time:
@@ -49,7 +49,7 @@
 namespace t2sc {
 namespace {
 
-constexpr int kBQ = 128, kUnit = 64;
+constexpr int kBQ = 128, kBK = 128, kUnit = 64, kFew = 8, kMaxSplits = 8;
 constexpr long long kWaitLimit = 4000000000ll;  // ~2 s of SM clocks
 
 struct TcArgs {
@@ -61,31 +61,25 @@ struct TcArgs {
   int batch, heads, head_dim, splits;
   float c;  // scale * log2(e)
   int *err;
+  // seqs and blocks of a batch of up to kFew sequences: no memory read away
+  int4 few_seqs[kFew];
+  int few_blocks[kFew + 1];
 };
 
 template <int DP, int NT>
 struct Shape {
-  static constexpr int kTile = kBQ * DP * 2;  // bytes of a query block
-  // Keys of a K or V block: two units, or one where two CTAs' shared memory
-  // would leave a ring of only two slots (300 queries over 20000 keys,
-  // 12 x 128: RINGT us).
-  static constexpr int kBK = NT == 1 && DP == 128 ? 64 : 128, kUB = kBK / kUnit;
-  static constexpr int kSlot = kBK * DP * 2, kHalf = kBK * 128;  // bytes of a slot, of its 64-channel half
-  static constexpr int kSlots = NT == 2 ? (DP == 128 ? 5 : 8) : 4;
+  static constexpr int kTile = 128 * DP * 2;  // bytes of a 128-row block
+  static constexpr int kSlots = NT == 2 ? (DP == 128 ? 5 : 8) : (DP == 128 ? 2 : 4);
   static constexpr int kExtra = 2048;         // barriers, m and l of the rows
-  static constexpr size_t kSmem = 1024 + (size_t)NT * kTile + (size_t)kSlots * kSlot + kExtra;
+  static constexpr size_t kSmem = 1024 + (size_t)(NT + kSlots) * kTile + kExtra;
   static constexpr int kThreads = 128 * (NT + 1);
   static constexpr uint32_t kCols = NT == 2 ? 512 : 256;
-  // Query blocks whose units join one barrier. At head_dim 128 the products
-  // bound the kernel and every wait of their thread counts: both blocks join
-  // one. Below, the exponentials do, and the two blocks' softmaxes should not
-  // want them at the same time: one each (23024 tokens, 16 x 64: JOINED ms).
-  static constexpr int kGroups = DP == 128 ? 1 : NT;
 };
 
-// Bounded wait of a whole warp, its verdict the same in every lane.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *abort, int *err) {
-  const bool ok = sm100::mbar_wait_bounded(bar, parity, abort, err, kDevErrTimeout, kWaitLimit);
+  bool ok = sm100::mbar_test_wait(bar, parity);
+  if (__all_sync(0xffffffffu, ok)) return true;
+  if (!ok) ok = sm100::mbar_wait_bounded(bar, parity, abort, err, kDevErrTimeout, kWaitLimit);
   return __all_sync(0xffffffffu, ok);
 }
 
@@ -115,24 +109,29 @@ __device__ __forceinline__ float ld_cluster1(uint32_t addr) {
 template <int DT, int DP, int NT>
 __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) attention_tc_kernel(const __grid_constant__ TcArgs a) {
   using S = Shape<DP, NT>;
-  constexpr int NS = S::kSlots, kSub = DP / 64, kBK = S::kBK, kUB = S::kUB;
+  constexpr int NS = S::kSlots, kSub = DP / 64;
   constexpr float kSlack = DT == T2SC_DT_F16 ? 7.f : 8.f, kLift = DT == T2SC_DT_F16 ? 8.f : 0.f;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t *ring = smem + NT * S::kTile;
-  float *row_m = reinterpret_cast<float *>(ring + NS * S::kSlot), *row_l = row_m + 128;  // split sums
+  float *row_m = reinterpret_cast<float *>(ring + NS * S::kTile), *row_l = row_m + 128;  // split sums
   uint64_t *bars = reinterpret_cast<uint64_t *>(row_l + 128);
-  // bars: q_full[NT], s_full[NT][2], o_prev[NT], o_full[NT], ready[kGroups][2], full[NS], empty[NS]
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 5 * NT + 2 * S::kGroups + 2 * NS);
+  // bars: q_full[NT], s_full[NT][2], o_prev[NT], o_full[NT], ready[2], full[NS], empty[NS]
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 5 * NT + 2 + 2 * NS);
   volatile int *abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
   int *where = reinterpret_cast<int *>(tmem_slot + 2);  // the CTA's work
   const uint32_t qsm = sm100::smem_u32(smem), rsm = sm100::smem_u32(ring), bar0 = sm100::smem_u32(bars);
   const uint32_t q_full = bar0, s_full = q_full + 8 * NT, o_prev = s_full + 16 * NT, o_full = o_prev + 8 * NT;
-  const uint32_t ready = o_full + 8 * NT, full0 = ready + 16 * S::kGroups, empty0 = full0 + 8 * NS;
+  const uint32_t ready = o_full + 8 * NT, full0 = ready + 16, empty0 = full0 + 8 * NS;
   // lane 0's value is every lane's: the compiler may keep it in uniform registers
   const int warp = uniform((int)threadIdx.x >> 5), lane = threadIdx.x & 31, wg = warp >> 2;
   constexpr int kTmaWarp = 4 * NT, kMmaWarp = 4 * NT + 1, kFeedWarp = 4 * NT + 2;
 
+  if (warp == kTmaWarp && lane == 0) {
+    sm100::tma_prefetch(&a.map_q);
+    sm100::tma_prefetch(&a.map_k);
+    sm100::tma_prefetch(&a.map_v);
+  }
   if (threadIdx.x == 0) {
     for (int i = 0; i < NT; i++) {
       sm100::mbar_init(q_full + 8 * i, 1);
@@ -141,18 +140,27 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
       sm100::mbar_init(o_full + 8 * i, 1);
     }
     // the CTA's sequence, head and query block: blocks of a head are neighbours, heads of a sequence follow
-    const int64_t id = blockIdx.x / a.splits;
-    int lo = 0, hi = a.batch - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (__ldg(a.blocks + mid) * a.heads <= id)
-        lo = mid;
-      else
-        hi = mid - 1;
+    const int id = (int)blockIdx.x / a.splits;
+    int4 seq;
+    int first, n;
+    if (a.batch <= kFew) {
+      int lo = 0;
+      while (lo + 1 < a.batch && a.few_blocks[lo + 1] * a.heads <= id) lo++;
+      seq = a.few_seqs[lo];
+      first = a.few_blocks[lo], n = a.few_blocks[lo + 1] - first;
+    } else {
+      int lo = 0, hi = a.batch - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (__ldg(a.blocks + mid) * a.heads <= id)
+          lo = mid;
+        else
+          hi = mid - 1;
+      }
+      seq = __ldg(a.seqs + lo);
+      first = (int)__ldg(a.blocks + lo), n = (int)__ldg(a.blocks + lo + 1) - first;
     }
-    const int64_t first = __ldg(a.blocks + lo), n = __ldg(a.blocks + lo + 1) - first, local = id - first * a.heads;
-    const int4 seq = __ldg(a.seqs + lo);
-    const int head = (int)(local / n), block = (int)(local % n);
+    const int local = id - first * a.heads, head = local / n, block = local - head * n;
     where[0] = head;
     where[1] = seq.x + block * (NT * kBQ);          // first query row
     where[2] = seq.y - block * (NT * kBQ);          // query rows left
@@ -162,10 +170,8 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
       sm100::mbar_init(full0 + 8 * s, 1);
       sm100::mbar_init(empty0 + 8 * s, 1);
     }
-    // a unit's P (4 warps a query block), and its V and the next K
-    const bool second = NT == 2 && where[2] > kBQ;
-    for (int g = 0; g < S::kGroups; g++)
-      for (int b = 0; b < 2; b++) sm100::mbar_init(ready + 16 * g + 8 * b, (second && S::kGroups == 1 ? 8 : 4) + 1);
+    // a unit's P of every query block (4 warps each), and its V and the next K
+    for (int b = 0; b < 2; b++) sm100::mbar_init(ready + 8 * b, (NT == 2 && where[2] > kBQ ? 8 : 4) + 1);
     *abort = 0;
     sm100::fence_mbar_init();
   }
@@ -206,10 +212,10 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
           break;
         }
         if (lane == 0) {
-          sm100::mbar_arrive_expect_tx(full0 + 8 * s, S::kSlot);
+          sm100::mbar_arrive_expect_tx(full0 + 8 * s, S::kTile);
           const void *map = j & 1 ? &a.map_v : &a.map_k;
           for (int h = 0; h < kSub; h++)
-            sm100::tma_load_3d(rsm + s * S::kSlot + h * S::kHalf, map, h * 64, head, kv0 + (t0 + (j >> 1)) * kBK, full0 + 8 * s);
+            sm100::tma_load_3d(rsm + s * S::kTile + h * 16384, map, h * 64, head, kv0 + (t0 + (j >> 1)) * kBK, full0 + 8 * s);
         }
         __syncwarp();
         it++;
@@ -237,41 +243,36 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
         // descriptors: both operands' high words are the same (1024 bytes between 8-row atoms, 128-byte swizzle)
         const uint64_t dq0 = sm100::smem_desc(qsm, 128);
         const uint32_t hi = (uint32_t)(dq0 >> 32), q_lo = (uint32_t)dq0, k_lo = (uint32_t)sm100::smem_desc(rsm, 128),
-                       v_lo = (uint32_t)sm100::smem_desc_mn(rsm, S::kHalf);
-        constexpr uint32_t kTile16 = S::kTile >> 4, kSlot16 = S::kSlot >> 4, kHalf16 = S::kHalf >> 4, kUnit16 = kUnit * 128 >> 4;
+                       v_lo = (uint32_t)sm100::smem_desc_mn(rsm, 16384);
+        constexpr uint32_t kTile16 = S::kTile >> 4, kUnit16 = kUnit * 128 >> 4;
         bool ok = true;
         auto wait = [&](uint32_t bar, uint32_t parity) {
           ok = ok && sm100::mbar_wait_bounded(bar, parity, abort, a.err, kDevErrTimeout, kWaitLimit);
           sm100::tc_fence_after();
         };
-        auto scores = [&](int i, int b, uint32_t kslot, bool done) {  // S into buffer b; b is the unit's place in a block of two
-          const uint32_t dq = q_lo + i * kTile16, dk = k_lo + kslot * kSlot16 + (kUB == 2 ? b * kUnit16 : 0),
-                         d = s_tmem + i * 128 + b * kUnit;
+        auto scores = [&](int i, int b, uint32_t kslot, bool done) {  // S into buffer b = the unit's half of its block
+          const uint32_t dq = q_lo + i * kTile16, dk = k_lo + kslot * kTile16 + b * kUnit16, d = s_tmem + i * 128 + b * kUnit;
           if (ksteps == DP / 16) {
 #pragma unroll
             for (int kk = 0; kk < DP / 16; kk++)
-              sm100::mma_f16_lo(d, dq + (kk >> 2) * 1024 + (kk & 3) * 2, dk + (kk >> 2) * kHalf16 + (kk & 3) * 2, hi, idesc_s, kk > 0);
+              sm100::mma_f16_lo(d, dq + (kk >> 2) * 1024 + (kk & 3) * 2, dk + (kk >> 2) * 1024 + (kk & 3) * 2, hi, idesc_s, kk > 0);
           } else {
 #pragma unroll 1
             for (int kk = 0; kk < ksteps; kk++)
-              sm100::mma_f16_lo(d, dq + (kk >> 2) * 1024 + (kk & 3) * 2, dk + (kk >> 2) * kHalf16 + (kk & 3) * 2, hi, idesc_s, kk > 0);
+              sm100::mma_f16_lo(d, dq + (kk >> 2) * 1024 + (kk & 3) * 2, dk + (kk >> 2) * 1024 + (kk & 3) * 2, hi, idesc_s, kk > 0);
           }
           sm100::mma_commit(s_full + 16 * i + 8 * b);
           if (done && i == nt - 1) sm100::mma_commit(empty0 + 8 * kslot);  // the block's last unit, for the last query block
         };
-        // ring position of the V block at hand, and of the K block of two units on (block j's loads are 2 j and 2 j + 1)
-        uint32_t vslot = 1, kslot = kUB == 2 ? 2 : 4 % NS;
-        auto next_block = [&]() {
-          vslot = vslot + 2 >= NS ? vslot + 2 - NS : vslot + 2;
-          kslot = kslot + 2 >= NS ? kslot + 2 - NS : kslot + 2;
-        };
+        // ring position of the V block at hand, and of the K block behind it
+        uint32_t vslot = 1 % NS, kslot = 2 % NS;
         auto unit = [&](int u, int b, bool last) {
-          const uint32_t dv = v_lo + vslot * kSlot16 + (kUB == 2 ? b * kUnit16 : 0);
+          const uint32_t dv = v_lo + vslot * kTile16 + b * kUnit16;
+          wait(ready + 8 * b, (u >> 1) & 1);
+          if (!ok) return;
 #pragma unroll
           for (int i = 0; i < NT; i++) {
             if (i >= nt) break;
-            if (i < S::kGroups) wait(ready + 16 * i + 8 * b, (u >> 1) & 1);
-            if (!ok) break;
             const uint32_t o = o_tmem + i * DP, p = s_tmem + i * 128 + b * kUnit;
             if (!last) {
 #pragma unroll
@@ -281,9 +282,9 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
 #pragma unroll 1
               for (int kk = 0; kk < steps; kk++) sm100::mma_f16_ts_lo(o, p + kk * 8, dv + kk * 128, hi, idesc_o, u + kk > 0);
             }
-            if (i == nt - 1 && (kUB == 1 || b == 1 || last)) sm100::mma_commit(empty0 + 8 * vslot);
+            if (i == nt - 1 && (b == 1 || last)) sm100::mma_commit(empty0 + 8 * vslot);
             if (u + 2 < units)
-              scores(i, b, kslot, kUB == 1 || b == 1 || u + 2 == units - 1);
+              scores(i, b, kslot, b == 1 || u + 2 == units - 1);
             else
               sm100::mma_commit((last ? o_full : o_prev) + 8 * i);
           }
@@ -292,15 +293,14 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
         for (int u = 0; u < min(units, 2); u++)
           for (int i = 0; i < nt; i++) {
             if (u == 0) wait(q_full + 8 * i, 0);
-            if (u == 1 && kUB == 1 && i == 0) wait(full0 + 16, 0);
-            if (ok) scores(i, u, kUB == 2 ? 0 : 2 * u, kUB == 1 || u == 1 || units == 1);
+            if (ok) scores(i, u, 0, u == 1 || units == 1);
           }
 #pragma unroll 1
         for (int u = 0; u < units && ok; u += 2) {
           unit(u, 0, u + 1 >= units);
-          if (kUB == 1) next_block();
           if (u + 1 < units && ok) unit(u + 1, 1, u + 2 >= units);
-          next_block();
+          vslot = kslot + 1 == NS ? 0 : kslot + 1;
+          kslot = vslot + 1 == NS ? 0 : vslot + 1;
         }
         // all issued MMAs retire before TMEM and shared memory are given up: in
         // the regular case o_full told so; after an abort wait for a last commit
@@ -314,30 +314,25 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
       // Joins a unit's barrier once its V block and the K block of two units
       // on are there, and zeros the V rows behind the last key, up to the 16
       // that a product step takes.
-      // Every load is waited for, the first units' K too: a wait for a slot's
+      // Every load is waited for in turn, the first K too: a wait for a slot's
       // next phase is only good once the one before it has completed.
-      bool first = warp_wait(full0, 0, abort, a.err);
-      if (kUB == 1 && units > 1) first = first && warp_wait(full0 + 16, 0, abort, a.err);
+      const bool first = warp_wait(full0, 0, abort, a.err);
       for (int u = 0; u < units && first; u++) {
-        bool over = true;  // the barrier's last use, two units ago
-        for (int g = 0; g < min(S::kGroups, nt); g++)
-          over = over && (u < 2 || warp_wait(ready + 16 * g + 8 * (u & 1), ((u - 2) >> 1) & 1, abort, a.err));
-        if (!over) break;
-        if (u % kUB == 0) {
-          const uint32_t v = 2 * (u / kUB) + 1, k = 2 * ((u + 2) / kUB);  // loads: block j's K is number 2 j, its V 2 j + 1
+        if (u > 1 && !warp_wait(ready + 8 * (u & 1), ((u - 2) >> 1) & 1, abort, a.err)) break;  // its last use is over
+        if (!(u & 1)) {
+          const uint32_t v = u + 1, k = u + 2;  // loads: block j's K is number 2 j, its V 2 j + 1
           if (!warp_wait(full0 + 8 * (v % NS), (v / NS) & 1, abort, a.err)) break;
           if (u + 2 < units && !warp_wait(full0 + 8 * (k % NS), (k / NS) & 1, abort, a.err)) break;
           const int valid = keys - u * kUnit;  // of this block's
           if (valid < kBK && valid % 16) {
-            uint8_t *rows = ring + v % NS * S::kSlot + valid * 128;
+            uint8_t *rows = ring + v % NS * S::kTile + valid * 128;
             for (int x = lane; x < (16 - valid % 16) * 8 * kSub; x += 32)
-              *reinterpret_cast<uint4 *>(rows + x % kSub * S::kHalf + x / kSub * 16) = make_uint4(0, 0, 0, 0);
+              *reinterpret_cast<uint4 *>(rows + x % kSub * 16384 + x / kSub * 16) = make_uint4(0, 0, 0, 0);
             sm100::fence_proxy_async_smem();
           }
         }
         __syncwarp();
-        if (lane == 0)
-          for (int g = 0; g < min(S::kGroups, nt); g++) sm100::mbar_arrive(ready + 16 * g + 8 * (u & 1));
+        if (lane == 0) sm100::mbar_arrive(ready + 8 * (u & 1));
       }
     }
     __syncwarp();
@@ -426,7 +421,7 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
         }
         sm100::tc_fence_before();
         __syncwarp();
-        if (lane == 0) sm100::mbar_arrive(ready + (S::kGroups == 1 ? 0 : 16 * i) + 8 * b);
+        if (lane == 0) sm100::mbar_arrive(ready + 8 * b);
       }
       if (n > 0 && ok) ok = warp_wait(o_full + 8 * i, 0, abort, a.err);
       sm100::tc_fence_after();
@@ -525,16 +520,16 @@ int launch(t2sc_seqs *s, const AttnArgs &a, int splits, std::string &err) {
   auto kernel = attention_tc_kernel<DT, DP, NT>;
   TcArgs t;
   const uint64_t D = a.head_dim, H = a.heads;
-  auto encode = [&](CUtensorMap *m, const char *p, int64_t ld, int64_t rows, uint32_t box_rows) -> int {
+  auto encode = [&](CUtensorMap *m, const char *p, int64_t ld, int64_t rows) -> int {
     const uint64_t dims[3] = {D, H, (uint64_t)std::max<int64_t>(rows, 1)};
     const uint64_t strides[2] = {D * 2, rows > 1 ? (uint64_t)ld * 2 : D * H * 2};
-    const uint32_t box[3] = {64, 1, box_rows};
+    const uint32_t box[3] = {64, 1, 128};
     return tensormap_16bit(m, DT, 3, p, dims, strides, box, err);
   };
-  T2SC_TRY(encode(&t.map_q, a.q, a.ldq, s->q_rows, kBQ));
+  T2SC_TRY(encode(&t.map_q, a.q, a.ldq, s->q_rows));
   const bool keys = s->kv_off[s->batch] > s->kv_off[0];
-  T2SC_TRY(encode(&t.map_k, keys ? a.k : a.q, keys ? a.ldk : a.ldq, keys ? s->kv_rows : 1, S::kBK));  // never read without keys
-  T2SC_TRY(encode(&t.map_v, keys ? a.v : a.q, keys ? a.ldv : a.ldq, keys ? s->kv_rows : 1, S::kBK));
+  T2SC_TRY(encode(&t.map_k, keys ? a.k : a.q, keys ? a.ldk : a.ldq, keys ? s->kv_rows : 1));  // never read without keys
+  T2SC_TRY(encode(&t.map_v, keys ? a.v : a.q, keys ? a.ldv : a.ldq, keys ? s->kv_rows : 1));
   t.out = a.out, t.ldo = a.ldo;
   t.seqs = s->d_sorted;
   t.blocks = s->d_blocks + (NT == 2 ? 0 : s->batch + 1);
@@ -542,6 +537,10 @@ int launch(t2sc_seqs *s, const AttnArgs &a, int splits, std::string &err) {
   t.c = a.scale * 1.4426950408889634f, t.err = ctx->d_err;
   const int64_t grid = (NT == 2 ? s->blocks256 : s->blocks128) * a.heads * splits;
   if (grid > INT32_MAX) return fail(ctx, T2SC_ERR_UNSUPPORTED, "attention: too many query blocks in one call");
+  for (int b = 0; b <= kFew && b <= s->batch; b++) {
+    t.few_blocks[b] = (int)(NT == 2 ? s->few_blocks256[b] : s->few_blocks128[b]);
+    if (b < kFew && b < s->batch) t.few_seqs[b] = s->few_seqs[b];
+  }
   static std::atomic<uint64_t> allowed{0};
   T2SC_TRY(allow_smem(ctx, kernel, (int)S::kSmem, allowed, err));
   cudaLaunchConfig_t cfg = {};
@@ -555,16 +554,64 @@ int launch(t2sc_seqs *s, const AttnArgs &a, int splits, std::string &err) {
   return T2SC_OK;
 }
 
+// Clusters of n CTAs that the device runs at once with one CTA an SM (asked
+// for once per device; the occupancy query counts one CTA of a kernel with
+// tensor memory an SM, two run).
+struct Clusters {
+  std::atomic<int> known{0};
+  int at_once[kMaxSplits + 1] = {};
+};
+
+template <class K>
+const int *clusters_at_once(t2sc_ctx *ctx, K kernel, int threads, size_t smem, Clusters (&table)[64]) {
+  Clusters &t = table[ctx->device & 63];
+  if (!t.known.load(std::memory_order_acquire)) {
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    for (int n = 1; n <= kMaxSplits; n++) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(n * 1024), cfg.blockDim = dim3(threads), cfg.dynamicSmemBytes = smem;
+      cudaLaunchAttribute at[1];
+      at[0].id = cudaLaunchAttributeClusterDimension;
+      at[0].val.clusterDim.x = n, at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+      cfg.attrs = at, cfg.numAttrs = 1;
+      int count = 0;
+      if (cudaOccupancyMaxActiveClusters(&count, kernel, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        count = ctx->num_sms / n;
+      }
+      t.at_once[n] = count;
+    }
+    t.known.store(1, std::memory_order_release);
+  }
+  return t.at_once;
+}
+
 template <int DT, int DP>
 int launch_dp(t2sc_seqs *s, const AttnArgs &a, std::string &err) {
-  const int64_t sms = s->ctx->num_sms, pairs = s->blocks256 * a.heads, singles = s->blocks128 * a.heads;
-  // Two query blocks a CTA once they fill the SMs; below that one block a
-  // CTA (two CTAs an SM), its keys split while CTA places stay free and every
-  // part keeps at least two key blocks.
-  if (pairs >= sms) return launch<DT, DP, 2>(s, a, 1, err);
-  int splits = 1;
-  while (splits < 8 && singles * splits * 2 <= 2 * sms && s->max_kv >= (int64_t)512 * splits) splits *= 2;
-  return launch<DT, DP, 1>(s, a, splits, err);
+  // What ends first, in the time that one query block alone on an SM takes
+  // for a unit (0.67 us at head_dim 128): a CTA's rounds x (its units x what
+  // one takes + kFixed to begin and end). With two query blocks a CTA a pair
+  // of units takes kPair (0.83 us); with one, and its keys in n parts, two
+  // CTAs that share an SM take kShared for a unit of both, and kExchange goes
+  // to the parts' exchange. 300 queries over 20000 keys, 12 x 128: 75 us with
+  // the 6 parts this finds, 98 with 8 (two rounds), 99 with 4, 262 with two
+  // blocks a CTA; 20 x 300 tokens, 16 x 64: 39 us with one part, 47 with two
+  // blocks a CTA.
+  constexpr double kFixed = 8, kPair = 1.25, kShared = 1.6, kExchange = 3;
+  const double units = (double)((s->max_kv + kUnit - 1) / kUnit);
+  const int64_t pairs = s->blocks256 * a.heads, singles = s->blocks128 * a.heads;
+  double least = (double)((pairs + s->ctx->num_sms - 1) / s->ctx->num_sms) * (units * kPair + kFixed);
+  int best = 0;
+  static Clusters table[64];
+  const int *at_once = clusters_at_once(s->ctx, attention_tc_kernel<DT, DP, 1>, Shape<DP, 1>::kThreads, Shape<DP, 1>::kSmem, table);
+  for (int n = 1; n <= kMaxSplits; n++) {
+    if (at_once[n] < 1 || (n > 1 && units < 4 * n)) continue;
+    const int64_t rounds = (singles + at_once[n] - 1) / at_once[n];
+    const double part = (double)((int64_t)(units + n - 1) / n);
+    const double cost = (double)(rounds / 2) * (part * kShared + kFixed) + (double)(rounds % 2) * (part + kFixed) + (n > 1 ? kExchange : 0);
+    if (cost < least) least = cost, best = n;
+  }
+  return best == 0 ? launch<DT, DP, 2>(s, a, 1, err) : launch<DT, DP, 1>(s, a, best, err);
 }
 
 }  // namespace
