@@ -344,6 +344,23 @@ def test_attention_first_offset_above_zero(t2sc):
         ref.assert_close(out[a:b], *ref.attention(q[a:b], k[kv_off[0]:], v[kv_off[0]:], ql, kl, 0.125))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_attention_very_many_sequences(t2sc, dtype):
+    """100,000 sequences of none to four tokens: finding a block's sequence stays cheap."""
+    import torch
+    g = _gen(34)
+    lens = np.random.default_rng(6).integers(0, 5, 100000)
+    q, k, v = (_normal(g, int(lens.sum()), 1, 16, dtype=dtype) for _ in range(3))
+    y = t2sc.SequenceLayout(lens).attention_device(q, k, v)
+    # tokens of sequences of one get their own v; a sample of the others against the formula
+    off = np.concatenate([[0], np.cumsum(lens)])
+    ones = torch.from_numpy(off[:-1][lens == 1]).cuda()
+    assert torch.equal(y[ones], v[ones])
+    for b in np.nonzero(lens > 1)[0][::9973]:
+        r = slice(int(off[b]), int(off[b + 1]))
+        ref.assert_close(y[r], *ref.attention(q[r], k[r], v[r], [int(lens[b])], [int(lens[b])], 0.25))
+
+
 def test_attention_many_sequences(t2sc):
     """More sequences than SMs, most of them short, some empty."""
     g = _gen(33)

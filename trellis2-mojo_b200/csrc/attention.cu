@@ -50,18 +50,17 @@ __global__ void __launch_bounds__(kThreads) attention_simt_kernel(const AttnArgs
   float *qs = smem, *kv = qs + kBQ * pitch, *ps = kv + kBKV * pitch;  // ps: [kBQ][kBKV + 1]
   const int tid = threadIdx.x, row = tid >> 2, part = tid & 3;
   const int head = blockIdx.y;
-  // the CTA's sequence and its block of queries inside it
-  int64_t left = blockIdx.x;
-  int4 seq = make_int4(0, 0, 0, 0);
-  int b = 0;
-  for (; b < a.batch; b++) {
-    seq = __ldg(a.seqs + b);
-    const int64_t blocks = ((int64_t)seq.y + kBQ - 1) / kBQ;
-    if (left < blocks) break;
-    left -= blocks;
+  // the CTA's sequence (the last one that begins at or before this block) and its block of queries inside it
+  int lo = 0, hi = a.batch - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (__ldg(a.blocks32 + mid) <= (int64_t)blockIdx.x)
+      lo = mid;
+    else
+      hi = mid - 1;
   }
-  if (b == a.batch) return;
-  const int64_t q0 = seq.x + left * kBQ;
+  const int4 seq = __ldg(a.seqs + lo);
+  const int64_t q0 = seq.x + ((int64_t)blockIdx.x - __ldg(a.blocks32 + lo)) * kBQ;
   const int here = (int)min((int64_t)kBQ, seq.x + (int64_t)seq.y - q0);
   const int64_t at = (int64_t)head * D;
   for (int i = tid; i < kBQ * D; i += kThreads) {
@@ -137,11 +136,9 @@ __global__ void __launch_bounds__(kThreads) attention_simt_kernel(const AttnArgs
 
 int attention_simt(t2sc_seqs *s, const AttnArgs &a, int dtype, std::string &err) {
   t2sc_ctx *ctx = s->ctx;
-  int64_t blocks = 0;
-  for (int64_t b = 0; b < s->batch; b++) blocks += (s->q_off[b + 1] - s->q_off[b] + kBQ - 1) / kBQ;
-  if (blocks == 0) return T2SC_OK;
+  if (s->blocks32 > INT32_MAX) return fail(ctx, T2SC_ERR_UNSUPPORTED, "attention: too many query blocks in one call");
   const size_t smem = ((kBQ + kBKV) * (size_t)(a.head_dim + 1) + kBQ * (kBKV + 1)) * sizeof(float);
-  const dim3 grid((unsigned)blocks, (unsigned)a.heads);
+  const dim3 grid((unsigned)s->blocks32, (unsigned)a.heads);
   auto go = [&](auto kernel) -> int {
     T2SC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "attention");
     kernel<<<grid, kThreads, smem, ctx->stream>>>(a);
@@ -186,10 +183,11 @@ int t2sc_seqs_create(t2sc_ctx *ctx, const int64_t *q_offsets, const int64_t *kv_
                        (int)(s->kv_off[b + 1] - s->kv_off[b]));
     std::vector<int4> sorted(h.begin(), h.begin() + batch);
     std::stable_sort(sorted.begin(), sorted.end(), [](const int4 &x, const int4 &y) { return x.w > y.w; });
-    std::vector<int64_t> blocks(2 * (size_t)(batch + 1), 0);
+    std::vector<int64_t> blocks(3 * (size_t)(batch + 1), 0);
     for (int64_t b = 0; b < batch; b++) {
       blocks[b + 1] = blocks[b] + ((int64_t)sorted[b].y + 255) / 256;
       blocks[batch + 1 + b + 1] = blocks[batch + 1 + b] + ((int64_t)sorted[b].y + 127) / 128;
+      blocks[2 * (batch + 1) + b + 1] = blocks[2 * (batch + 1) + b] + ((int64_t)h[b].y + kBQ - 1) / kBQ;
       s->max_q = std::max<int64_t>(s->max_q, sorted[b].y);
       s->max_kv = std::max<int64_t>(s->max_kv, sorted[b].w);
     }
@@ -197,10 +195,10 @@ int t2sc_seqs_create(t2sc_ctx *ctx, const int64_t *q_offsets, const int64_t *kv_
       s->few_blocks256[b] = b <= batch ? blocks[b] : 0, s->few_blocks128[b] = b <= batch ? blocks[batch + 1 + b] : 0;
       if (b < 8) s->few_seqs[b] = b < batch ? sorted[b] : make_int4(0, 0, 0, 0);
     }
-    s->blocks256 = blocks[batch], s->blocks128 = blocks[2 * batch + 1];
+    s->blocks256 = blocks[batch], s->blocks128 = blocks[2 * batch + 1], s->blocks32 = blocks[3 * batch + 2];
     // one allocation: sequences in order, sorted, block counts
     const size_t nb = (size_t)batch + 1, bytes = 2 * nb * sizeof(int4) + blocks.size() * sizeof(int64_t);
-    T2SC_CUDA(cudaMalloc((void **)&s->d_seqs, bytes), "seqs");
+    T2SC_CUDA(cudaMallocAsync((void **)&s->d_seqs, bytes, ctx->own_stream), "seqs");
     s->d_sorted = s->d_seqs + nb;
     s->d_blocks = reinterpret_cast<int64_t *>(s->d_sorted + nb);
     sorted.resize(nb);
@@ -208,7 +206,8 @@ int t2sc_seqs_create(t2sc_ctx *ctx, const int64_t *q_offsets, const int64_t *kv_
     memcpy(image.data(), h.data(), nb * sizeof(int4));
     memcpy(image.data() + nb * sizeof(int4), sorted.data(), nb * sizeof(int4));
     memcpy(image.data() + 2 * nb * sizeof(int4), blocks.data(), blocks.size() * sizeof(int64_t));
-    T2SC_CUDA(cudaMemcpy(s->d_seqs, image.data(), bytes, cudaMemcpyHostToDevice), "seqs");
+    T2SC_CUDA(cudaMemcpyAsync(s->d_seqs, image.data(), bytes, cudaMemcpyHostToDevice, ctx->own_stream), "seqs");
+    T2SC_CUDA(cudaStreamSynchronize(ctx->own_stream), "seqs");
     *out = s.release();
     return T2SC_OK;
   });
@@ -249,7 +248,7 @@ int t2sc_attention_device(t2sc_seqs *seqs, const void *q, int64_t q_stride, cons
     a.q = static_cast<const char *>(q), a.k = static_cast<const char *>(k), a.v = static_cast<const char *>(v);
     a.out = static_cast<char *>(out);
     a.ldq = q_stride, a.ldk = k_stride, a.ldv = v_stride, a.ldo = out_stride;
-    a.seqs = seqs->d_seqs, a.batch = (int)seqs->batch, a.heads = heads, a.head_dim = head_dim, a.scale = scale;
+    a.seqs = seqs->d_seqs, a.blocks32 = seqs->d_blocks + 2 * (seqs->batch + 1), a.batch = (int)seqs->batch, a.heads = heads, a.head_dim = head_dim, a.scale = scale;
     DeviceGuard g(ctx->device);
     if (attention_rows_takes(seqs, a, dtype)) return attention_rows(seqs, a, dtype, ctx->last_error);
     return attention_tc_takes(seqs, a, dtype) ? attention_tc(seqs, a, dtype, ctx->last_error)

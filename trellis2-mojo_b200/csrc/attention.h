@@ -14,9 +14,9 @@ struct t2sc_seqs {
   int64_t q_rows = 0, kv_rows = 0;     // rows up to the last offset
   int64_t q_total = 0;                 // query rows inside sequences
   int64_t max_q = 0, max_kv = 0;       // queries, keys of the longest sequence
-  int64_t blocks128 = 0, blocks256 = 0;  // blocks of 128 / 256 query rows, sequence by sequence
+  int64_t blocks32 = 0, blocks128 = 0, blocks256 = 0;  // blocks of 32 / 128 / 256 query rows, sequence by sequence
   int4 *d_sorted = nullptr;            // as d_seqs, most keys first
-  int64_t *d_blocks = nullptr;         // [2][batch + 1] blocks of 256 / 128 rows before each sequence of d_sorted
+  int64_t *d_blocks = nullptr;         // [3][batch + 1] blocks of 256 / 128 rows before each of d_sorted, of 32 rows before each of d_seqs
   // the first sequences of d_sorted and d_blocks, for kernels to carry in their arguments
   int4 few_seqs[8];
   int64_t few_blocks256[9], few_blocks128[9];
@@ -30,6 +30,7 @@ struct AttnArgs {
   char *out = nullptr;
   int64_t ldq = 0, ldk = 0, ldv = 0, ldo = 0;  // elements between rows
   const int4 *seqs = nullptr;
+  const int64_t *blocks32 = nullptr;  // [batch + 1] blocks of 32 query rows before each sequence
   int batch = 0, heads = 0, head_dim = 0;
   float scale = 0.f;
 };

@@ -404,9 +404,12 @@ int t2sc_rope_create(t2sc_ctx *ctx, int head_dim, int pairs_x, int pairs_y, int 
       r->n_axis[i] = n[i];
       for (int j = 0; j < n[i]; j++) turns.push_back(std::pow(theta, -(double)j / n[i]) / (2.0 * 3.14159265358979323846));
     }
-    T2SC_CUDA(cudaMalloc((void **)&r->d_turns, (turns.size() + 1) * sizeof(double)), "rope frequencies");
+    // on the context's own stream: nothing else on the device waits
+    T2SC_CUDA(cudaMallocAsync((void **)&r->d_turns, (turns.size() + 1) * sizeof(double), ctx->own_stream), "rope frequencies");
     if (!turns.empty())
-      T2SC_CUDA(cudaMemcpy(r->d_turns, turns.data(), turns.size() * sizeof(double), cudaMemcpyHostToDevice), "rope frequencies");
+      T2SC_CUDA(cudaMemcpyAsync(r->d_turns, turns.data(), turns.size() * sizeof(double), cudaMemcpyHostToDevice, ctx->own_stream),
+                "rope frequencies");
+    T2SC_CUDA(cudaStreamSynchronize(ctx->own_stream), "rope frequencies");
     *out = r.release();
     return T2SC_OK;
   });
