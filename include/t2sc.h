@@ -281,18 +281,22 @@ int t2sc_c2s_block_forward_device(t2sc_c2s_block *block, t2sc_coords *coords, co
  * (with residual [rows, co]). Unlike t2sc_linear_forward_device it takes the
  * weight as it lies on the device and keeps nothing. y may be residual
  * itself (same address and stride); any other overlap with an input is
- * refused. 16-bit x and w whose rows start on 16 bytes (address and stride)
- * run on the tensor cores, f32 and other 16-bit rows on the CUDA cores. */
+ * refused. co and ci up to 2^28. 16-bit x and w whose rows start on 16 bytes
+ * (address and stride) run on the tensor cores, f32 and other 16-bit rows on
+ * the CUDA cores. */
 int t2sc_dense_linear_device(t2sc_ctx *ctx, const void *x, int64_t x_stride, const void *w, int64_t w_stride,
                              const float *bias, const void *residual, int64_t residual_stride, void *y,
                              int64_t y_stride, int64_t rows, int co, int ci, int flags, int dtype);
 
 /* Rotary positions with three axes: pair j of axis a (a = 0, 1, 2 for
  * columns x, y, z of the coordinates) turns by coords[row, 1 + a] *
- * theta^(-j / pairs_a) radians. Pairs are taken by the axes in order; the
- * head's remaining pairs do not turn. layout: pair p is channels 2p and
- * 2p + 1 (PAIRS) or p and p + head_dim / 2 (HALVES). Angles are formed in 64
- * bits: every int32 position is exact to f32. head_dim even, 2..256. */
+ * theta^(-j / pairs_a) radians, theta >= 1. Pairs are taken by the axes in
+ * order; the head's remaining pairs do not turn. layout: pair p is channels
+ * 2p and 2p + 1 (PAIRS) or p and p + head_dim / 2 (HALVES). Angles are formed
+ * in 64 bits: to f32 precision for positions up to 2^26, within 2^-20 radians
+ * for every int32 position. head_dim even, 2..256. Destroying a handle waits
+ * for the kernels that read it; a graph that captured calls with one needs it
+ * for as long as it is replayed (t2sc_seqs too). */
 #define T2SC_ROPE_PAIRS 0
 #define T2SC_ROPE_HALVES 1
 typedef struct t2sc_rope t2sc_rope;
@@ -315,9 +319,9 @@ int t2sc_qk_norm_rope_device(t2sc_ctx *ctx, t2sc_rope *rope, const int32_t *coor
 
 /* The sequences of a ragged batch: sequence b's queries are rows
  * [q_offsets[b], q_offsets[b + 1]) and its keys rows [kv_offsets[b],
- * kv_offsets[b + 1]) (host int64 [batch + 1], not falling; kv_offsets NULL:
- * the same as q_offsets, self-attention). Built once per set of coordinates
- * and shared by every layer. */
+ * kv_offsets[b + 1]) (host int64 [batch + 1], not falling, up to 2^31 - 2^16;
+ * kv_offsets NULL: the same as q_offsets, self-attention; batch up to 2^20).
+ * Built once per set of coordinates and shared by every layer. */
 typedef struct t2sc_seqs t2sc_seqs;
 int t2sc_seqs_create(t2sc_ctx *ctx, const int64_t *q_offsets, const int64_t *kv_offsets, int64_t batch,
                      t2sc_seqs **out);
@@ -327,9 +331,10 @@ int t2sc_seqs_destroy(t2sc_seqs *seqs);
  * keys gives zeros. q, out: device [rows, heads, head_dim] of dtype with
  * rows >= the last q offset; k, v likewise with the kv offsets. Rows outside
  * the sequences are neither read for a result nor written. out must not
- * overlap q, k or v. head_dim 1..256; 16-bit types with head_dim a multiple
- * of 8 up to 128 and rows that start on 16 bytes run on the tensor cores,
- * everything else on the CUDA cores. */
+ * overlap q, k or v. head_dim 1..256, scale finite (of any sign, or 0);
+ * 16-bit types with head_dim a multiple of 8 up to 128, rows that start on 16
+ * bytes and 0 < scale < 1e38 run on the tensor cores, everything else on the
+ * CUDA cores. */
 int t2sc_attention_device(t2sc_seqs *seqs, const void *q, int64_t q_stride, const void *k, int64_t k_stride,
                           const void *v, int64_t v_stride, void *out, int64_t out_stride, int heads, int head_dim,
                           float scale, int dtype);

@@ -573,3 +573,184 @@ def test_refusals(t2sc):
     assert t2sc.SequenceLayout([]).attention_device(z(0, 2, 64), z(0, 2, 64), z(0, 2, 64)).shape == (0, 2, 64)
     assert t2sc.SequenceLayout([3, 2], [0, 0]).attention_device(q, q[:0], q[:0])[:5].abs().max().item() == 0
     t2sc.Context.default(0).synchronize()
+
+
+# ---- calls at the edges of what is allowed ----
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("rows", [1, 5, 150])
+def test_linear_activations_of_huge_values(t2sc, dtype, rows):
+    """SiLU and GELU go to 0 on the left and to the value on the right, however far out."""
+    import torch
+    dt = getattr(torch, dtype)
+    x = torch.zeros(rows, 16, device="cuda", dtype=dt)
+    x[:, 0] = 1
+    w = torch.zeros(8, 16, device="cuda", dtype=dt)
+    w[:, 0] = torch.tensor([-3e38, -1e30, -1e20, -200.0, 200.0, 1e12, 1e30, 3e38], device="cuda")
+    for act in ("silu", "gelu"):
+        y = t2sc.dense_linear_device(x, w, activation=act)
+        want = torch.where(w[:, 0] > 0, w[:, 0], 0).expand(rows, 8)
+        assert torch.equal(y.abs(), want)
+
+
+def test_linear_more_outputs_than_a_grid_axis(t2sc):
+    """f32 with more column tiles than the 65535 of a grid's second axis."""
+    import torch
+    g = _gen(15)
+    co = 65537 * 64 + 3
+    x, w, b = _normal(g, 70, 4), _normal(g, co, 4), _normal(g, co)
+    y = t2sc.dense_linear_device(x, w, b)
+    for c in (slice(0, 70), slice(co // 2, co // 2 + 70), slice(co - 70, co)):
+        ref.assert_close(y[:, c], *ref.linear(x, w[c], b[c]))
+    ones = torch.ones(70, 4, device="cuda")
+    w.fill_(0.25)
+    assert torch.equal(t2sc.dense_linear_device(ones, w), torch.ones(70, co, device="cuda"))
+
+
+def test_layouts_dropped_at_once(t2sc):
+    """A layout that is dropped right after its call, its memory given to the next ones, while the kernel still waits
+    behind other work on its stream."""
+    import torch
+    g = _gen(16)
+    lens = [13 * (i % 7) for i in range(40)]
+    q, k, v = (_normal(g, sum(lens), 2, 64, dtype="bfloat16") for _ in range(3))
+    want = t2sc.SequenceLayout(lens).attention_device(q, k, v)
+    torch.cuda.synchronize()
+    got = []
+    for rep in range(8):
+        torch.cuda._sleep(20_000_000)
+        got.append(t2sc.SequenceLayout(lens).attention_device(q, k, v))
+        t2sc.SequenceLayout([1] * 40, [0] * 40)
+    assert all(torch.equal(y, want) for y in got)
+
+
+def test_attention_head_dims_in_turn_and_extreme_scales(t2sc):
+    """CUDA-core calls of large and small heads in turn; scales whose product with log2(e) overflows; scores of zero."""
+    g = _gen(17)
+    for d in (256, 8, 200, 33):
+        q, k, v = (_normal(g, 50, 2, d) for _ in range(3))
+        ref.assert_close(t2sc.SequenceLayout([50]).attention_device(q, k, v), *ref.attention(q, k, v, [50], [50], d ** -0.5))
+    import torch
+    for n in (2, 130):
+        q = torch.zeros(n, 2, 64, device="cuda", dtype=torch.bfloat16)
+        v = _normal(g, n, 2, 64, dtype="bfloat16")
+        y = t2sc.SequenceLayout([n]).attention_device(q, q, v, scale=3e38)
+        ref.assert_close(y, *ref.attention(q, q, v, [n], [n], 1.0))
+
+
+def test_the_contexts_stream_stays_as_set(t2sc):
+    """Another operator of the same context, called after one of these, runs on the stream that the program gave the
+    context: it sees rows that are written there late."""
+    import torch
+    ctx = t2sc.Context(0)
+    g = _gen(18)
+    mine = torch.cuda.Stream()
+    ctx.set_stream(mine.cuda_stream)
+    norm = t2sc.LayerNorm32(64, ctx=ctx)
+    new = _normal(g, 40, 64)
+    want = norm.forward_device(new)
+    rows, y = torch.zeros(40, 64, device="cuda"), torch.zeros(40, 64, device="cuda")
+    x, w = _normal(g, 40, 64, dtype="bfloat16"), _normal(g, 48, 64, dtype="bfloat16")
+    torch.cuda.synchronize()
+    before = ctx.launch_count()
+    with torch.cuda.stream(mine):
+        torch.cuda._sleep(100_000_000)
+        rows.copy_(new)
+    z = t2sc.dense_linear_device(x, w, ctx=ctx)
+    norm.forward_device(rows, y)
+    ref.assert_close(z, *ref.linear(x, w))
+    assert ctx.launch_count() == before + 2
+    ctx.synchronize()
+    assert torch.equal(y, want)
+    ctx.close()
+
+
+def test_handles_made_and_dropped_during_a_capture(t2sc):
+    """The first calls of a context, and handles that come and go, while a graph is captured: replays give the same bits."""
+    import gc
+    import torch
+    g = _gen(19)
+    lens = [70, 3, 200]
+    n = sum(lens)
+    q, k, v = (_normal(g, n, 2, 64, dtype="bfloat16") for _ in range(3))
+    x, w = _normal(g, n, 128, dtype="bfloat16"), _normal(g, 128, 128, std=0.1, dtype="bfloat16")
+    coords = torch.randint(0, 64, (n, 4), generator=g, device="cuda", dtype=torch.int32)
+    layout, rope = t2sc.SequenceLayout(lens), t2sc.RotaryPositionEmbedder(64)
+    want = [layout.attention_device(rope.forward_device(q, coords), k, v), t2sc.dense_linear_device(x, w)]
+    dropped = [t2sc.SequenceLayout([5, 6]), t2sc.RotaryPositionEmbedder(32)]
+    torch.cuda.synchronize()
+    graph, held = torch.cuda.CUDAGraph(), []
+    with torch.cuda.graph(graph):
+        ctx = t2sc.Context(0)
+        held += [t2sc.SequenceLayout(lens, ctx=ctx), t2sc.RotaryPositionEmbedder(64, ctx=ctx), ctx]
+        got = [held[0].attention_device(held[1].forward_device(q, coords), k, v), t2sc.dense_linear_device(x, w, ctx=ctx)]
+        dropped.clear()
+        gc.collect()
+    for y in got:
+        y.fill_(NAN)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    del graph, got
+    held[2].synchronize()
+
+
+def test_two_threads_with_contexts_of_their_own(t2sc):
+    """Two threads, a context and a stream each, calling at once."""
+    import threading
+    import torch
+    g = _gen(21)
+    cases = []
+    for i, (lens, d) in enumerate((([130, 20], 64), ([40, 7, 300], 128))):
+        q, k, v = (_normal(g, sum(lens), 3, d, dtype="float16") for _ in range(3))
+        x, w = _normal(g, 90, 256, dtype="bfloat16"), _normal(g, 200, 256, std=1 / 16, dtype="bfloat16")
+        f = _normal(g, 33, 2, 24 if i else 200)
+        cases.append((lens, q, k, v, x, w, f))
+    torch.cuda.synchronize()
+    errors = []
+
+    def work(lens, q, k, v, x, w, f):
+        try:
+            ctx, stream = t2sc.Context(0), torch.cuda.Stream()
+            layout, few = t2sc.SequenceLayout(lens, ctx=ctx), t2sc.SequenceLayout([33], ctx=ctx)
+            rope = t2sc.RotaryPositionEmbedder(q.shape[2], ctx=ctx)
+            coords = torch.arange(4 * len(q), device="cuda", dtype=torch.int32).view(-1, 4)
+            torch.cuda.synchronize()
+            with torch.cuda.stream(stream):
+                for rep in range(30):
+                    ys = [layout.attention_device(rope.forward_device(q, coords), k, v), few.attention_device(f, f, f),
+                          t2sc.dense_linear_device(x, w, activation="gelu", ctx=ctx)]
+                    stream.synchronize()
+                    first = ys if rep == 0 else first
+                    assert all(torch.equal(a, b) for a, b in zip(ys, first))
+            ref.assert_close(ys[1], *ref.attention(f, f, f, [33], [33], f.shape[2] ** -0.5))
+            ref.assert_close(ys[2], *ref.linear(x, w, None, "gelu"))
+            ctx.synchronize()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=c) for c in cases]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+
+
+def test_more_refusals(t2sc):
+    import torch
+    z = lambda *s, dt=torch.bfloat16: torch.zeros(s, device="cuda", dtype=dt)  # noqa: E731
+    w = (np.zeros((16, 16), np.float32), None)
+    attn = t2sc.SparseMultiHeadAttention(16, 2, w, to_qkv=(np.zeros((48, 16), np.float32), None))
+    layout = t2sc.SequenceLayout([4])
+    bad = [
+        lambda: t2sc.RotaryPositionEmbedder(64, theta=0.5), lambda: t2sc.RotaryPositionEmbedder(64, theta=float("inf")),
+        lambda: t2sc.SequenceLayout([2.5, 1.0]), lambda: t2sc.SequenceLayout([2 ** 31 - 1]),
+        lambda: t2sc.SequenceLayout([3], [2 ** 31 - 1000]),
+        lambda: attn.forward_device(z(4, 16), layout, context=z(4, 16)),
+    ]
+    for call in bad:
+        with pytest.raises((ValueError, t2sc.T2SCError)):
+            call()
+    assert attn.forward_device(z(4, 16), layout).shape == (4, 16)
+    t2sc.Context.default(0).synchronize()

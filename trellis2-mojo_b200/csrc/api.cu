@@ -66,6 +66,7 @@ int t2sc_ctx_create(int device, t2sc_ctx **out) {
     int ndev = 0;
     if (cudaGetDeviceCount(&ndev) != cudaSuccess || device < 0 || device >= ndev) return T2SC_ERR_CUDA;
     DeviceGuard g(device);
+    CaptureTolerant relaxed;
     cudaDeviceProp prop;
     if (cudaGetDeviceProperties(&prop, device) != cudaSuccess) return T2SC_ERR_CUDA;
     if (prop.major != 10) return T2SC_ERR_UNSUPPORTED;  // built for sm_100a only
@@ -82,7 +83,9 @@ int t2sc_ctx_create(int device, t2sc_ctx **out) {
     }
     ctx->stream = ctx->own_stream;
     if (cudaMalloc((void **)&ctx->d_err, sizeof(int)) != cudaSuccess) return T2SC_ERR_OOM;
-    if (cudaMemset(ctx->d_err, 0, sizeof(int)) != cudaSuccess) return T2SC_ERR_CUDA;
+    if (cudaMemsetAsync(ctx->d_err, 0, sizeof(int), ctx->own_stream) != cudaSuccess ||
+        cudaStreamSynchronize(ctx->own_stream) != cudaSuccess)
+      return T2SC_ERR_CUDA;
     *out = ctx.release();
     return T2SC_OK;
   });

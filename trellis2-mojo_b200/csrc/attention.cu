@@ -20,6 +20,7 @@ namespace t2sc {
 namespace {
 
 constexpr int kMaxHeadDim = 256;
+constexpr int64_t kMaxRow = INT32_MAX - 65535;  // block counts and ends of rows stay below 2^31
 
 template <int DT>
 __device__ __forceinline__ float ld1(const char *p, int64_t i) {
@@ -137,10 +138,13 @@ __global__ void __launch_bounds__(kThreads) attention_simt_kernel(const AttnArgs
 int attention_simt(t2sc_seqs *s, const AttnArgs &a, int dtype, std::string &err) {
   t2sc_ctx *ctx = s->ctx;
   if (s->blocks32 > INT32_MAX) return fail(ctx, T2SC_ERR_UNSUPPORTED, "attention: too many query blocks in one call");
-  const size_t smem = ((kBQ + kBKV) * (size_t)(a.head_dim + 1) + kBQ * (kBKV + 1)) * sizeof(float);
+  auto smem_of = [](int head_dim) { return ((kBQ + kBKV) * (size_t)(head_dim + 1) + kBQ * (kBKV + 1)) * sizeof(float); };
+  const size_t smem = smem_of(a.head_dim);
   const dim3 grid((unsigned)s->blocks32, (unsigned)a.heads);
   auto go = [&](auto kernel) -> int {
-    T2SC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "attention");
+    // for the largest head: calls of other head dims may be in other threads
+    static std::atomic<uint64_t> allowed[3] = {};
+    T2SC_TRY(allow_smem(ctx, kernel, (int)smem_of(kMaxHeadDim), allowed[dtype], err));
     kernel<<<grid, kThreads, smem, ctx->stream>>>(a);
     T2SC_LAUNCHED(ctx, "attention");
     return T2SC_OK;
@@ -159,16 +163,17 @@ extern "C" {
 int t2sc_seqs_create(t2sc_ctx *ctx, const int64_t *q_offsets, const int64_t *kv_offsets, int64_t batch, t2sc_seqs **out) {
   if (!ctx || !out) return T2SC_ERR_INVALID;
   *out = nullptr;
-  if (batch < 0 || batch > (1 << 20)) return fail(ctx, T2SC_ERR_INVALID, "seqs: batch must be in [0, 2^20]");
-  if (!q_offsets) return fail(ctx, T2SC_ERR_INVALID, "seqs: null offsets");
-  if (!kv_offsets) kv_offsets = q_offsets;
-  for (const int64_t *off : {q_offsets, kv_offsets}) {
-    if (off[0] < 0 || off[batch] > INT32_MAX) return fail(ctx, T2SC_ERR_INVALID, "seqs: offsets must be in [0, 2^31)");
-    for (int64_t b = 0; b < batch; b++)
-      if (off[b + 1] < off[b]) return fail(ctx, T2SC_ERR_INVALID, "seqs: offsets must not fall");
-  }
   return guarded(ctx, [&]() -> int {
+    if (batch < 0 || batch > (1 << 20)) return fail(ctx, T2SC_ERR_INVALID, "seqs: batch must be in [0, 2^20]");
+    if (!q_offsets) return fail(ctx, T2SC_ERR_INVALID, "seqs: null offsets");
+    if (!kv_offsets) kv_offsets = q_offsets;
+    for (const int64_t *off : {q_offsets, kv_offsets}) {
+      if (off[0] < 0 || off[batch] > kMaxRow) return fail(ctx, T2SC_ERR_INVALID, "seqs: offsets must be in [0, 2^31 - 2^16]");
+      for (int64_t b = 0; b < batch; b++)
+        if (off[b + 1] < off[b]) return fail(ctx, T2SC_ERR_INVALID, "seqs: offsets must not fall");
+    }
     DeviceGuard g(ctx->device);
+    CaptureTolerant relaxed;
     std::string &err = ctx->last_error;
     std::unique_ptr<t2sc_seqs, int (*)(t2sc_seqs *)> s(new t2sc_seqs(), t2sc_seqs_destroy);
     s->ctx = ctx;
@@ -198,7 +203,7 @@ int t2sc_seqs_create(t2sc_ctx *ctx, const int64_t *q_offsets, const int64_t *kv_
     s->blocks256 = blocks[batch], s->blocks128 = blocks[2 * batch + 1], s->blocks32 = blocks[3 * batch + 2];
     // one allocation: sequences in order, sorted, block counts
     const size_t nb = (size_t)batch + 1, bytes = 2 * nb * sizeof(int4) + blocks.size() * sizeof(int64_t);
-    T2SC_CUDA(cudaMallocAsync((void **)&s->d_seqs, bytes, ctx->own_stream), "seqs");
+    T2SC_CUDA(cudaMalloc((void **)&s->d_seqs, bytes), "seqs");
     s->d_sorted = s->d_seqs + nb;
     s->d_blocks = reinterpret_cast<int64_t *>(s->d_sorted + nb);
     sorted.resize(nb);
@@ -216,7 +221,8 @@ int t2sc_seqs_create(t2sc_ctx *ctx, const int64_t *q_offsets, const int64_t *kv_
 int t2sc_seqs_destroy(t2sc_seqs *s) {
   if (!s) return T2SC_OK;
   DeviceGuard g(s->ctx->device);
-  if (s->d_seqs) cudaFree(s->d_seqs);
+  CaptureTolerant relaxed;
+  if (s->d_seqs) cudaFree(s->d_seqs);  // waits for the kernels that read it, on whatever stream
   delete s;
   return T2SC_OK;
 }

@@ -35,7 +35,7 @@ struct AttnArgs {
   float scale = 0.f;
 };
 
-// 16-bit rows that start on 16 bytes, head_dim a multiple of 8 up to 128, scale > 0.
+// 16-bit rows that start on 16 bytes, head_dim a multiple of 8 up to 128, scale in (0, 1e38).
 bool attention_tc_takes(const t2sc_seqs *s, const AttnArgs &a, int dtype);
 int attention_tc(t2sc_seqs *s, const AttnArgs &a, int dtype, std::string &err);
 // As attention_tc, for at most 4 queries a sequence.

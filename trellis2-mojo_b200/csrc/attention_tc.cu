@@ -619,8 +619,8 @@ int launch_dp(t2sc_seqs *s, const AttnArgs &a, std::string &err) {
 bool attention_tc_takes(const t2sc_seqs *s, const AttnArgs &a, int dtype) {
   auto on16 = [](const void *p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0; };
   const bool keys = s->kv_off[s->batch] > s->kv_off[0];
-  // scores are compared before they are scaled: the scale has to keep their order
-  return dtype != T2SC_DT_F32 && a.head_dim % 8 == 0 && a.head_dim <= 128 && a.scale > 0.f && on16(a.q, a.ldq) &&
+  // scores are compared before they are scaled: the scale has to keep their order; scale * log2(e) has to be finite
+  return dtype != T2SC_DT_F32 && a.head_dim % 8 == 0 && a.head_dim <= 128 && a.scale > 0.f && a.scale < 1e38f && on16(a.q, a.ldq) &&
          on16(a.out, a.ldo) && (!keys || (on16(a.k, a.ldk) && on16(a.v, a.ldv)));
 }
 

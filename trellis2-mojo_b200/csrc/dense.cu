@@ -39,8 +39,9 @@ template <int DT>
 __global__ void __launch_bounds__(256) dense_simt_kernel(const DenseArgs a) {
   __shared__ float xs[kBK][kBM + 4], ws[kBK][kBN + 4];
   const int tid = threadIdx.x, tr = tid / 16 * 4, tc = tid % 16 * 4;
-  const int64_t row0 = (int64_t)blockIdx.x * kBM;
-  const int col0 = (int)blockIdx.y * kBN;
+  const unsigned row_tiles = (unsigned)((a.rows + kBM - 1) / kBM);  // fastest
+  const int64_t row0 = (int64_t)(blockIdx.x % row_tiles) * kBM;
+  const int col0 = (int)(blockIdx.x / row_tiles) * kBN;
   float acc[4][4] = {};
   for (int k0 = 0; k0 < a.ci; k0 += kBK) {
     for (int i = tid; i < kBM * kBK; i += 256) {
@@ -78,9 +79,9 @@ __global__ void __launch_bounds__(256) dense_simt_kernel(const DenseArgs a) {
 }  // namespace
 
 int dense_simt(t2sc_ctx *ctx, const DenseArgs &a, int dtype, std::string &err) {
-  const int64_t gx = (a.rows + kBM - 1) / kBM, gy = (a.co + kBN - 1) / kBN;
-  if (gy > 65535) return fail(ctx, T2SC_ERR_UNSUPPORTED, "dense_linear: more than 4194240 outputs");
-  const dim3 grid((unsigned)gx, (unsigned)gy);
+  const int64_t tiles = ((a.rows + kBM - 1) / kBM) * ((a.co + kBN - 1) / kBN);
+  if (tiles > INT32_MAX) return fail(ctx, T2SC_ERR_UNSUPPORTED, "dense_linear: too many outputs in one call");
+  const unsigned grid = (unsigned)tiles;
   if (dtype == T2SC_DT_F32)
     dense_simt_kernel<T2SC_DT_F32><<<grid, 256, 0, ctx->stream>>>(a);
   else if (dtype == T2SC_DT_BF16)
@@ -101,7 +102,8 @@ extern "C" int t2sc_dense_linear_device(t2sc_ctx *ctx, const void *x, int64_t x_
   if (!ctx) return T2SC_ERR_INVALID;
   return guarded(ctx, [&]() -> int {
     if (rows < 0 || rows > INT32_MAX) return fail(ctx, T2SC_ERR_INVALID, "dense_linear: rows must be in [0, 2^31)");
-    if (co < 1 || ci < 1) return fail(ctx, T2SC_ERR_INVALID, "dense_linear: need co >= 1 and ci >= 1");
+    if (co < 1 || ci < 1 || co > kMaxStride || ci > kMaxStride)
+      return fail(ctx, T2SC_ERR_INVALID, "dense_linear: co and ci must be in [1, 2^28]");
     if (!dtype_known(dtype)) return fail(ctx, T2SC_ERR_INVALID, "dense_linear: unknown dtype");
     if (flags & ~(T2SC_SILU | T2SC_GELU | T2SC_RESIDUAL)) return fail(ctx, T2SC_ERR_INVALID, "dense_linear: unknown flags");
     if ((flags & T2SC_SILU) && (flags & T2SC_GELU)) return fail(ctx, T2SC_ERR_INVALID, "dense_linear: SILU and GELU exclude each other");

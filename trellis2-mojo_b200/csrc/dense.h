@@ -20,16 +20,18 @@ struct DenseArgs {
   int co = 0, ci = 0, act = 0;
 };
 
-// 0.5 v (1 + tanh(u)) = v / (1 + e^(-2u)), u = sqrt(2/pi) (v + 0.044715 v^3):
-// one exponential, and no cancellation in the negative tail. The exponent is
-// clamped as in silu().
+// v / (1 + e^-v) and 0.5 v (1 + tanh(u)) = v / (1 + e^(-2u)), u = sqrt(2/pi)
+// (v + 0.044715 v^3): one exponential, and no cancellation in the negative
+// tail. The exponential may become infinite: any finite v over it is 0, the
+// limit of both, however large v is.
+__device__ __forceinline__ float silu_any(float v) { return __fdividef(v, 1.0f + __expf(-v)); }
 __device__ __forceinline__ float gelu_tanh(float v) {
   const float u2 = v * (1.5957691216057308f + 0.07135481627f * v * v);
-  return __fdividef(v, 1.0f + __expf(fminf(-u2, 80.0f)));
+  return __fdividef(v, 1.0f + __expf(-u2));
 }
 
 __device__ __forceinline__ float activate(float v, int act) {
-  if (act & T2SC_SILU) return silu(v);
+  if (act & T2SC_SILU) return silu_any(v);
   if (act & T2SC_GELU) return gelu_tanh(v);
   return v;
 }

@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
         }
         if (a.act & T2SC_SILU) {
 #pragma unroll
-          for (int j = 0; j < 64; j++) v[j] = silu(v[j]);
+          for (int j = 0; j < 64; j++) v[j] = silu_any(v[j]);
         } else if (a.act & T2SC_GELU) {
 #pragma unroll
           for (int j = 0; j < 64; j++) v[j] = gelu_tanh(v[j]);

@@ -23,6 +23,15 @@ struct DeviceGuard {
   }
 };
 
+// Allows this thread's allocations and frees while some stream is being
+// captured into a graph (a handle that is made, or dropped by a garbage
+// collector, meanwhile). The captured stream is not touched.
+struct CaptureTolerant {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  CaptureTolerant() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  ~CaptureTolerant() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
 inline int fail(t2sc_ctx *ctx, int code, const std::string &msg) {
   if (ctx) ctx->last_error = msg;
   return code;
@@ -37,12 +46,17 @@ inline int fail(t2sc_ctx *ctx, int code, const std::string &msg) {
 // Runs an entry point's body; C++ exceptions never cross the C ABI.
 template <class F>
 int guarded(t2sc_ctx *ctx, F &&body) {
+  bool oom = false;
   try {
     return body();
   } catch (const std::bad_alloc &) {
-    return fail(ctx, T2SC_ERR_OOM, "host allocation failed");
+    oom = true;
   } catch (...) {
-    return fail(ctx, T2SC_ERR_INVALID, "unexpected exception");
+  }
+  try {
+    return oom ? fail(ctx, T2SC_ERR_OOM, "host allocation failed") : fail(ctx, T2SC_ERR_INVALID, "unexpected exception");
+  } catch (...) {  // no memory for the message either
+    return oom ? T2SC_ERR_OOM : T2SC_ERR_INVALID;
   }
 }
 

@@ -5,7 +5,10 @@
 // Pair j of axis a turns by coords[row, 1 + a] * theta^(-j / n_a). The angle
 // is formed in turns (2 pi = 1) and in 64 bits and reduced to half a turn
 // before it is rounded: a 32-bit angle of a position of 10^3 would already be
-// off by 3e-5, and any int32 position is allowed here.
+// off by 3e-5, and any int32 position is allowed here. With theta >= 1 a
+// position turns by at most 2^31 / (2 pi) turns, whose product and frequency
+// are each off by 2^-53 relative: 2^-23 turns at the farthest positions, and
+// less than the rounding to f32 below 2^26.
 //
 // The operators move their rows once in and once out and do ~10 operations a
 // value, so HBM bounds them if enough bytes are in flight and the
@@ -383,16 +386,17 @@ int t2sc_rope_create(t2sc_ctx *ctx, int head_dim, int pairs_x, int pairs_y, int 
                      t2sc_rope **out) {
   if (!ctx || !out) return T2SC_ERR_INVALID;
   *out = nullptr;
-  if (head_dim < 2 || head_dim % 2 || head_dim > kMaxHeadDim)
-    return fail(ctx, T2SC_ERR_INVALID, "rope: head_dim must be even and in [2, 256]");
-  const int n[3] = {pairs_x, pairs_y, pairs_z};
-  for (int i = 0; i < 3; i++)
-    if (n[i] < 0 || n[i] > head_dim / 2) return fail(ctx, T2SC_ERR_INVALID, "rope: pairs of an axis must be in [0, head_dim / 2]");
-  if (n[0] + n[1] + n[2] > head_dim / 2) return fail(ctx, T2SC_ERR_INVALID, "rope: the axes take more pairs than a head has");
-  if (!(theta > 0.0) || !std::isfinite(theta)) return fail(ctx, T2SC_ERR_INVALID, "rope: theta must be positive and finite");
-  if (layout != T2SC_ROPE_PAIRS && layout != T2SC_ROPE_HALVES) return fail(ctx, T2SC_ERR_INVALID, "rope: unknown layout");
   return guarded(ctx, [&]() -> int {
+    if (head_dim < 2 || head_dim % 2 || head_dim > kMaxHeadDim)
+      return fail(ctx, T2SC_ERR_INVALID, "rope: head_dim must be even and in [2, 256]");
+    const int n[3] = {pairs_x, pairs_y, pairs_z};
+    for (int i = 0; i < 3; i++)
+      if (n[i] < 0 || n[i] > head_dim / 2) return fail(ctx, T2SC_ERR_INVALID, "rope: pairs of an axis must be in [0, head_dim / 2]");
+    if (n[0] + n[1] + n[2] > head_dim / 2) return fail(ctx, T2SC_ERR_INVALID, "rope: the axes take more pairs than a head has");
+    if (!(theta >= 1.0) || !std::isfinite(theta)) return fail(ctx, T2SC_ERR_INVALID, "rope: theta must be at least 1 and finite");
+    if (layout != T2SC_ROPE_PAIRS && layout != T2SC_ROPE_HALVES) return fail(ctx, T2SC_ERR_INVALID, "rope: unknown layout");
     DeviceGuard g(ctx->device);
+    CaptureTolerant relaxed;
     std::string &err = ctx->last_error;
     std::unique_ptr<t2sc_rope, int (*)(t2sc_rope *)> r(new t2sc_rope(), t2sc_rope_destroy);
     r->ctx = ctx;
@@ -405,7 +409,7 @@ int t2sc_rope_create(t2sc_ctx *ctx, int head_dim, int pairs_x, int pairs_y, int 
       for (int j = 0; j < n[i]; j++) turns.push_back(std::pow(theta, -(double)j / n[i]) / (2.0 * 3.14159265358979323846));
     }
     // on the context's own stream: nothing else on the device waits
-    T2SC_CUDA(cudaMallocAsync((void **)&r->d_turns, (turns.size() + 1) * sizeof(double), ctx->own_stream), "rope frequencies");
+    T2SC_CUDA(cudaMalloc((void **)&r->d_turns, (turns.size() + 1) * sizeof(double)), "rope frequencies");
     if (!turns.empty())
       T2SC_CUDA(cudaMemcpyAsync(r->d_turns, turns.data(), turns.size() * sizeof(double), cudaMemcpyHostToDevice, ctx->own_stream),
                 "rope frequencies");
@@ -418,7 +422,8 @@ int t2sc_rope_create(t2sc_ctx *ctx, int head_dim, int pairs_x, int pairs_y, int 
 int t2sc_rope_destroy(t2sc_rope *r) {
   if (!r) return T2SC_OK;
   DeviceGuard g(r->ctx->device);
-  if (r->d_turns) cudaFree(r->d_turns);
+  CaptureTolerant relaxed;
+  if (r->d_turns) cudaFree(r->d_turns);  // waits for the kernels that read it, on whatever stream
   delete r;
   return T2SC_OK;
 }

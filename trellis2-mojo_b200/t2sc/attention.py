@@ -1,7 +1,10 @@
 """The attention block over voxel tokens, on the device.
 
 Operators over CUDA tensors of rows, each one C-ABI call on torch's current
-stream:
+stream (the stream of the Context that they are given stays as it was set).
+They are for inference: results carry no gradient. As all calls of a Context,
+those of one Context (and of the handles made with it) come from one thread at
+a time.
   dense_linear_device      act(x @ w^T + bias) + residual   (linear, trellis2_mojo/modules/nn.mojo:27-266)
   RotaryPositionEmbedder   rotary positions over x, y, z    (trellis2_mojo/modules/rope.mojo)
   qk_norm_rope_device      per-head RMS norm + rotation     (bias_rms_rope_qkv, trellis2_mojo/gpu/attention.mojo:507)
@@ -94,11 +97,13 @@ def _context(ctx, t):
 
 
 def _on_torch_stream(ctx):
-    """The context's work goes to torch's current stream of its device."""
+    """The library context to call with, its work on torch's current stream of the device."""
     stream = torch.cuda.current_stream(ctx.device).cuda_stream if _raw_stream is None else _raw_stream(ctx.device)
     stream = stream or 1    # handle 0 would name the context's own stream, 1 is cudaStreamLegacy
-    if ctx.stream_ptr != stream:
-        ctx.set_stream(stream)
+    beside = ctx._beside_torch or ctx.beside_torch()
+    if beside.stream != stream:
+        beside.use(stream)
+    return beside.handle
 
 
 # the handle alone, without a Stream object around it (2 us less a call)
@@ -133,11 +138,11 @@ def dense_linear_device(x, weight, bias=None, activation=None, residual=None, ou
             raise ValueError("dense_linear: out must be [rows, co]")
     b = None if bias is None else _f32(bias, device, (co,), "dense_linear: bias")
     if rows:
-        _on_torch_stream(ctx)
-        rc = _linear(ctx.handle, x.data_ptr(), ldx, weight.data_ptr(), ldw, b, res, ldr, out.data_ptr(), ldy, rows, co, ci,
+        handle = _on_torch_stream(ctx)
+        rc = _linear(handle, x.data_ptr(), ldx, weight.data_ptr(), ldw, b, res, ldr, out.data_ptr(), ldy, rows, co, ci,
                      flags, code)
         if rc:
-            check(rc, ctx.handle)
+            check(rc, handle)
     return out
 
 
@@ -145,8 +150,10 @@ class RotaryPositionEmbedder:
     """Rotary positions over the voxel axes x, y, z (columns 1..3 of the
     coordinates). Each axis takes pairs[a] of a head's head_dim / 2 pairs
     (default: a third each, rounded down), pair j of an axis turning by
-    position * theta^(-j / pairs[a]); the rest do not turn. layout: "pairs"
-    (channels 2p, 2p + 1) or "halves" (channels p, p + head_dim / 2)."""
+    position * theta^(-j / pairs[a]), theta >= 1; the rest do not turn.
+    layout: "pairs" (channels 2p, 2p + 1) or "halves" (channels p, p +
+    head_dim / 2). A graph that captured a call with it needs it for as long as
+    it is replayed."""
 
     def __init__(self, head_dim, pairs=None, theta=10000.0, layout="pairs", ctx=None):
         if layout not in _LAYOUTS:
@@ -156,9 +163,9 @@ class RotaryPositionEmbedder:
         if len(self.pairs) != 3:
             raise ValueError("RotaryPositionEmbedder: pairs are three counts, of x, y and z")
         self.ctx = ctx or Context.default()
-        h = ctypes.c_void_p()
-        check(lib.t2sc_rope_create(self.ctx.handle, self.head_dim, *self.pairs, self.theta, _LAYOUTS[layout],
-                                   ctypes.byref(h)), self.ctx.handle)
+        h, beside = ctypes.c_void_p(), self.ctx.beside_torch().handle
+        check(lib.t2sc_rope_create(beside, self.head_dim, *self.pairs, self.theta, _LAYOUTS[layout], ctypes.byref(h)),
+              beside)
         self.handle = h
 
     def forward_device(self, x, coords, out=None):
@@ -177,10 +184,10 @@ class RotaryPositionEmbedder:
             if (r, h, e) != (rows, heads, d):
                 raise ValueError("RotaryPositionEmbedder: out must have x's shape")
         if rows:
-            _on_torch_stream(ctx)
+            handle = _on_torch_stream(ctx)
             rc = _rope_apply(self.handle, at, x.data_ptr(), ldx, out.data_ptr(), ldy, rows, heads, code)
             if rc:
-                check(rc, ctx.handle)
+                check(rc, handle)
         return out
 
     def __del__(self):
@@ -227,11 +234,11 @@ def qk_norm_rope_device(q, k, gain_q, gain_k, coords=None, rope=None, eps=1e-6, 
         raise ValueError("qk_norm_rope: out_k without k")
     at = _coords(coords, device, rows) if rope is not None else None
     if rows:
-        _on_torch_stream(ctx)
-        rc = _qk_norm_rope(ctx.handle, None if rope is None else rope.handle, at, q.data_ptr(), ldq, kp, ldk, gq, gk,
+        handle = _on_torch_stream(ctx)
+        rc = _qk_norm_rope(handle, None if rope is None else rope.handle, at, q.data_ptr(), ldq, kp, ldk, gq, gk,
                            out_q.data_ptr(), ldqo, kop, ldko, rows, heads, d, eps, code)
         if rc:
-            check(rc, ctx.handle)
+            check(rc, handle)
     return out_q, out_k
 
 
@@ -239,7 +246,8 @@ class SequenceLayout:
     """The sequences of a ragged batch: lengths of each one's queries and of
     its keys (None: the same, self-attention). Built once for a set of
     coordinates (`of` a SparseTensor: one sequence per batch entry) and
-    shared by every layer and step."""
+    shared by every layer and step. A graph that captured its attention needs
+    it for as long as it is replayed."""
 
     def __init__(self, q_lens, kv_lens=None, ctx=None):
         self.q_offsets = self._offsets(q_lens)
@@ -248,9 +256,9 @@ class SequenceLayout:
             raise ValueError("SequenceLayout: as many key lengths as query lengths")
         self.q_rows, self.kv_rows = int(self.q_offsets[-1]), int(self.kv_offsets[-1])
         self.ctx = ctx or Context.default()
-        h = ctypes.c_void_p()
-        check(lib.t2sc_seqs_create(self.ctx.handle, self.q_offsets.ctypes.data, self.kv_offsets.ctypes.data,
-                                   len(self.q_offsets) - 1, ctypes.byref(h)), self.ctx.handle)
+        h, beside = ctypes.c_void_p(), self.ctx.beside_torch().handle
+        check(lib.t2sc_seqs_create(beside, self.q_offsets.ctypes.data, self.kv_offsets.ctypes.data,
+                                   len(self.q_offsets) - 1, ctypes.byref(h)), beside)
         self.handle = h
 
     @classmethod
@@ -260,7 +268,10 @@ class SequenceLayout:
 
     @staticmethod
     def _offsets(lens):
-        lens = np.asarray(lens, dtype=np.int64).reshape(-1)
+        given = np.asarray(lens).reshape(-1)
+        if given.size and given.dtype.kind not in "iu":
+            raise ValueError("SequenceLayout: lengths must be whole numbers")
+        lens = given.astype(np.int64)
         if len(lens) and lens.min() < 0:
             raise ValueError("SequenceLayout: lengths must not be negative")
         return np.concatenate([[0], np.cumsum(lens)]).astype(np.int64)
@@ -286,11 +297,11 @@ class SequenceLayout:
             r, h, e, ldo = _heads3d(out, device, dtype, "attention: out")
             if (r, h, e) != (rows, heads, d):
                 raise ValueError("attention: out must have q's shape")
-        _on_torch_stream(ctx)
+        handle = _on_torch_stream(ctx)
         rc = _attention(self.handle, q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, out.data_ptr(), ldo, heads, d,
                         d ** -0.5 if scale is None else scale, code)
         if rc:
-            check(rc, ctx.handle)
+            check(rc, handle)
         return out
 
     def __del__(self):
@@ -334,7 +345,7 @@ class SparseMultiHeadAttention:
         self.channels, self.heads, self.head_dim = channels, heads, channels // heads
         self.cross, self.rope, self.eps, self.dtype = to_qkv is None, rope, float(eps), dtype
         dev, dt = f"cuda:{self.ctx.device}", _torch_dtype(dtype)
-    
+
         def pair(wb, co, ci=None):
             w, b = _tensor(wb[0], dt, dev), _tensor(wb[1], torch.float32, dev)
             if w.dim() != 2 or w.shape[0] != co or (ci is not None and w.shape[1] != ci) or \
@@ -370,6 +381,8 @@ class SparseMultiHeadAttention:
                 qk_norm_rope_device(q, None, self._gains[0], None, eps=self.eps, out_q=q, ctx=self.ctx)
                 qk_norm_rope_device(k, None, self._gains[1], None, eps=self.eps, out_q=k, ctx=self.ctx)
         else:
+            if context is not None:
+                raise ValueError("SparseMultiHeadAttention: a context, but no to_q and to_kv")
             qkv = dense_linear_device(x, *self._qkv, ctx=self.ctx).view(rows, 3, h, d)
             q, k, v = qkv[:, 0], qkv[:, 1], qkv[:, 2]
             if self._gains:

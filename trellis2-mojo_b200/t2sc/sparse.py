@@ -40,7 +40,7 @@ class Context:
         check(rc)
         self.handle = h
         self.device = device
-        self.stream_ptr = None    # as last set; None: the context's own stream
+        self._beside_torch = None
 
     @classmethod
     def default(cls, device=0):
@@ -52,18 +52,51 @@ class Context:
         """Compute check + a bounded device wait that must time out cleanly."""
         check(lib.t2sc_ctx_selftest(self.handle, wait_us), self.handle)
 
+    def beside_torch(self):
+        """The library context of the operators that follow torch's current
+        stream, so that they leave the stream of this one as it was set."""
+        if self._beside_torch is None:
+            self._beside_torch = TorchContext(self.device)
+        return self._beside_torch
+
+    def _both(self):
+        return (self,) if self._beside_torch is None else (self, self._beside_torch)
+
     def synchronize(self):
-        check(lib.t2sc_ctx_synchronize(self.handle), self.handle)
+        for c in self._both():
+            check(lib.t2sc_ctx_synchronize(c.handle), c.handle)
 
     def launch_count(self):
-        v = ctypes.c_int64()
-        check(lib.t2sc_ctx_launch_count(self.handle, ctypes.byref(v)), self.handle)
-        return v.value
+        v, n = ctypes.c_int64(), 0
+        for c in self._both():
+            check(lib.t2sc_ctx_launch_count(c.handle, ctypes.byref(v)), c.handle)
+            n += v.value
+        return n
 
     def set_stream(self, stream_ptr):
         check(lib.t2sc_ctx_set_stream(self.handle, ctypes.c_void_p(stream_ptr) if stream_ptr else None),
               self.handle)
-        self.stream_ptr = stream_ptr or None
+
+    def close(self):
+        if self._beside_torch is not None:
+            self._beside_torch.close()
+        if self.handle:
+            lib.t2sc_ctx_destroy(self.handle)
+            self.handle = None
+
+
+class TorchContext:
+    """A library context whose stream is set before each call (Context.beside_torch)."""
+
+    def __init__(self, device):
+        h = ctypes.c_void_p()
+        check(lib.t2sc_ctx_create(device, ctypes.byref(h)))
+        self.handle = h
+        self.stream = None    # as last set; None: the context's own
+
+    def use(self, stream):
+        check(lib.t2sc_ctx_set_stream(self.handle, ctypes.c_void_p(stream)), self.handle)
+        self.stream = stream
 
     def close(self):
         if self.handle:
