@@ -754,3 +754,86 @@ def test_more_refusals(t2sc):
             call()
     assert attn.forward_device(z(4, 16), layout).shape == (4, 16)
     t2sc.Context.default(0).synchronize()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("rows,ci,co", [(200, 8192, 128), (300, 4100, 130), (129, 6152, 260), (513, 8192, 4), (700, 9000, 33)])
+def test_linear_few_tiles_over_a_long_axis(t2sc, dtype, rows, ci, co):
+    """Several tiles of rows with the K axis split, ragged in every direction, in place and with an unaligned result."""
+    import torch
+    g = _gen(rows + ci)
+    x, w, b = _normal(g, rows, ci, dtype=dtype), _normal(g, co, ci, std=ci ** -0.5, dtype=dtype), _normal(g, co)
+    for pad in (8, 5):
+        rv, buf = _inside(rows, co, dtype, pad_cols=pad)
+        rv.copy_(_normal(g, rows, co, dtype=dtype))
+        want = ref.linear(x, w, b, "gelu", rv.clone())
+        first = t2sc.dense_linear_device(x, w, b, activation="gelu", residual=rv)
+        t2sc.dense_linear_device(x, w, b, activation="gelu", residual=rv, out=rv)
+        assert torch.equal(first, rv) and _untouched(buf, rows, co)
+        ref.assert_close(rv, *want)
+
+
+def test_calls_in_a_row_see_each_others_results(t2sc):
+    """Kernels begin while the one before them ends: chains of small calls that read what the last one wrote and
+    overwrite what it read, each kind behind each other, in a graph and eagerly."""
+    import torch
+    g = _gen(23)
+    h, d = 2, 64
+    c = h * d
+    w = [_normal(g, c, c, std=c ** -0.5, dtype="bfloat16") for _ in range(4)]
+    gain = torch.ones(h, d, device="cuda")
+    coords = torch.randint(0, 64, (512, 4), generator=g, device="cuda", dtype=torch.int32)
+    rope = t2sc.RotaryPositionEmbedder(d)
+    layouts = {m: (t2sc.SequenceLayout([m]), t2sc.SequenceLayout([1, 1], [m - m // 4, m // 4]),
+                   t2sc.SequenceLayout([0, 0], [m, 0])) for m in (1, 4, 24, 300)}
+
+    def chain(bufs, m):
+        a, b = (t[:m] for t in bufs)
+        one, few, none = layouts[m]
+        heads = lambda t: t.view(m, h, d)  # noqa: E731
+        for i in range(6):
+            t2sc.dense_linear_device(a, w[i % 4], activation="silu", out=b)
+            t2sc.qk_norm_rope_device(heads(b), None, gain, None, coords=coords[:m], rope=rope, out_q=heads(b))
+            one.attention_device(heads(b), heads(b), heads(b), out=heads(a))
+            none.attention_device(heads(b), heads(b), heads(b), out=heads(a))
+            t2sc.dense_linear_device(a, w[(i + 1) % 4], residual=b, out=b)
+            rope.forward_device(heads(b), coords[:m], out=heads(b))
+            if m > 3:
+                few.attention_device(heads(b), heads(b), heads(b), out=heads(a))
+            t2sc.dense_linear_device(b, w[(i + 2) % 4], residual=a, out=a)
+        return a
+
+    for m in (1, 4, 24, 300):
+        start = _normal(g, 300, c, dtype="bfloat16")
+        slow = [start.clone(), torch.zeros_like(start)]
+        # the same chain with the device idle between any two calls
+        sync = torch.cuda.synchronize
+        patched = [(t2sc, "dense_linear_device"), (t2sc, "qk_norm_rope_device"), (type(rope), "forward_device"),
+                   (t2sc.SequenceLayout, "attention_device")]
+        kept = [getattr(o, name) for o, name in patched]
+
+        def waiting(f):
+            def call(*args, **kw):
+                y = f(*args, **kw)
+                sync()
+                return y
+            return call
+
+        for (o, name), f in zip(patched, kept):
+            setattr(o, name, waiting(f))
+        try:
+            want = chain(slow, m).clone()
+        finally:
+            for (o, name), f in zip(patched, kept):
+                setattr(o, name, f)
+        for _ in range(5):
+            bufs = [start.clone(), torch.zeros_like(start)]
+            assert torch.equal(chain(bufs, m), want)
+        bufs = [start.clone(), torch.zeros_like(start)]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = chain(bufs, m)
+        for _ in range(5):
+            bufs[0].copy_(start)
+            graph.replay()
+            assert torch.equal(y, want)

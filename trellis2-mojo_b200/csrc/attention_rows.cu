@@ -88,7 +88,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_rows_kernel(const __gri
   const int head = id % a.heads;
   const int4 seq = __ldg(a.seqs + id / a.heads);
   const int rows = seq.y, keys = seq.w;
-  if (rows == 0) return;  // the whole cluster
+  sm100::next_kernel_may_start();
+  if (rows == 0) {  // the whole cluster
+    sm100::previous_kernel_done();
+    return;
+  }
   const int all = (keys + kBlock - 1) / kBlock, per = (all + x.splits - 1) / x.splits;
   const int b0 = min(split * per, all), n = min(b0 + per, all) - b0;  // this CTA's blocks
   const uint32_t full0 = sm100::smem_u32(bars), empty0 = full0 + 8 * kStages, ring0 = sm100::smem_u32(ring);
@@ -101,6 +105,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_rows_kernel(const __gri
     sm100::fence_mbar_init();
   }
   __syncthreads();
+  sm100::previous_kernel_done();
   float q[R][8], o[R][8], m[R], l[R];
   if (warp == kWarps) {
     // -------------------------------- TMA --------------------------------
@@ -266,45 +271,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_rows_kernel(const __gri
   sm100::cluster_sync();  // no CTA leaves before the others have read its sums
 }
 
-// Clusters of each size that the device runs at once (asked for once per device).
-struct Clusters {
-  std::atomic<int> known{0};
-  int at_once[kMaxSplits + 1] = {};
-};
-
-template <class K>
-int clusters_at_once(t2sc_ctx *ctx, K kernel, Clusters (&table)[64], const int **out, std::string &err) {
-  Clusters &t = table[ctx->device & 63];
-  if (!t.known.load(std::memory_order_acquire)) {
-    T2SC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem), "attention");
-    T2SC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "attention");
-    for (int n = 1; n <= kMaxSplits; n++) {
-      cudaLaunchConfig_t cfg = {};
-      cfg.gridDim = dim3(n * 1024), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = kSmem;
-      cudaLaunchAttribute at[1];
-      at[0].id = cudaLaunchAttributeClusterDimension;
-      at[0].val.clusterDim.x = n, at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-      cfg.attrs = at, cfg.numAttrs = 1;
-      int count = 0;
-      if (cudaOccupancyMaxActiveClusters(&count, kernel, &cfg) != cudaSuccess) {
-        cudaGetLastError();
-        count = 0;
-      }
-      t.at_once[n] = count;
-    }
-    t.known.store(1, std::memory_order_release);
-  }
-  *out = t.at_once;
-  return T2SC_OK;
-}
-
 template <int DT, int G, int R>
 int launch(t2sc_seqs *s, const AttnArgs &a, std::string &err) {
   t2sc_ctx *ctx = s->ctx;
   auto kernel = attention_rows_kernel<DT, G, R>;
-  static Clusters table[64];
+  static Clusters<kMaxSplits> table[64];
   const int *at_once = nullptr;
-  T2SC_TRY(clusters_at_once(ctx, kernel, table, &at_once, err));
+  T2SC_TRY(clusters_at_once(ctx, kernel, kThreads, kSmem, table, &at_once, err));
   RowsArgs x;
   x.a = a;
   x.c = a.scale * 1.4426950408889634f;
@@ -329,13 +302,7 @@ int launch(t2sc_seqs *s, const AttnArgs &a, std::string &err) {
   };
   T2SC_TRY(encode(&x.map_k, a.k, a.ldk));
   T2SC_TRY(encode(&x.map_v, a.v, a.ldv));
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(ctas * x.splits)), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = kSmem, cfg.stream = ctx->stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = x.splits, at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at, cfg.numAttrs = 1;
-  T2SC_CUDA(cudaLaunchKernelEx(&cfg, kernel, x), "attention");
+  T2SC_CUDA(launch_overlapped(kernel, ctas * x.splits, kThreads, kSmem, ctx->stream, x.splits, x), "attention");
   T2SC_LAUNCHED(ctx, "attention");
   return T2SC_OK;
 }

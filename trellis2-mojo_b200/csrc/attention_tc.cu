@@ -127,6 +127,7 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
   const int warp = uniform((int)threadIdx.x >> 5), lane = threadIdx.x & 31, wg = warp >> 2;
   constexpr int kTmaWarp = 4 * NT, kMmaWarp = 4 * NT + 1, kFeedWarp = 4 * NT + 2;
 
+  sm100::next_kernel_may_start();
   if (warp == kTmaWarp && lane == 0) {
     sm100::tma_prefetch(&a.map_q);
     sm100::tma_prefetch(&a.map_k);
@@ -182,6 +183,7 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
   sm100::tc_fence_before();
   __syncthreads();
   sm100::tc_fence_after();
+  sm100::previous_kernel_done();
   const uint32_t tmem = uniform(*tmem_slot);
   const int head = uniform(where[0]), q0 = uniform(where[1]), here = min(uniform(where[2]), NT * kBQ), kv0 = uniform(where[3]),
             kv_len = uniform(where[4]);
@@ -543,47 +545,9 @@ int launch(t2sc_seqs *s, const AttnArgs &a, int splits, std::string &err) {
   }
   static std::atomic<uint64_t> allowed{0};
   T2SC_TRY(allow_smem(ctx, kernel, (int)S::kSmem, allowed, err));
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid), cfg.blockDim = dim3(S::kThreads), cfg.dynamicSmemBytes = S::kSmem, cfg.stream = ctx->stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = splits, at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at, cfg.numAttrs = 1;
-  T2SC_CUDA(cudaLaunchKernelEx(&cfg, kernel, t), "attention");
+  T2SC_CUDA(launch_overlapped(kernel, grid, S::kThreads, S::kSmem, ctx->stream, splits, t), "attention");
   T2SC_LAUNCHED(ctx, "attention");
   return T2SC_OK;
-}
-
-// Clusters of n CTAs that the device runs at once with one CTA an SM (asked
-// for once per device; the occupancy query counts one CTA of a kernel with
-// tensor memory an SM, two run).
-struct Clusters {
-  std::atomic<int> known{0};
-  int at_once[kMaxSplits + 1] = {};
-};
-
-template <class K>
-const int *clusters_at_once(t2sc_ctx *ctx, K kernel, int threads, size_t smem, Clusters (&table)[64]) {
-  Clusters &t = table[ctx->device & 63];
-  if (!t.known.load(std::memory_order_acquire)) {
-    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    for (int n = 1; n <= kMaxSplits; n++) {
-      cudaLaunchConfig_t cfg = {};
-      cfg.gridDim = dim3(n * 1024), cfg.blockDim = dim3(threads), cfg.dynamicSmemBytes = smem;
-      cudaLaunchAttribute at[1];
-      at[0].id = cudaLaunchAttributeClusterDimension;
-      at[0].val.clusterDim.x = n, at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-      cfg.attrs = at, cfg.numAttrs = 1;
-      int count = 0;
-      if (cudaOccupancyMaxActiveClusters(&count, kernel, &cfg) != cudaSuccess) {
-        cudaGetLastError();
-        count = ctx->num_sms / n;
-      }
-      t.at_once[n] = count;
-    }
-    t.known.store(1, std::memory_order_release);
-  }
-  return t.at_once;
 }
 
 template <int DT, int DP>
@@ -602,8 +566,9 @@ int launch_dp(t2sc_seqs *s, const AttnArgs &a, std::string &err) {
   const int64_t pairs = s->blocks256 * a.heads, singles = s->blocks128 * a.heads;
   double least = (double)((pairs + s->ctx->num_sms - 1) / s->ctx->num_sms) * (units * kPair + kFixed);
   int best = 0;
-  static Clusters table[64];
-  const int *at_once = clusters_at_once(s->ctx, attention_tc_kernel<DT, DP, 1>, Shape<DP, 1>::kThreads, Shape<DP, 1>::kSmem, table);
+  static Clusters<kMaxSplits> table[64];
+  const int *at_once = nullptr;
+  T2SC_TRY(clusters_at_once(s->ctx, attention_tc_kernel<DT, DP, 1>, Shape<DP, 1>::kThreads, Shape<DP, 1>::kSmem, table, &at_once, err));
   for (int n = 1; n <= kMaxSplits; n++) {
     if (at_once[n] < 1 || (n > 1 && units < 4 * n)) continue;
     const int64_t rounds = (singles + at_once[n] - 1) / at_once[n];

@@ -39,7 +39,9 @@ __device__ __forceinline__ float activate(float v, int act) {
 // 16-bit rows that start on 16 bytes (what TMA needs of x and w).
 bool dense_tc_takes(const DenseArgs &a, int dtype);
 int dense_tc(t2sc_ctx *ctx, const DenseArgs &a, int dtype, std::string &err);
-// Such rows, few of them.
+// What its best tile shape (*best) is expected to take.
+double dense_tc_us(t2sc_ctx *ctx, const DenseArgs &a, int *best);
+// Such rows, few of them, or few tiles of outputs over a long K axis.
 bool dense_skinny_takes(t2sc_ctx *ctx, const DenseArgs &a, int dtype);
 int dense_skinny(t2sc_ctx *ctx, const DenseArgs &a, int dtype, std::string &err);
 // At most 2 such rows, ci a multiple of 8.

@@ -15,6 +15,7 @@
 #include "dense.h"
 #include "entry.h"
 #include "internal.h"
+#include "sm100.cuh"
 
 namespace t2sc {
 namespace {
@@ -41,6 +42,7 @@ __device__ __forceinline__ float ld16(const char *p, int64_t i) {
 template <int DT, int R, int UNROLL>
 __global__ void __launch_bounds__(32 * kWarps) dense_rows_kernel(const DenseArgs a, int slices) {
   __shared__ float sums[kWarps][R][kOut];
+  sm100::previous_kernel_done();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int slice = warp % slices, groups = kWarps / slices;
   const int o0 = ((int)blockIdx.x * groups + warp / slices) * kOut;
@@ -114,11 +116,9 @@ int launch(t2sc_ctx *ctx, const DenseArgs &a, std::string &err) {
   // K slices until there are 16 warps an SM, at least two K blocks a slice
   int slices = 1;
   while (slices < kWarps && out_groups * slices < 16 * ctx->num_sms && blocks >= 4 * slices) slices *= 2;
-  const unsigned grid = (unsigned)((out_groups + kWarps / slices - 1) / (kWarps / slices));
-  if (a.rows == 1)
-    dense_rows_kernel<DT, 1, 3><<<grid, 32 * kWarps, 0, ctx->stream>>>(a, slices);
-  else
-    dense_rows_kernel<DT, 2, 2><<<grid, 32 * kWarps, 0, ctx->stream>>>(a, slices);
+  const int grid = (out_groups + kWarps / slices - 1) / (kWarps / slices);
+  auto kernel = a.rows == 1 ? dense_rows_kernel<DT, 1, 3> : dense_rows_kernel<DT, 2, 2>;
+  T2SC_CUDA(launch_overlapped(kernel, grid, 32 * kWarps, 0, ctx->stream, 1, a, slices), "dense_linear");
   T2SC_LAUNCHED(ctx, "dense_linear");
   return T2SC_OK;
 }

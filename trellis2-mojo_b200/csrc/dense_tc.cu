@@ -89,6 +89,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
   const uint32_t tfull0 = empty0 + 8 * NS, tempty0 = tfull0 + 16, done = tempty0 + 16;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = CG == 2 ? sm100::cluster_rank() : 0;
+  sm100::next_kernel_may_start();
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < NS; s++) {
@@ -116,6 +117,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
   __syncthreads();
   if (CG == 2) sm100::cluster_sync();  // the other CTA's barriers are ready before anything arrives on them
   sm100::tc_fence_after();
+  sm100::previous_kernel_done();
   const uint32_t tmem = *tmem_slot;
   const int64_t ntiles = (int64_t)a.m_tiles * a.n_tiles;
   const int64_t slot = blockIdx.x / CG;
@@ -382,36 +384,27 @@ int launch(t2sc_ctx *ctx, const DenseArgs &a, std::string &err) {
   auto kernel = dense_tc_kernel<DT, CG, BN>;
   static std::atomic<uint64_t> allowed{0};
   T2SC_TRY(allow_smem(ctx, kernel, (int)S::kSmem, allowed, err));
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)t.slots * CG), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = S::kSmem, cfg.stream = ctx->stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = CG, at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at, cfg.numAttrs = 1;
-  T2SC_CUDA(cudaLaunchKernelEx(&cfg, kernel, t), "dense_linear");
+  T2SC_CUDA(launch_overlapped(kernel, (int64_t)t.slots * CG, kThreads, S::kSmem, ctx->stream, CG, t), "dense_linear");
   T2SC_LAUNCHED(ctx, "dense_linear");
   return T2SC_OK;
 }
 
+// The tile shapes: rounds of tiles x (a K step x K steps + the tile's own) + the
+// launch, the first tiles' way in and the last one's epilogue, in microseconds
+// as measured with weights out of L2 ([64..1000] rows, 1024..8192 -> 128..6144:
+// within 7 %). A step is bound by what an SM takes in, 55 of its 64 bytes a
+// clock from L2, but for the pair's 256 columns, where the products are close.
+struct Option {
+  int cg, bn;
+  double step, rest;
+};
+constexpr Option kOptions[] = {{2, 256, 0.31, 5.5}, {2, 128, 0.24, 3.7}, {1, 128, 0.25, 2.9}, {1, 64, 0.218, 3.1}};
+constexpr double kTile = 0.6;
+
 template <int DT>
 int launch_dt(t2sc_ctx *ctx, const DenseArgs &a, std::string &err) {
-  // The tile shape that finishes first: rounds of tiles x (clocks of a K step
-  // of that shape x K steps + a tile's fixed part).
-  struct Option {
-    int cg, bn;
-    double step;
-  };
-  constexpr Option options[] = {{2, 256, 520}, {2, 128, 300}, {1, 128, 330}, {1, 64, 220}};
-  const double k_iters = (a.ci + kBK - 1) / kBK;
   int best = 0;
-  double least = 1e300;
-  for (int i = 0; i < 4; i++) {
-    const Option &o = options[i];
-    const double tiles = (double)((a.rows + kTileM * o.cg - 1) / (kTileM * o.cg)) * ((a.co + o.bn - 1) / o.bn);
-    const double slots = ctx->num_sms / o.cg, rounds = (double)(int64_t)((tiles + slots - 1) / slots);
-    const double clocks = rounds * (k_iters * o.step + 600) + 8 * o.bn;
-    if (clocks < least) least = clocks, best = i;
-  }
+  dense_tc_us(ctx, a, &best);
   switch (best) {
     case 0: return launch<DT, 2, 256>(ctx, a, err);
     case 1: return launch<DT, 2, 128>(ctx, a, err);
@@ -421,6 +414,18 @@ int launch_dt(t2sc_ctx *ctx, const DenseArgs &a, std::string &err) {
 }
 
 }  // namespace
+
+double dense_tc_us(t2sc_ctx *ctx, const DenseArgs &a, int *best) {
+  const double k_iters = (a.ci + kBK - 1) / kBK;
+  double least = 1e300;
+  for (int i = 0; i < 4; i++) {
+    const Option &o = kOptions[i];
+    const int64_t tiles = ((a.rows + kTileM * o.cg - 1) / (kTileM * o.cg)) * ((a.co + o.bn - 1) / o.bn), slots = ctx->num_sms / o.cg;
+    const double us = (double)((tiles + slots - 1) / slots) * (k_iters * o.step + kTile) + o.rest;
+    if (us < least) least = us, *best = i;
+  }
+  return least;
+}
 
 bool dense_tc_takes(const DenseArgs &a, int dtype) {
   auto on16 = [](const void *p, int64_t ld, int64_t rows) {

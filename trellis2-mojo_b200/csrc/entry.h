@@ -70,6 +70,57 @@ int allow_smem(t2sc_ctx *ctx, K kernel, int bytes, std::atomic<uint64_t> &done, 
   return T2SC_OK;
 }
 
+// Clusters of 1 to MAX CTAs, one CTA an SM, that a device runs at once; 0: not
+// known. Asked for once per device and kernel (the query counts one CTA of a
+// kernel with tensor memory an SM, where two run).
+template <int MAX>
+struct Clusters {
+  std::atomic<int> known{0};
+  int at_once[MAX + 1] = {};
+};
+
+template <int MAX, class K>
+int clusters_at_once(t2sc_ctx *ctx, K kernel, int threads, size_t smem, Clusters<MAX> (&table)[64], const int **out, std::string &err) {
+  Clusters<MAX> &t = table[ctx->device & 63];
+  if (!t.known.load(std::memory_order_acquire)) {
+    T2SC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "shared memory size");
+    if (MAX > 8) T2SC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "cluster size");
+    for (int n = 1; n <= MAX; n++) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(n * 1024), cfg.blockDim = dim3(threads), cfg.dynamicSmemBytes = smem;
+      cudaLaunchAttribute at[1];
+      at[0].id = cudaLaunchAttributeClusterDimension;
+      at[0].val.clusterDim.x = n, at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+      cfg.attrs = at, cfg.numAttrs = 1;
+      int count = 0;
+      if (cudaOccupancyMaxActiveClusters(&count, kernel, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        count = 0;
+      }
+      t.at_once[n] = count;
+    }
+    t.known.store(1, std::memory_order_release);
+  }
+  *out = t.at_once;
+  return T2SC_OK;
+}
+
+// Launches a kernel that begins while the one before it on the stream ends
+// (see next_kernel_may_start), in clusters of `cluster` CTAs.
+template <class A, class... Args>
+cudaError_t launch_overlapped(void (*kernel)(A, Args...), int64_t grid, int threads, size_t smem, cudaStream_t stream, int cluster,
+                              const A &first, Args... rest) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid), cfg.blockDim = dim3((unsigned)threads), cfg.dynamicSmemBytes = smem, cfg.stream = stream;
+  cudaLaunchAttribute at[2] = {};
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = (unsigned)cluster, at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cfg.attrs = at, cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kernel, first, rest...);
+}
+
 inline bool dtype_known(int dtype) { return dtype == T2SC_DT_F32 || dtype == T2SC_DT_F16 || dtype == T2SC_DT_BF16; }
 inline int dtype_size(int dtype) { return dtype == T2SC_DT_F32 ? 4 : 2; }
 

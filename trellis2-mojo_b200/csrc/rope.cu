@@ -116,6 +116,7 @@ template <int DT, bool NORM, bool PAIRS, int R>
 __global__ void __launch_bounds__(kThreads) rope_vec_kernel(const RopeArgs a, int t_rows, int lanes, int chunks, int slots) {
   constexpr int E = Chunk<DT>::kElems, H = E / 2;  // values of a chunk, packed pairs of them
   extern __shared__ float2 turn[];                 // [t_rows][pairs]
+  sm100::previous_kernel_done();
   const int groups = (int)blockDim.x / lanes, gid = (int)threadIdx.x / lanes, sub = (int)threadIdx.x % lanes;
   const int64_t row0 = (int64_t)blockIdx.x * t_rows;
   const int here = (int)min((int64_t)t_rows, a.rows - row0);
@@ -311,7 +312,8 @@ int launch(t2sc_ctx *ctx, const RopeArgs &a, std::string &err) {
       const int threads = (int)std::min<int64_t>(kThreads, (t_rows * row_threads + 31) / 32 * 32);
       const int64_t grid = (a.rows + t_rows - 1) / t_rows;
       const size_t smem = (size_t)t_rows * (a.head_dim / 2) * sizeof(float2);  // <= 16 x 128 x 8 bytes
-      rope_vec_kernel<DT, NORM, PAIRS, R><<<(unsigned)grid, threads, smem, ctx->stream>>>(a, (int)t_rows, lanes, chunks, slots);
+      T2SC_CUDA(launch_overlapped(rope_vec_kernel<DT, NORM, PAIRS, R>, grid, threads, smem, ctx->stream, 1, a, (int)t_rows, lanes, chunks, slots),
+                "rope");
       T2SC_LAUNCHED(ctx, "rope");
       return T2SC_OK;
     };
