@@ -837,3 +837,20 @@ def test_calls_in_a_row_see_each_others_results(t2sc):
             bufs[0].copy_(start)
             graph.replay()
             assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("d", [64, 128, 40])
+@pytest.mark.parametrize("q_len", [1, 2, 4])
+def test_attention_more_short_calls_than_sms(t2sc, dtype, d, q_len):
+    """Few queries of more sequences and heads than SMs, keys of none, of one and of many blocks, bad values behind them."""
+    import torch
+    g = _gen(24 + d + q_len)
+    kv_lens = [0, 1, 33, 64, 65, 700, 129, 2, 0, 5] * 3
+    q_lens = [q_len if i % 7 else 1 for i in range(len(kv_lens))]
+    n = sum(kv_lens)
+    q = _normal(g, sum(q_lens), 12, d, dtype=dtype)
+    k, v = (torch.full((n + 64, 12, d), NAN, device="cuda", dtype=getattr(torch, dtype)) for _ in range(2))
+    k[:n], v[:n] = (_normal(g, n, 12, d, dtype=dtype) for _ in range(2))
+    y = t2sc.SequenceLayout(q_lens, kv_lens).attention_device(q, k, v)
+    ref.assert_close(y, *ref.attention(q, k[:n], v[:n], q_lens, kv_lens, d ** -0.5))

@@ -5,10 +5,11 @@
 //
 // One warp brings blocks of keys, K and V, into a ring of shared-memory
 // stages by TMA: 192 KB of an SM in flight (held in registers instead, a
-// third of that, the call ran at half the speed). 16 warps take a few keys of
-// a block each: 8 channels a lane, G lanes a key, 32 / G keys a step. Every
-// group of G lanes keeps its own running maximum, sum and f32 output of each
-// query; they are merged over the warp by shuffles, over the CTA's warps
+// third of that, the call ran at half the speed), in one CTA, or in two where
+// there are more sequences and heads than SMs. Its 16 or 8 warps take a few
+// keys of a block each: 8 channels a lane, G lanes a key, 32 / G keys a step.
+// Every group of G lanes keeps its own running maximum, sum and f32 output of
+// each query; they are merged over the warp by shuffles, over the CTA's warps
 // through shared memory and over the cluster's CTAs, which split the keys,
 // through distributed shared memory, in a fixed order.
 #include <cuda_bf16.h>
@@ -26,9 +27,15 @@
 namespace t2sc {
 namespace {
 
-constexpr int kMaxRows = 4, kWarps = 16, kMaxSplits = 16, kThreads = 32 * (kWarps + 1);
-constexpr int kStages = 6, kStageBytes = 32768;  // K block, then V block, 16 KB each
-constexpr size_t kSmem = 1024 + kStages * kStageBytes;
+constexpr int kMaxRows = 4, kMaxSplits = 16, kStages = 6;
+
+// W: warps that compute, 16 with one CTA an SM, 8 with two.
+template <int W>
+struct Shape {
+  static constexpr int kWarps = W, kThreads = 32 * (W + 1);
+  static constexpr int kStageBytes = W * 2048;  // K block, then V block
+  static constexpr size_t kSmem = 1024 + kStages * kStageBytes;
+};
 constexpr long long kWaitLimit = 4000000000ll;  // ~2 s of SM clocks
 
 struct RowsArgs {
@@ -64,10 +71,11 @@ __device__ __forceinline__ void unpack8(const uint4 &u, float (&f)[8]) {
 __device__ __forceinline__ float weight(float m, float to) { return m == to ? 1.f : ex2(m - to); }
 
 // Maxima are of scores times log2(e).
-template <int DT, int G, int R>
-__global__ void __launch_bounds__(kThreads, 1) attention_rows_kernel(const __grid_constant__ RowsArgs x) {
+template <int DT, int G, int R, int W>
+__global__ void __launch_bounds__(Shape<W>::kThreads, 16 / W) attention_rows_kernel(const __grid_constant__ RowsArgs x) {
+  constexpr int kWarps = W, kThreads = Shape<W>::kThreads, kStageBytes = Shape<W>::kStageBytes;
   constexpr int kKeys = 32 / G, kSteps = 2;              // keys a warp and step, steps a block
-  constexpr int kBlock = kWarps * kKeys * kSteps;        // keys a stage: 128 of 64 channels, 64 of 128
+  constexpr int kBlock = kWarps * kKeys * kSteps;        // keys a stage: with 16 warps 128 of 64 channels, 64 of 128
   constexpr int kSub = G / 8;                            // 64-channel halves, each rows of 128 bytes
   static_assert(kBlock * 128 * kSub == kStageBytes / 2, "a block fills half a stage");
   extern __shared__ __align__(1024) uint8_t raw[];
@@ -271,10 +279,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_rows_kernel(const __gri
   sm100::cluster_sync();  // no CTA leaves before the others have read its sums
 }
 
-template <int DT, int G, int R>
+template <int DT, int G, int R, int W>
 int launch(t2sc_seqs *s, const AttnArgs &a, std::string &err) {
+  constexpr int kThreads = Shape<W>::kThreads;
+  constexpr size_t kSmem = Shape<W>::kSmem;
   t2sc_ctx *ctx = s->ctx;
-  auto kernel = attention_rows_kernel<DT, G, R>;
+  auto kernel = attention_rows_kernel<DT, G, R, W>;
   static Clusters<kMaxSplits> table[64];
   const int *at_once = nullptr;
   T2SC_TRY(clusters_at_once(ctx, kernel, kThreads, kSmem, table, &at_once, err));
@@ -282,14 +292,15 @@ int launch(t2sc_seqs *s, const AttnArgs &a, std::string &err) {
   x.a = a;
   x.c = a.scale * 1.4426950408889634f;
   x.err = ctx->d_err;
-  constexpr int block = kWarps * (32 / G) * 2;
+  constexpr int block = W * (32 / G) * 2;
   // The number of key splits that ends first: rounds of clusters x blocks of
-  // the longest sequence a CTA takes (+ 2 for what it costs to begin and end).
+  // the longest sequence a CTA takes (+ 2 of 32 KB for what it costs to begin
+  // and end).
   const int64_t ctas = s->batch * a.heads, blocks = (s->max_kv + block - 1) / block;
   int64_t least = INT64_MAX;
   for (int n = 1; n <= kMaxSplits; n++) {
     if (at_once[n] < 1 || (n > 1 && n > blocks)) continue;
-    const int64_t cost = ((ctas + at_once[n] - 1) / at_once[n]) * ((blocks + n - 1) / n + 2);
+    const int64_t cost = ((ctas + at_once[n] - 1) / at_once[n]) * ((blocks + n - 1) / n + 32 / W);
     if (cost < least) least = cost, x.splits = n;
   }
   if (ctas * x.splits > INT32_MAX) return fail(ctx, T2SC_ERR_UNSUPPORTED, "attention: too many sequences and heads in one call");
@@ -307,11 +318,21 @@ int launch(t2sc_seqs *s, const AttnArgs &a, std::string &err) {
   return T2SC_OK;
 }
 
+template <int DT, int G, int R>
+int launch_warps(t2sc_seqs *s, const AttnArgs &a, std::string &err) {
+  // More sequences and heads than SMs: two CTAs of half the size an SM, one's
+  // begin and end beside the other's keys (12 sequences of 600 keys, 16 x 64:
+  // 9.5 us, 13.8 with one; 32 of 6000 122 and 130). Fewer, whose keys are
+  // split: one (6 of 6000, 12 x 128: 38 us, 43 with two).
+  if (s->batch * a.heads > s->ctx->num_sms) return launch<DT, G, R, 8>(s, a, err);
+  return launch<DT, G, R, 16>(s, a, err);
+}
+
 template <int DT, int G>
 int launch_rows(t2sc_seqs *s, const AttnArgs &a, std::string &err) {
-  if (s->max_q == 1) return launch<DT, G, 1>(s, a, err);
-  if (s->max_q == 2) return launch<DT, G, 2>(s, a, err);
-  return launch<DT, G, 4>(s, a, err);
+  if (s->max_q == 1) return launch_warps<DT, G, 1>(s, a, err);
+  if (s->max_q == 2) return launch_warps<DT, G, 2>(s, a, err);
+  return launch_warps<DT, G, 4>(s, a, err);
 }
 
 template <int DT>
