@@ -196,6 +196,12 @@ int t2sc_seqs_create(t2sc_ctx *ctx, const int64_t *q_offsets, const int64_t *kv_
       s->max_q = std::max<int64_t>(s->max_q, sorted[b].y);
       s->max_kv = std::max<int64_t>(s->max_kv, sorted[b].w);
     }
+    for (const int4 &q : sorted) {
+      const int64_t b256 = ((int64_t)q.y + 255) / 256, b128 = ((int64_t)q.y + 127) / 128;
+      const double units = (double)(((int64_t)q.w + 63) / 64);
+      s->work256 += b256 * units, s->work128 += b128 * units;
+      if ((int64_t)q.w * 8 >= s->max_kv * 7) s->long256 += b256, s->long128 += b128, s->long_q = std::max<int64_t>(s->long_q, q.y);
+    }
     for (int64_t b = 0; b <= 8; b++) {
       s->few_blocks256[b] = b <= batch ? blocks[b] : 0, s->few_blocks128[b] = b <= batch ? blocks[batch + 1 + b] : 0;
       if (b < 8) s->few_seqs[b] = b < batch ? sorted[b] : make_int4(0, 0, 0, 0);

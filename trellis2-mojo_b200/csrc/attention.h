@@ -15,6 +15,9 @@ struct t2sc_seqs {
   int64_t q_total = 0;                 // query rows inside sequences
   int64_t max_q = 0, max_kv = 0;       // queries, keys of the longest sequence
   int64_t blocks32 = 0, blocks128 = 0, blocks256 = 0;  // blocks of 32 / 128 / 256 query rows, sequence by sequence
+  int64_t long128 = 0, long256 = 0;    // blocks of 128 / 256 rows of sequences with at least 7/8 of the longest one's keys
+  int64_t long_q = 0;                  // most queries of one of these
+  double work128 = 0, work256 = 0;     // sum over the blocks of their units of 64 keys
   int4 *d_sorted = nullptr;            // as d_seqs, most keys first
   int64_t *d_blocks = nullptr;         // [3][batch + 1] blocks of 256 / 128 rows before each of d_sorted, of 32 rows before each of d_seqs
   // the first sequences of d_sorted and d_blocks, for kernels to carry in their arguments

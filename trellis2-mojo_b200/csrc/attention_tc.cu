@@ -553,27 +553,40 @@ int launch(t2sc_seqs *s, const AttnArgs &a, int splits, std::string &err) {
 template <int DT, int DP>
 int launch_dp(t2sc_seqs *s, const AttnArgs &a, std::string &err) {
   // What ends first, in the time that one query block alone on an SM takes
-  // for a unit (0.67 us at head_dim 128): a CTA's rounds x (its units x what
-  // one takes + kFixed to begin and end). With two query blocks a CTA a pair
-  // of units takes kPair (0.83 us); with one, and its keys in n parts, two
-  // CTAs that share an SM take kShared for a unit of both, and kExchange goes
-  // to the parts' exchange. 300 queries over 20000 keys, 12 x 128: 75 us with
-  // the 6 parts this finds, 98 with 8 (two rounds), 99 with 4, 262 with two
-  // blocks a CTA; 20 x 300 tokens, 16 x 64: 39 us with one part, 47 with two
-  // blocks a CTA.
-  constexpr double kFixed = 8, kPair = 1.25, kShared = 1.6, kExchange = 3;
-  const double units = (double)((s->max_kv + kUnit - 1) / kUnit);
-  const int64_t pairs = s->blocks256 * a.heads, singles = s->blocks128 * a.heads;
-  double least = (double)((pairs + s->ctx->num_sms - 1) / s->ctx->num_sms) * (units * kPair + kFixed);
+  // for a unit (0.67 us at head_dim 128). A CTA takes its units x what one
+  // takes + kFixed to begin and end: with two query blocks a CTA a pair of
+  // units takes kPair (0.83 us); with one, and its keys in n parts, two CTAs
+  // that share an SM take kShared for a unit of both, and kExchange goes to
+  // the parts' exchange. The end is that of the longest sequences' rounds of
+  // CTAs, or, where others follow them, of all CTAs' time spread over the SMs
+  // and half a CTA, and not before the rounds that they would take with a unit
+  // each. 300 queries over 20000 keys, 12 x 128: 75 us with the 6
+  // parts this finds, 98 with 8 (two rounds), 99 with 4, 262 with two blocks a
+  // CTA; 20 x 300 tokens, 16 x 64: 39 us with one part, 47 with two blocks a
+  // CTA; 21888 queries over 1029 keys, 16 x 64: 180 us with one block, 189
+  // with two, 12 x 128 179 and 150.
+  constexpr double kFixed = 8, kPair = 1.25, kShared = DP == 64 ? 1.25 : 1.6, kExchange = 3;
+  const double units = (double)((s->max_kv + kUnit - 1) / kUnit), heads = a.heads, sms = s->ctx->num_sms;
+  auto rounds = [&](int64_t blocks, int64_t slots) { return (blocks * a.heads + slots - 1) / slots; };
+  double least = (double)rounds(s->long256, s->ctx->num_sms) * (units * (s->long_q > kBQ ? kPair : 1) + kFixed);
+  if (s->long256 < s->blocks256) {
+    const double all = s->work256 * kPair + s->blocks256 * kFixed;
+    least = std::max({least, all * heads / sms + all / s->blocks256 / 2, (double)rounds(s->blocks256, s->ctx->num_sms) * (kPair + kFixed)});
+  }
   int best = 0;
   static Clusters<kMaxSplits> table[64];
   const int *at_once = nullptr;
   T2SC_TRY(clusters_at_once(s->ctx, attention_tc_kernel<DT, DP, 1>, Shape<DP, 1>::kThreads, Shape<DP, 1>::kSmem, table, &at_once, err));
   for (int n = 1; n <= kMaxSplits; n++) {
     if (at_once[n] < 1 || (n > 1 && units < 4 * n)) continue;
-    const int64_t rounds = (singles + at_once[n] - 1) / at_once[n];
-    const double part = (double)((int64_t)(units + n - 1) / n);
-    const double cost = (double)(rounds / 2) * (part * kShared + kFixed) + (double)(rounds % 2) * (part + kFixed) + (n > 1 ? kExchange : 0);
+    const int64_t r = rounds(s->long128, at_once[n]);
+    const double part = (double)((int64_t)(units + n - 1) / n), fixed = n > 1 ? kFixed + kExchange : kFixed;
+    double cost = (double)(r / 2) * (part * kShared + fixed) + (double)(r % 2) * (part + fixed);
+    if (s->long128 < s->blocks128) {
+      const double all = s->work128 / n * kShared + s->blocks128 * fixed;  // of two CTAs that share an SM
+      cost = std::max({cost, all * heads / (2 * at_once[n]) + all / s->blocks128 / 2,
+                       (double)rounds(s->blocks128, 2 * at_once[n]) * (kShared + fixed)});
+    }
     if (cost < least) least = cost, best = n;
   }
   return best == 0 ? launch<DT, DP, 2>(s, a, 1, err) : launch<DT, DP, 1>(s, a, best, err);
