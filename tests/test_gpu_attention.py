@@ -854,3 +854,24 @@ def test_attention_more_short_calls_than_sms(t2sc, dtype, d, q_len):
     k[:n], v[:n] = (_normal(g, n, 12, d, dtype=dtype) for _ in range(2))
     y = t2sc.SequenceLayout(q_lens, kv_lens).attention_device(q, k, v)
     ref.assert_close(y, *ref.attention(q, k[:n], v[:n], q_lens, kv_lens, d ** -0.5))
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("rows,ci,co", [(1000, 136, 2143), (777, 64, 321), (4000, 40, 65), (300, 72, 4100)])
+def test_linear_odd_rows_of_many_tiles(t2sc, dtype, rows, ci, co):
+    """Tiles whose rows start anywhere: odd widths, the last columns and rows of a tile, in place and not."""
+    import torch
+    g = _gen(rows + co)
+    x, w, b = _normal(g, rows, ci, dtype=dtype), _normal(g, co, ci, std=ci ** -0.5, dtype=dtype), _normal(g, co)
+    for pad in (0, 3, 8):
+        rv, buf = _inside(rows, co, dtype, pad_cols=pad)
+        rv.copy_(_normal(g, rows, co, dtype=dtype))
+        want = ref.linear(x, w, b, "silu", rv.clone())
+        first = t2sc.dense_linear_device(x, w, b, activation="silu", residual=rv)
+        t2sc.dense_linear_device(x, w, b, activation="silu", residual=rv, out=rv)
+        assert torch.equal(first, rv) and _untouched(buf, rows, co)
+        ref.assert_close(rv, *want)
+        plain, buf = _inside(rows, co, dtype, pad_cols=pad)
+        t2sc.dense_linear_device(x, w, out=plain)
+        assert _untouched(buf, rows, co)
+        ref.assert_close(plain, *ref.linear(x, w))
