@@ -77,6 +77,14 @@ class Context:
         check(lib.t2sc_ctx_set_stream(self.handle, ctypes.c_void_p(stream_ptr) if stream_ptr else None),
               self.handle)
 
+    def use_torch_stream(self):
+        """Runs this context's work on the stream that is torch's current one
+        on its device at the time of the call. (The operators over CUDA
+        tensors, attention.py, follow torch's current stream by themselves.)"""
+        import torch
+        # handle 0, torch's default stream, would name the context's own; 1 is cudaStreamLegacy, the same stream
+        self.set_stream(torch.cuda.current_stream(self.device).cuda_stream or 1)
+
     def close(self):
         if self._beside_torch is not None:
             self._beside_torch.close()
