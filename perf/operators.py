@@ -161,6 +161,7 @@ def prepare(case, seed):
         if own:
             t2sc = _t2sc()
             s["ctx"] = t2sc.Context.default(0)
+            s["ctx"].use_torch_stream()
             s["rope"] = t2sc.RotaryPositionEmbedder(d, theta=THETA, layout=case["layout"], ctx=s["ctx"])
     else:
         q, kv = _lens(case["q"]), _lens(case["kv"])
@@ -174,12 +175,14 @@ def prepare(case, seed):
         if own:
             t2sc = _t2sc()
             s["ctx"] = t2sc.Context.default(0)
+            s["ctx"].use_torch_stream()
             s["layout"] = t2sc.SequenceLayout(q, kv, ctx=s["ctx"])
         else:
             s["rows"], s["q_at"], _ = _padded(q)
             _, s["kv_at"], s["kv_there"] = _padded(kv)
     if own and case["op"] == "linear":
         s["ctx"] = _t2sc().Context.default(0)
+        s["ctx"].use_torch_stream()
     return s
 
 
