@@ -1,0 +1,55 @@
+"""The attention-block operators where calls meet: kernels that overlap the one
+before them, several streams and threads, and the ends of what a call may be.
+Bounds and plain 64-bit forms: _attention_ref.py."""
+import pytest
+
+import _attention_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+
+def _gen(seed):
+    import torch
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _normal(g, *shape, std=1.0, dtype="float32"):
+    import torch
+    return (torch.randn(shape, generator=g, device="cuda") * std).to(getattr(torch, dtype))
+
+
+@pytest.mark.parametrize("d,lens", [(64, [900, 2100]), (128, [1500]), (64, [40, 260])])
+def test_kernels_with_tensor_memory_behind_each_other(t2sc, d, lens):
+    """Attention, which takes most or all of an SM's tensor memory, and linear calls of few and of many rows behind it, on two
+    streams at once: every call's result is the one that it has alone."""
+    import torch
+    g = _gen(d + sum(lens))
+    heads, n = 8, sum(lens)
+    c = heads * d
+    work = []
+    for i in range(2):
+        ctx = t2sc.Context(0)
+        q, k, v = (_normal(g, n, heads, d, dtype="bfloat16") for _ in range(3))
+        w = _normal(g, 256, c, std=c ** -0.5, dtype="bfloat16")
+        work.append((ctx, torch.cuda.Stream(), t2sc.SequenceLayout(lens, ctx=ctx), q, k, v, w))
+
+    def calls(ctx, layout, q, k, v, w):
+        a = layout.attention_device(q, k, v).view(n, c)
+        return [a] + [t2sc.dense_linear_device(a[:m], w, ctx=ctx) for m in (5, 40, 600, n) if m <= n]
+
+    want = []
+    for ctx, stream, layout, q, k, v, w in work:
+        want.append(calls(ctx, layout, q, k, v, w))
+        torch.cuda.synchronize()
+        ref.assert_close(want[-1][0].view(n, heads, d), *ref.attention(q, k, v, lens, lens, d ** -0.5))
+        ref.assert_close(want[-1][-1], *ref.linear(want[-1][0], w))
+    got = [[], []]
+    for rep in range(20):
+        for i, (ctx, stream, layout, q, k, v, w) in enumerate(work):
+            with torch.cuda.stream(stream):
+                got[i].append(calls(ctx, layout, q, k, v, w))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for ys in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(ys, want[i]))
+        work[i][0].synchronize()

@@ -127,7 +127,6 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
   const int warp = uniform((int)threadIdx.x >> 5), lane = threadIdx.x & 31, wg = warp >> 2;
   constexpr int kTmaWarp = 4 * NT, kMmaWarp = 4 * NT + 1, kFeedWarp = 4 * NT + 2;
 
-  sm100::next_kernel_may_start();
   if (warp == kTmaWarp && lane == 0) {
     sm100::tma_prefetch(&a.map_q);
     sm100::tma_prefetch(&a.map_k);
@@ -183,6 +182,7 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
   sm100::tc_fence_before();
   __syncthreads();
   sm100::tc_fence_after();
+  sm100::next_kernel_may_start();
   sm100::previous_kernel_done();
   const uint32_t tmem = uniform(*tmem_slot);
   const int head = uniform(where[0]), q0 = uniform(where[1]), here = min(uniform(where[2]), NT * kBQ), kv0 = uniform(where[3]),

@@ -116,7 +116,6 @@ __global__ void __launch_bounds__(kThreads, 2) dense_skinny_kernel(const __grid_
   const int o0 = tile / a.row_tiles * kM, row0 = tile % a.row_tiles * N;  // the row tiles of a piece of w are neighbours
   const int rows = min(N, a.rows - row0);
   const int per = (a.k_iters + a.slices - 1) / a.slices, k0 = min(slice * per, a.k_iters), n = min(k0 + per, a.k_iters) - k0;
-  sm100::next_kernel_may_start();
   if (warp == 4 && lane == 0) {
     sm100::tma_prefetch(&a.map_x);
     sm100::tma_prefetch(&a.map_w);
@@ -137,6 +136,7 @@ __global__ void __launch_bounds__(kThreads, 2) dense_skinny_kernel(const __grid_
   sm100::tc_fence_before();
   __syncthreads();
   sm100::tc_fence_after();
+  sm100::next_kernel_may_start();
   sm100::previous_kernel_done();
   const uint32_t tmem = *tmem_slot;
   if (warp == 4) {

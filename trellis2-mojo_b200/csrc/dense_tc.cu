@@ -92,7 +92,6 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
   const uint32_t tfull0 = empty0 + 8 * NS, tempty0 = tfull0 + 16, done = tempty0 + 16;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = CG == 2 ? sm100::cluster_rank() : 0;
-  sm100::next_kernel_may_start();
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < NS; s++) {
@@ -120,6 +119,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
   __syncthreads();
   if (CG == 2) sm100::cluster_sync();  // the other CTA's barriers are ready before anything arrives on them
   sm100::tc_fence_after();
+  sm100::next_kernel_may_start();
   sm100::previous_kernel_done();
   const uint32_t tmem = *tmem_slot;
   const int64_t ntiles = (int64_t)a.m_tiles * a.n_tiles;

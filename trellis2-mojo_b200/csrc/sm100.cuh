@@ -201,7 +201,10 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t saddr, uint32_t row_bytes
 // kernel may have written, before it writes, and before it ends. Kernels with
 // a preamble (barriers, tensor memory) also let the next one begin its own as
 // soon as all their blocks run; those without leave it to their end, where the
-// next one's waiting blocks take no room from theirs. An attention block's six
+// next one's waiting blocks take no room from theirs. A block that allocates
+// tensor memory does so before it lets the next kernel start: that one's blocks
+// keep what they allocate until this kernel has ended, so that a block which
+// still had to allocate could wait for them, and they for it. An attention block's six
 // calls in a graph: one row of 1536 channels 21.2 -> 19.9 us, [4000, 1024] 230
 // -> 226; attention alone, 1203 + 738 tokens, 26.8 -> 24.9 us.
 __device__ __forceinline__ void next_kernel_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
