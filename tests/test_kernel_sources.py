@@ -40,3 +40,13 @@ def test_tensor_memory_is_allocated_before_the_next_kernel_may_start(name):
     assert "__syncthreads()" in between
     if "tmem_alloc_pair" in text:
         assert "cluster_sync()" in between
+
+
+@pytest.mark.parametrize("name", SOURCES)
+def test_non_coherent_loads_are_of_the_handles_own_tables(name):
+    """__ldg needs memory that nothing writes during the kernel's whole life. An overlapped kernel's life begins while the one
+    before it writes, so rows, weights, gains, biases and coordinates are read by ordinary loads."""
+    text = SOURCES[name]
+    asked = [re.match(r"\s*(reinterpret_cast<[^>]*>\()?\s*([\w.]+)", text[m.end():]).group(2)
+             for m in re.finditer(r"\b__ldg\(", text)]
+    assert set(asked) <= {"a.seqs", "a.blocks", "a.turns"}, asked

@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(Shape<W>::kThreads, 16 / W) attention_rows_ker
 #pragma unroll
     for (int r = 0; r < R; r++) {
       uint4 u = make_uint4(0, 0, 0, 0);
-      if (r < rows && in) u = __ldg(reinterpret_cast<const uint4 *>(a.q + ((int64_t)(seq.x + r) * a.ldq + at) * 2));
+      if (r < rows && in) u = *reinterpret_cast<const uint4 *>(a.q + ((int64_t)(seq.x + r) * a.ldq + at) * 2);
       unpack8<DT>(u, q[r]);
       m[r] = -INFINITY, l[r] = 0.f;
 #pragma unroll

@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(32 * kWarps) dense_rows_kernel(const DenseArgs
     for (int i = 0; i < UNROLL; i++) {
       const bool in = kb + i < k_last && (kb + i) * 32 + lane < chunks;
 #pragma unroll
-      for (int o = 0; o < kOut; o++) wr[i][o] = in ? __ldg(w[o] + (kb + i) * 32) : make_uint4(0, 0, 0, 0);
+      for (int o = 0; o < kOut; o++) wr[i][o] = in ? w[o][(kb + i) * 32] : make_uint4(0, 0, 0, 0);
     }
 #pragma unroll
     for (int i = 0; i < UNROLL; i++) {
@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(32 * kWarps) dense_rows_kernel(const DenseArgs
 #pragma unroll
       for (int r = 0; r < R; r++) {
         float xf[8];
-        unpack8<DT>(in ? __ldg(x[r] + (kb + i) * 32) : make_uint4(0, 0, 0, 0), xf);
+        unpack8<DT>(in ? x[r][(kb + i) * 32] : make_uint4(0, 0, 0, 0), xf);
 #pragma unroll
         for (int o = 0; o < kOut; o++)
 #pragma unroll
@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(32 * kWarps) dense_rows_kernel(const DenseArgs
     if (r >= a.rows || col >= a.co) continue;
     float v = 0.f;
     for (int s = 0; s < slices; s++) v += sums[g * slices + s][r][o];
-    if (a.bias) v += __ldg(a.bias + col);
+    if (a.bias) v += a.bias[col];
     v = activate(v, a.act);
     if (a.res) v += ld16<DT>(a.res, r * a.ldr + col);
     if (DT == T2SC_DT_BF16)

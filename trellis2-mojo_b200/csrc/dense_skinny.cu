@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(kThreads, 2) dense_skinny_kernel(const __grid_
     const uint32_t at = sm100::smem_u32(sums) + 4 * c4;
     float b4[4];
 #pragma unroll
-    for (int j = 0; j < 4; j++) b4[j] = a.bias && o0 + c4 + j < a.co ? __ldg(a.bias + o0 + c4 + j) : 0.f;
+    for (int j = 0; j < 4; j++) b4[j] = a.bias && o0 + c4 + j < a.co ? a.bias[o0 + c4 + j] : 0.f;
     const int step = a.slices * 4;
     for (int r = slice + a.slices * warp; r < rows; r += 2 * step) {  // two rows at a time
       float4 t[2][kMaxSlices];

@@ -235,8 +235,8 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
       float bias0, bias1;
       auto load_bias = [&](int col0) {
         const int col = col0 + lane;
-        bias0 = a.bias && col < a.co ? __ldg(a.bias + col) : 0.f;
-        bias1 = a.bias && col + 32 < a.co ? __ldg(a.bias + col + 32) : 0.f;
+        bias0 = a.bias && col < a.co ? a.bias[col] : 0.f;
+        bias1 = a.bias && col + 32 < a.co ? a.bias[col + 32] : 0.f;
       };
       uint32_t res[32];  // whole rows: a lane's 8 chunks; else row r's columns lane and lane + 32
       auto load_residual = [&](int col0) {

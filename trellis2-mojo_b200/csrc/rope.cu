@@ -60,7 +60,7 @@ struct RopeArgs {
 // cos and sin of pair p at the coordinates of one row.
 __device__ __forceinline__ float2 turn_of(const RopeArgs &a, int64_t row, int p) {
   const int axis = p < a.n0 ? 0 : (p < a.n01 ? 1 : 2);
-  double t = (double)__ldg(a.coords + row * 4 + 1 + axis) * __ldg(a.turns + p);
+  double t = (double)a.coords[row * 4 + 1 + axis] * __ldg(a.turns + p);
   t -= rint(t);
   float s, c;
   sincospif((float)(2.0 * t), &s, &c);
@@ -134,8 +134,8 @@ __global__ void __launch_bounds__(kThreads) rope_vec_kernel(const RopeArgs a, in
       raw[r][0] = raw[r][1] = make_uint4(0, 0, 0, 0);
       if (live && h0 + r < a.per_row) {
         const char *p = a.in[t] + (row0 + row) * a.in_stride[t] + h * 2 * half + sub * 16;
-        raw[r][0] = __ldcs(reinterpret_cast<const uint4 *>(p));
-        raw[r][1] = __ldcs(reinterpret_cast<const uint4 *>(p + half));
+        raw[r][0] = sm100::ld_streaming(p);
+        raw[r][1] = sm100::ld_streaming(p + half);
       }
     }
     if (base == 0) {
@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(kThreads) rope_vec_kernel(const RopeArgs a, in
           for (int q = 0; q < 2; q++)
 #pragma unroll
             for (int e4 = 0; e4 < E / 4; e4++) {
-              const ulonglong2 m = __ldg(reinterpret_cast<const ulonglong2 *>(g + q * pairs) + e4);
+              const ulonglong2 m = reinterpret_cast<const ulonglong2 *>(g + q * pairs)[e4];
               uint64_t *z = x + q * H + e4 * 2;
               z[0] = sm100::mul_f32x2(z[0], sm100::mul_f32x2(m.x, inv2));
               z[1] = sm100::mul_f32x2(z[1], sm100::mul_f32x2(m.y, inv2));
@@ -277,7 +277,7 @@ __global__ void __launch_bounds__(kThreads) rope_scalar_kernel(const RopeArgs a)
     const int iu = PAIRS ? 2 * p : p, iv = PAIRS ? 2 * p + 1 : p + half;
     if (NORM) {
       const float *g = a.gain[t] + h * a.head_dim;
-      u[q] *= inv * __ldg(g + iu), v[q] *= inv * __ldg(g + iv);
+      u[q] *= inv * g[iu], v[q] *= inv * g[iv];
     }
     if (p < a.rotated) {
       const float2 cs = turn_of(a, row, p);

@@ -207,8 +207,19 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t saddr, uint32_t row_bytes
 // still had to allocate could wait for them, and they for it. An attention block's six
 // calls in a graph: one row of 1536 channels 21.2 -> 19.9 us, [4000, 1024] 230
 // -> 226; attention alone, 1203 + 738 tokens, 26.8 -> 24.9 us.
+//
+// What another kernel may have written is read by ordinary loads behind
+// previous_kernel_done(), or by ld_streaming: __ldg is for memory that nothing
+// writes during the kernel's whole life, which here begins while the kernel
+// before still writes (a handle's own tables are such memory).
 __device__ __forceinline__ void next_kernel_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void previous_kernel_done() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// 16 bytes that are read once.
+__device__ __forceinline__ uint4 ld_streaming(const void *p) {
+  uint4 u;
+  asm volatile("ld.global.cs.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "l"(p) : "memory");
+  return u;
+}
 
 // ---- clusters ----
 __device__ __forceinline__ uint32_t cluster_rank() {
