@@ -70,6 +70,13 @@ int t2sc_ctx_destroy(t2sc_ctx *ctx);
  * context's own stream; cudaStreamLegacy, (void *)1, is the legacy default
  * stream). */
 int t2sc_ctx_set_stream(t2sc_ctx *ctx, void *cuda_stream);
+/* As t2sc_ctx_set_stream, for calls that go to several streams in turn: what
+ * the context has launched on the stream that it leaves stays covered by
+ * t2sc_ctx_synchronize and t2sc_ctx_destroy (an event is recorded on that
+ * stream, which must still exist). */
+int t2sc_ctx_switch_stream(t2sc_ctx *ctx, void *cuda_stream);
+/* Waits for the context's work and returns T2SC_ERR_TIMEOUT or another status
+ * where a kernel of it has reported an error since the last time. */
 int t2sc_ctx_synchronize(t2sc_ctx *ctx);
 const char *t2sc_last_error(const t2sc_ctx *ctx);
 /* Kernel launches issued by this context since creation (diagnostics). */

@@ -53,3 +53,36 @@ def test_kernels_with_tensor_memory_behind_each_other(t2sc, d, lens):
         for ys in got[i]:
             assert all(torch.equal(a, b) for a, b in zip(ys, want[i]))
         work[i][0].synchronize()
+
+
+def test_synchronize_waits_for_every_stream(t2sc):
+    """A call that still waits on one torch stream, then one on another: Context.synchronize alone leaves both streams idle, and
+    so does close; calls captured in between run only when their graph is replayed."""
+    import torch
+    g = _gen(1)
+    ctx = t2sc.Context(0)
+    x, w = _normal(g, 300, 64, dtype="bfloat16"), _normal(g, 96, 64, std=0.125, dtype="bfloat16")
+    want = t2sc.dense_linear_device(x, w, ctx=ctx)
+    layout = t2sc.SequenceLayout([300], ctx=ctx)
+    q = x.view(300, 1, 64)
+    torch.cuda.synchronize()
+    a, b, c = (torch.cuda.Stream() for _ in range(3))
+    for end in (ctx.synchronize, ctx.synchronize, ctx.close):
+        graph = torch.cuda.CUDAGraph()
+        for stream in (a, b):
+            with torch.cuda.stream(stream):
+                torch.cuda._sleep(400_000_000)
+                y = t2sc.dense_linear_device(x, w, ctx=ctx)
+        with torch.cuda.stream(c):
+            graph.capture_begin()
+            z = layout.attention_device(q, q, q)
+            graph.capture_end()
+        t2sc.dense_linear_device(x, w, ctx=ctx)
+        assert not a.query() and not b.query()
+        end()
+        assert a.query() and b.query()
+        assert torch.equal(y, want)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.isfinite(z).all()
+        del graph

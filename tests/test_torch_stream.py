@@ -26,7 +26,7 @@ def test_use_torch_stream_sets_torchs_stream(t2sc, monkeypatch, torch_handle, wa
     asked, given = [], []
     monkeypatch.setattr(torch.cuda, "current_stream",
                         lambda device=None: asked.append(device) or types.SimpleNamespace(cuda_stream=torch_handle))
-    monkeypatch.setattr(ctx, "set_stream", given.append)
+    monkeypatch.setattr(ctx, "_switch_stream", given.append)
     ctx.use_torch_stream()
     assert asked == [3] and given == [want]
 

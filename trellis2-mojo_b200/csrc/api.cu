@@ -32,9 +32,46 @@ struct DevBuf {
   }
 };
 
+bool capturing(cudaStream_t stream) {
+  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(stream, &st) == cudaSuccess) return st != cudaStreamCaptureStatusNone;
+  cudaGetLastError();  // the legacy stream while one that waits for it is captured
+  return true;
+}
+
+// Remembers the work on the context's stream, which it is about to leave. No
+// event goes into a graph that is being captured there.
+int note_left(t2sc_ctx *ctx) {
+  std::string &err = ctx->last_error;
+  cudaEvent_t &event = ctx->left[ctx->stream];
+  if (capturing(ctx->stream)) return T2SC_OK;
+  if (!event) T2SC_CUDA(cudaEventCreateWithFlags(&event, cudaEventDisableTiming), "stream switch");
+  T2SC_CUDA(cudaEventRecord(event, ctx->stream), "stream switch");
+  return T2SC_OK;
+}
+
+int wait_left(t2sc_ctx *ctx) {
+  std::string &err = ctx->last_error;
+  for (auto it = ctx->left.begin(); it != ctx->left.end();) {
+    if (it->second) {
+      T2SC_CUDA(cudaEventSynchronize(it->second), "stream synchronize");
+      cudaEventDestroy(it->second);
+    } else if (!capturing(it->first)) {
+      T2SC_CUDA(cudaStreamSynchronize(it->first), "stream synchronize");
+    } else {
+      ++it;
+      continue;
+    }
+    it = ctx->left.erase(it);
+  }
+  return T2SC_OK;
+}
+
 int check_sync(t2sc_ctx *ctx) {
   std::string &err = ctx->last_error;
   T2SC_CUDA(cudaStreamSynchronize(ctx->stream), "stream synchronize");
+  T2SC_TRY(wait_left(ctx));
+  ctx->launches_waited = ctx->launches;
   int flags = 0;
   T2SC_TRY(read_dev_err(ctx, &flags));
   if (flags & kDevErrTimeout)
@@ -95,6 +132,9 @@ int t2sc_ctx_destroy(t2sc_ctx *ctx) {
   if (!ctx) return T2SC_OK;
   DeviceGuard g(ctx->device);
   cudaStreamSynchronize(ctx->stream);
+  wait_left(ctx);
+  for (auto &kv : ctx->left)
+    if (kv.second) cudaEventDestroy(kv.second);
   for (void *p : ctx->stage)
     if (p) cudaFree(p);
   for (auto &kv : ctx->id_maps) free_map(kv.second);
@@ -112,10 +152,26 @@ int t2sc_ctx_set_stream(t2sc_ctx *ctx, void *stream) {
   return T2SC_OK;
 }
 
+int t2sc_ctx_switch_stream(t2sc_ctx *ctx, void *stream) {
+  if (!ctx) return T2SC_ERR_INVALID;
+  const cudaStream_t to = stream ? static_cast<cudaStream_t>(stream) : ctx->own_stream;
+  if (to == ctx->stream) return T2SC_OK;
+  return guarded(ctx, [&]() -> int {
+    DeviceGuard g(ctx->device);
+    CaptureTolerant relaxed;
+    if (ctx->launches != ctx->launches_waited) T2SC_TRY(note_left(ctx));
+    ctx->launches_waited = ctx->launches;
+    ctx->stream = to;
+    return T2SC_OK;
+  });
+}
+
 int t2sc_ctx_synchronize(t2sc_ctx *ctx) {
   if (!ctx) return T2SC_ERR_INVALID;
-  DeviceGuard g(ctx->device);
-  return check_sync(ctx);
+  return guarded(ctx, [&]() -> int {
+    DeviceGuard g(ctx->device);
+    return check_sync(ctx);
+  });
 }
 
 const char *t2sc_last_error(const t2sc_ctx *ctx) { return ctx ? ctx->last_error.c_str() : "null context"; }

@@ -38,6 +38,10 @@ struct t2sc_ctx {
   int num_sms = 148;
   cudaStream_t own_stream = nullptr;
   cudaStream_t stream = nullptr;
+  // streams that t2sc_ctx_switch_stream left with work on them, each with an
+  // event behind that work (null: none could be recorded), until waited for
+  std::map<cudaStream_t, cudaEvent_t> left;
+  int64_t launches_waited = 0;  // launches up to the last switch or wait
   int *d_err = nullptr;      // device error flags (one int)
   int64_t launches = 0;      // kernels launched by this context
   std::string last_error;

@@ -29,6 +29,7 @@ SIGNATURES = {
     "t2sc_ctx_create": (I32, [I32, PP]),
     "t2sc_ctx_destroy": (I32, [P]),
     "t2sc_ctx_set_stream": (I32, [P, P]),
+    "t2sc_ctx_switch_stream": (I32, [P, P]),
     "t2sc_ctx_synchronize": (I32, [P]),
     "t2sc_last_error": (ctypes.c_char_p, [P]),
     "t2sc_ctx_launch_count": (I32, [P, PI64]),

@@ -63,6 +63,7 @@ class Context:
         return (self,) if self._beside_torch is None else (self, self._beside_torch)
 
     def synchronize(self):
+        """Waits for the context's work, on torch's streams too, and raises what its kernels reported."""
         for c in self._both():
             check(lib.t2sc_ctx_synchronize(c.handle), c.handle)
 
@@ -83,7 +84,10 @@ class Context:
         tensors, attention.py, follow torch's current stream by themselves.)"""
         import torch
         # handle 0, torch's default stream, would name the context's own; 1 is cudaStreamLegacy, the same stream
-        self.set_stream(torch.cuda.current_stream(self.device).cuda_stream or 1)
+        self._switch_stream(torch.cuda.current_stream(self.device).cuda_stream or 1)
+
+    def _switch_stream(self, stream_ptr):
+        check(lib.t2sc_ctx_switch_stream(self.handle, ctypes.c_void_p(stream_ptr)), self.handle)
 
     def close(self):
         if self._beside_torch is not None:
@@ -103,7 +107,7 @@ class TorchContext:
         self.stream = None    # as last set; None: the context's own
 
     def use(self, stream):
-        check(lib.t2sc_ctx_set_stream(self.handle, ctypes.c_void_p(stream)), self.handle)
+        check(lib.t2sc_ctx_switch_stream(self.handle, ctypes.c_void_p(stream)), self.handle)
         self.stream = stream
 
     def close(self):
