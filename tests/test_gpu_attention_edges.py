@@ -86,3 +86,52 @@ def test_synchronize_waits_for_every_stream(t2sc):
         torch.cuda.synchronize()
         assert torch.isfinite(z).all()
         del graph
+
+
+def test_threads_share_a_context(t2sc):
+    """Threads with a stream each and one context: every call runs on its own thread's stream, behind the rows that are
+    written there late."""
+    import threading
+    import torch
+    g = _gen(2)
+    ctx = t2sc.Context(0)
+    threads, reps = 4, 40
+    new = [_normal(g, 40, 128, dtype="bfloat16") for _ in range(threads)]
+    w = _normal(g, 256, 128, std=0.1, dtype="bfloat16")
+    gain, coords = torch.ones(2, 64, device="cuda"), torch.arange(160, device="cuda", dtype=torch.int32).view(40, 4)
+    rope, layout = t2sc.RotaryPositionEmbedder(64, ctx=ctx), t2sc.SequenceLayout([40], ctx=ctx)
+
+    def calls(x):
+        y = t2sc.dense_linear_device(x, w, ctx=ctx)
+        q = x.view(40, 2, 64)
+        z = t2sc.qk_norm_rope_device(q, None, gain, None, coords=coords, rope=rope)[0]
+        return [y, z, layout.attention_device(rope.forward_device(z, coords), z, z)]
+
+    want = [calls(x) for x in new]
+    torch.cuda.synchronize()
+    bad, start = [], threading.Barrier(threads)
+
+    def work(i):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                rows = torch.zeros_like(new[i])
+                stream.synchronize()
+                start.wait()
+                for rep in range(reps):
+                    rows.zero_()
+                    torch.cuda._sleep(300_000)
+                    rows.copy_(new[i])
+                    got = calls(rows)
+                    if not all(bool(torch.equal(p, q)) for p, q in zip(got, want[i])):
+                        bad.append((i, rep))
+        except Exception as e:  # noqa: BLE001
+            bad.append(e)
+
+    pool = [threading.Thread(target=work, args=(i,)) for i in range(threads)]
+    for t in pool:
+        t.start()
+    for t in pool:
+        t.join()
+    ctx.synchronize()
+    assert not bad, bad[:3]

@@ -2,9 +2,9 @@
 
 Operators over CUDA tensors of rows, each one C-ABI call on torch's current
 stream (the stream of the Context that they are given stays as it was set).
-They are for inference: results carry no gradient. As all calls of a Context,
-those of one Context (and of the handles made with it) come from one thread at
-a time.
+They are for inference: results carry no gradient. Several threads may call
+them with one Context and its handles, or without one; each call runs on its
+own thread's current stream.
   dense_linear_device      act(x @ w^T + bias) + residual   (linear, trellis2_mojo/modules/nn.mojo:27-266)
   RotaryPositionEmbedder   rotary positions over x, y, z    (trellis2_mojo/modules/rope.mojo)
   qk_norm_rope_device      per-head RMS norm + rotation     (bias_rms_rope_qkv, trellis2_mojo/gpu/attention.mojo:507)
@@ -97,7 +97,8 @@ def _context(ctx, t):
 
 
 def _on_torch_stream(ctx):
-    """The library context to call with, its work on torch's current stream of the device."""
+    """The library context to call with, its work on torch's current stream of the device. Under the context's lock,
+    which is held until the call is made and its error is read."""
     stream = torch.cuda.current_stream(ctx.device).cuda_stream if _raw_stream is None else _raw_stream(ctx.device)
     stream = stream or 1    # handle 0 would name the context's own stream, 1 is cudaStreamLegacy
     beside = ctx._beside_torch or ctx.beside_torch()
@@ -138,11 +139,12 @@ def dense_linear_device(x, weight, bias=None, activation=None, residual=None, ou
             raise ValueError("dense_linear: out must be [rows, co]")
     b = None if bias is None else _f32(bias, device, (co,), "dense_linear: bias")
     if rows:
-        handle = _on_torch_stream(ctx)
-        rc = _linear(handle, x.data_ptr(), ldx, weight.data_ptr(), ldw, b, res, ldr, out.data_ptr(), ldy, rows, co, ci,
-                     flags, code)
-        if rc:
-            check(rc, handle)
+        with ctx._lock:
+            handle = _on_torch_stream(ctx)
+            rc = _linear(handle, x.data_ptr(), ldx, weight.data_ptr(), ldw, b, res, ldr, out.data_ptr(), ldy, rows, co, ci,
+                         flags, code)
+            if rc:
+                check(rc, handle)
     return out
 
 
@@ -163,9 +165,11 @@ class RotaryPositionEmbedder:
         if len(self.pairs) != 3:
             raise ValueError("RotaryPositionEmbedder: pairs are three counts, of x, y and z")
         self.ctx = ctx or Context.default()
-        h, beside = ctypes.c_void_p(), self.ctx.beside_torch().handle
-        check(lib.t2sc_rope_create(beside, self.head_dim, *self.pairs, self.theta, _LAYOUTS[layout], ctypes.byref(h)),
-              beside)
+        h = ctypes.c_void_p()
+        with self.ctx._lock:
+            beside = self.ctx.beside_torch().handle
+            check(lib.t2sc_rope_create(beside, self.head_dim, *self.pairs, self.theta, _LAYOUTS[layout], ctypes.byref(h)),
+                  beside)
         self.handle = h
 
     def forward_device(self, x, coords, out=None):
@@ -184,10 +188,11 @@ class RotaryPositionEmbedder:
             if (r, h, e) != (rows, heads, d):
                 raise ValueError("RotaryPositionEmbedder: out must have x's shape")
         if rows:
-            handle = _on_torch_stream(ctx)
-            rc = _rope_apply(self.handle, at, x.data_ptr(), ldx, out.data_ptr(), ldy, rows, heads, code)
-            if rc:
-                check(rc, handle)
+            with ctx._lock:
+                handle = _on_torch_stream(ctx)
+                rc = _rope_apply(self.handle, at, x.data_ptr(), ldx, out.data_ptr(), ldy, rows, heads, code)
+                if rc:
+                    check(rc, handle)
         return out
 
     def __del__(self):
@@ -234,11 +239,12 @@ def qk_norm_rope_device(q, k, gain_q, gain_k, coords=None, rope=None, eps=1e-6, 
         raise ValueError("qk_norm_rope: out_k without k")
     at = _coords(coords, device, rows) if rope is not None else None
     if rows:
-        handle = _on_torch_stream(ctx)
-        rc = _qk_norm_rope(handle, None if rope is None else rope.handle, at, q.data_ptr(), ldq, kp, ldk, gq, gk,
-                           out_q.data_ptr(), ldqo, kop, ldko, rows, heads, d, eps, code)
-        if rc:
-            check(rc, handle)
+        with ctx._lock:
+            handle = _on_torch_stream(ctx)
+            rc = _qk_norm_rope(handle, None if rope is None else rope.handle, at, q.data_ptr(), ldq, kp, ldk, gq, gk,
+                               out_q.data_ptr(), ldqo, kop, ldko, rows, heads, d, eps, code)
+            if rc:
+                check(rc, handle)
     return out_q, out_k
 
 
@@ -256,9 +262,11 @@ class SequenceLayout:
             raise ValueError("SequenceLayout: as many key lengths as query lengths")
         self.q_rows, self.kv_rows = int(self.q_offsets[-1]), int(self.kv_offsets[-1])
         self.ctx = ctx or Context.default()
-        h, beside = ctypes.c_void_p(), self.ctx.beside_torch().handle
-        check(lib.t2sc_seqs_create(beside, self.q_offsets.ctypes.data, self.kv_offsets.ctypes.data,
-                                   len(self.q_offsets) - 1, ctypes.byref(h)), beside)
+        h = ctypes.c_void_p()
+        with self.ctx._lock:
+            beside = self.ctx.beside_torch().handle
+            check(lib.t2sc_seqs_create(beside, self.q_offsets.ctypes.data, self.kv_offsets.ctypes.data,
+                                       len(self.q_offsets) - 1, ctypes.byref(h)), beside)
         self.handle = h
 
     @classmethod
@@ -297,11 +305,12 @@ class SequenceLayout:
             r, h, e, ldo = _heads3d(out, device, dtype, "attention: out")
             if (r, h, e) != (rows, heads, d):
                 raise ValueError("attention: out must have q's shape")
-        handle = _on_torch_stream(ctx)
-        rc = _attention(self.handle, q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, out.data_ptr(), ldo, heads, d,
-                        d ** -0.5 if scale is None else scale, code)
-        if rc:
-            check(rc, handle)
+        with ctx._lock:
+            handle = _on_torch_stream(ctx)
+            rc = _attention(self.handle, q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, out.data_ptr(), ldo, heads, d,
+                            d ** -0.5 if scale is None else scale, code)
+            if rc:
+                check(rc, handle)
         return out
 
     def __del__(self):

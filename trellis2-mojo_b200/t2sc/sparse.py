@@ -16,6 +16,7 @@ coordinate hash and neighbour maps live on the device in a handle shared by
 every tensor derived through ``replace`` (the reference's spatial cache).
 """
 import ctypes
+import threading
 
 import numpy as np
 
@@ -33,6 +34,7 @@ class Context:
     """One per device; replaces GpuContext (trellis2_mojo/gpu/context.mojo:116-165)."""
 
     _default = {}
+    _default_lock = threading.Lock()
 
     def __init__(self, device=0):
         h = ctypes.c_void_p()
@@ -41,12 +43,19 @@ class Context:
         self.handle = h
         self.device = device
         self._beside_torch = None
+        # held over a call of the operators that follow torch's stream: setting the stream, the launch and
+        # reading an error are one step, whichever thread they come from
+        self._lock = threading.Lock()
 
     @classmethod
     def default(cls, device=0):
-        if device not in cls._default:
-            cls._default[device] = cls(device)
-        return cls._default[device]
+        ctx = cls._default.get(device)
+        if ctx is None:
+            with cls._default_lock:
+                if device not in cls._default:
+                    cls._default[device] = cls(device)
+                ctx = cls._default[device]
+        return ctx
 
     def selftest(self, wait_us=2000):
         """Compute check + a bounded device wait that must time out cleanly."""
@@ -54,7 +63,8 @@ class Context:
 
     def beside_torch(self):
         """The library context of the operators that follow torch's current
-        stream, so that they leave the stream of this one as it was set."""
+        stream, so that they leave the stream of this one as it was set. Made
+        and used under the context's lock."""
         if self._beside_torch is None:
             self._beside_torch = TorchContext(self.device)
         return self._beside_torch
@@ -64,8 +74,9 @@ class Context:
 
     def synchronize(self):
         """Waits for the context's work, on torch's streams too, and raises what its kernels reported."""
-        for c in self._both():
-            check(lib.t2sc_ctx_synchronize(c.handle), c.handle)
+        with self._lock:
+            for c in self._both():
+                check(lib.t2sc_ctx_synchronize(c.handle), c.handle)
 
     def launch_count(self):
         v, n = ctypes.c_int64(), 0
