@@ -302,8 +302,9 @@ int t2sc_dense_linear_device(t2sc_ctx *ctx, const void *x, int64_t x_stride, con
  * 2p and 2p + 1 (PAIRS) or p and p + head_dim / 2 (HALVES). Angles are formed
  * in 64 bits: to f32 precision for positions up to 2^26, within 2^-20 radians
  * for every int32 position. head_dim even, 2..256. Destroying a handle waits
- * for the kernels that read it; a graph that captured calls with one needs it
- * for as long as it is replayed (t2sc_seqs too). */
+ * for the kernels that read it, and may follow its context's destruction; a
+ * graph that captured calls with one needs it for as long as it is replayed
+ * (t2sc_seqs too). */
 #define T2SC_ROPE_PAIRS 0
 #define T2SC_ROPE_HALVES 1
 typedef struct t2sc_rope t2sc_rope;

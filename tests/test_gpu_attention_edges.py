@@ -135,3 +135,28 @@ def test_threads_share_a_context(t2sc):
         t.join()
     ctx.synchronize()
     assert not bad, bad[:3]
+
+
+def test_a_closed_context(t2sc):
+    """After Context.close its handles' calls are refused, and dropping the handles still gives their memory back."""
+    import gc
+    import torch
+    g = _gen(5)
+    ctx = t2sc.Context(0)
+    x, w = _normal(g, 6, 64, dtype="bfloat16"), _normal(g, 64, 64, dtype="bfloat16")
+    q, coords, gain = x.view(6, 1, 64), torch.zeros(6, 4, device="cuda", dtype=torch.int32), torch.ones(1, 64, device="cuda")
+    rope, layout = t2sc.RotaryPositionEmbedder(64, ctx=ctx), t2sc.SequenceLayout([6] + [0] * ((1 << 20) - 1), ctx=ctx)
+    layout.attention_device(rope.forward_device(q, coords), q, q)
+    ctx.close()
+    ctx.close()
+    for call in (lambda: t2sc.dense_linear_device(x, w, ctx=ctx), lambda: rope.forward_device(q, coords),
+                 lambda: t2sc.qk_norm_rope_device(q, None, gain, None, coords=coords, rope=rope),
+                 lambda: layout.attention_device(q, q, q), lambda: t2sc.SequenceLayout([3], ctx=ctx),
+                 lambda: t2sc.RotaryPositionEmbedder(64, ctx=ctx)):
+        with pytest.raises((ValueError, t2sc.T2SCError)):
+            call()
+    torch.cuda.synchronize()
+    before = torch.cuda.mem_get_info()[0]
+    del layout, rope
+    gc.collect()
+    assert torch.cuda.mem_get_info()[0] - before >= 40 << 20   # 2 x 16 MB of sequences, 24 MB of block counts

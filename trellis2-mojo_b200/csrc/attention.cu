@@ -177,6 +177,7 @@ int t2sc_seqs_create(t2sc_ctx *ctx, const int64_t *q_offsets, const int64_t *kv_
     std::string &err = ctx->last_error;
     std::unique_ptr<t2sc_seqs, int (*)(t2sc_seqs *)> s(new t2sc_seqs(), t2sc_seqs_destroy);
     s->ctx = ctx;
+    s->device = ctx->device;
     s->batch = batch;
     s->q_off.assign(q_offsets, q_offsets + batch + 1);
     s->kv_off.assign(kv_offsets, kv_offsets + batch + 1);
@@ -226,7 +227,7 @@ int t2sc_seqs_create(t2sc_ctx *ctx, const int64_t *q_offsets, const int64_t *kv_
 
 int t2sc_seqs_destroy(t2sc_seqs *s) {
   if (!s) return T2SC_OK;
-  DeviceGuard g(s->ctx->device);
+  DeviceGuard g(s->device);
   CaptureTolerant relaxed;
   if (s->d_seqs) cudaFree(s->d_seqs);  // waits for the kernels that read it, on whatever stream
   delete s;

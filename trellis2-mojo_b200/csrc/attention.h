@@ -9,6 +9,7 @@
 
 struct t2sc_seqs {
   t2sc_ctx *ctx = nullptr;
+  int device = 0;  // the context's, which may be gone when the handle is destroyed
   int64_t batch = 0;
   std::vector<int64_t> q_off, kv_off;  // [batch + 1]
   int64_t q_rows = 0, kv_rows = 0;     // rows up to the last offset

@@ -33,6 +33,7 @@
 
 struct t2sc_rope {
   t2sc_ctx *ctx = nullptr;
+  int device = 0;  // the context's, which may be gone when the handle is destroyed
   int head_dim = 0, layout = 0, rotated = 0;  // rotated: pairs that turn; the others stay
   double *d_turns = nullptr;                  // [rotated] turns per unit of position
   int n_axis[3] = {0, 0, 0};
@@ -402,6 +403,7 @@ int t2sc_rope_create(t2sc_ctx *ctx, int head_dim, int pairs_x, int pairs_y, int 
     std::string &err = ctx->last_error;
     std::unique_ptr<t2sc_rope, int (*)(t2sc_rope *)> r(new t2sc_rope(), t2sc_rope_destroy);
     r->ctx = ctx;
+    r->device = ctx->device;
     r->head_dim = head_dim;
     r->layout = layout;
     r->rotated = n[0] + n[1] + n[2];
@@ -423,7 +425,7 @@ int t2sc_rope_create(t2sc_ctx *ctx, int head_dim, int pairs_x, int pairs_y, int 
 
 int t2sc_rope_destroy(t2sc_rope *r) {
   if (!r) return T2SC_OK;
-  DeviceGuard g(r->ctx->device);
+  DeviceGuard g(r->device);
   CaptureTolerant relaxed;
   if (r->d_turns) cudaFree(r->d_turns);  // waits for the kernels that read it, on whatever stream
   delete r;

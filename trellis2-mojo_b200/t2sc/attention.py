@@ -102,6 +102,8 @@ def _on_torch_stream(ctx):
     stream = torch.cuda.current_stream(ctx.device).cuda_stream if _raw_stream is None else _raw_stream(ctx.device)
     stream = stream or 1    # handle 0 would name the context's own stream, 1 is cudaStreamLegacy
     beside = ctx._beside_torch or ctx.beside_torch()
+    if not beside.handle:
+        raise ValueError("the Context is closed")
     if beside.stream != stream:
         beside.use(stream)
     return beside.handle
@@ -197,7 +199,7 @@ class RotaryPositionEmbedder:
 
     def __del__(self):
         h = getattr(self, "handle", None)
-        if h and lib is not None and self.ctx.handle:   # None: the interpreter is shutting down
+        if h and lib is not None:   # None: the interpreter is shutting down
             lib.t2sc_rope_destroy(h)
             self.handle = None
 
@@ -315,7 +317,7 @@ class SequenceLayout:
 
     def __del__(self):
         h = getattr(self, "handle", None)
-        if h and lib is not None and self.ctx.handle:   # None: the interpreter is shutting down
+        if h and lib is not None:   # None: the interpreter is shutting down
             lib.t2sc_seqs_destroy(h)
             self.handle = None
 

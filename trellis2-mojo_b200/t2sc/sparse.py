@@ -66,6 +66,8 @@ class Context:
         stream, so that they leave the stream of this one as it was set. Made
         and used under the context's lock."""
         if self._beside_torch is None:
+            if not self.handle:
+                raise ValueError("the Context is closed")
             self._beside_torch = TorchContext(self.device)
         return self._beside_torch
 
@@ -101,11 +103,12 @@ class Context:
         check(lib.t2sc_ctx_switch_stream(self.handle, ctypes.c_void_p(stream_ptr)), self.handle)
 
     def close(self):
-        if self._beside_torch is not None:
-            self._beside_torch.close()
-        if self.handle:
-            lib.t2sc_ctx_destroy(self.handle)
-            self.handle = None
+        with self._lock:
+            if self._beside_torch is not None:
+                self._beside_torch.close()
+            if self.handle:
+                lib.t2sc_ctx_destroy(self.handle)
+                self.handle = None
 
 
 class TorchContext:
