@@ -163,3 +163,33 @@ def test_a_closed_context(t2sc):
     del layout, rope
     gc.collect()
     assert torch.cuda.mem_get_info()[0] - before >= 40 << 20   # 2 x 16 MB of sequences, 24 MB of block counts
+
+
+def test_gradients_are_refused_not_dropped(t2sc):
+    """Inputs that ask for gradients under grad mode are refused by every operator; without grad mode they run."""
+    import torch
+    g = _gen(4)
+    x, w, b = (_normal(g, *s, dtype="bfloat16") for s in ((20, 64), (64, 64), (20, 64)))
+    bias, gain = torch.zeros(64, device="cuda"), torch.ones(1, 64, device="cuda")
+    coords = torch.zeros(20, 4, device="cuda", dtype=torch.int32)
+    rope, layout = t2sc.RotaryPositionEmbedder(64), t2sc.SequenceLayout([20])
+    q = x.view(20, 1, 64)
+    leaf = lambda t: t.clone().requires_grad_()  # noqa: E731
+    calls = [lambda f: t2sc.dense_linear_device(f(x), w), lambda f: t2sc.dense_linear_device(x, f(w)),
+             lambda f: t2sc.dense_linear_device(x, w, f(bias)), lambda f: t2sc.dense_linear_device(x, w, residual=f(b)),
+             lambda f: t2sc.dense_linear_device(x, w, out=f(b)),
+             lambda f: rope.forward_device(f(q), coords), lambda f: rope.forward_device(q, coords, out=f(q)),
+             lambda f: t2sc.qk_norm_rope_device(f(q), None, gain, None)[0], lambda f: t2sc.qk_norm_rope_device(q, f(q), gain, gain)[0],
+             lambda f: t2sc.qk_norm_rope_device(q, q, f(gain), gain)[0], lambda f: t2sc.qk_norm_rope_device(q, q, gain, f(gain))[0],
+             lambda f: layout.attention_device(f(q), q, q), lambda f: layout.attention_device(q, f(q), q),
+             lambda f: layout.attention_device(q, q, f(q)), lambda f: layout.attention_device(q, q, q, out=f(q))]
+    for call in calls:
+        with pytest.raises(ValueError, match="gradient"):
+            call(leaf)
+        want = call(torch.clone)
+        with torch.no_grad():
+            y = call(leaf)
+        with torch.inference_mode():
+            z = call(torch.clone)
+        assert torch.equal(y.detach(), want) and torch.equal(z, want)
+    torch.cuda.synchronize()

@@ -2,7 +2,8 @@
 
 Operators over CUDA tensors of rows, each one C-ABI call on torch's current
 stream (the stream of the Context that they are given stays as it was set).
-They are for inference: results carry no gradient. Several threads may call
+They are for inference: under grad mode, inputs that require gradients are
+refused. Several threads may call
 them with one Context and its handles, or without one; each call runs on its
 own thread's current stream.
   dense_linear_device      act(x @ w^T + bias) + residual   (linear, trellis2_mojo/modules/nn.mojo:27-266)
@@ -88,6 +89,11 @@ def _coords(t, device, rows):
     return t.data_ptr()
 
 
+def _no_gradients(*tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError("the operator has no gradient: call it under torch.no_grad(), or with detached tensors")
+
+
 def _context(ctx, t):
     if ctx is not None:
         return ctx
@@ -140,6 +146,7 @@ def dense_linear_device(x, weight, bias=None, activation=None, residual=None, ou
         if r != rows or w != co:
             raise ValueError("dense_linear: out must be [rows, co]")
     b = None if bias is None else _f32(bias, device, (co,), "dense_linear: bias")
+    _no_gradients(x, weight, bias, residual, out)
     if rows:
         with ctx._lock:
             handle = _on_torch_stream(ctx)
@@ -189,6 +196,7 @@ class RotaryPositionEmbedder:
             r, h, e, ldy = _heads3d(out, device, dtype, "RotaryPositionEmbedder: out")
             if (r, h, e) != (rows, heads, d):
                 raise ValueError("RotaryPositionEmbedder: out must have x's shape")
+        _no_gradients(x, out)
         if rows:
             with ctx._lock:
                 handle = _on_torch_stream(ctx)
@@ -240,6 +248,7 @@ def qk_norm_rope_device(q, k, gain_q, gain_k, coords=None, rope=None, eps=1e-6, 
     elif out_k is not None:
         raise ValueError("qk_norm_rope: out_k without k")
     at = _coords(coords, device, rows) if rope is not None else None
+    _no_gradients(q, k, gain_q, None if k is None else gain_k, out_q, out_k)
     if rows:
         with ctx._lock:
             handle = _on_torch_stream(ctx)
@@ -307,6 +316,7 @@ class SequenceLayout:
             r, h, e, ldo = _heads3d(out, device, dtype, "attention: out")
             if (r, h, e) != (rows, heads, d):
                 raise ValueError("attention: out must have q's shape")
+        _no_gradients(q, k, v, out)
         with ctx._lock:
             handle = _on_torch_stream(ctx)
             rc = _attention(self.handle, q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, out.data_ptr(), ldo, heads, d,
