@@ -193,3 +193,22 @@ def test_gradients_are_refused_not_dropped(t2sc):
             z = call(torch.clone)
         assert torch.equal(y.detach(), want) and torch.equal(z, want)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("rows", [3, 200])
+def test_f32_activations_to_f32_rounding(t2sc, act, rows):
+    """f32 activations of exact sums (one product, by one), over their whole range. The argument of the exponential, t, is off
+    by at most 6 roundings (gelu: two constants, three products, a sum), which change the result by at most |t| times as much,
+    relative. expf is off by 2 ulp (2^-22) and the sum and the division by a rounding each. An exponential above 2^128 is
+    infinite and the result zero, off by less than |x| 2^-128."""
+    import math
+    import torch
+    x = torch.cat([torch.linspace(-14, 14, 2001), torch.tensor([0.0, -0.0, 1e-30, -1e-30, 60.0, -30.0])]).cuda()
+    x = x.expand(rows, -1).contiguous().view(-1, 1)
+    y = t2sc.dense_linear_device(x, torch.ones(1, 1, device="cuda"), activation=act)
+    xd = x.double()
+    t = xd if act == "silu" else 2 * math.sqrt(2 / math.pi) * (xd + 0.044715 * xd ** 3)
+    want = xd / (1 + torch.exp(-t))
+    tol = (6 * t.abs() * 2.0 ** -24 * (act == "gelu") + 2.0 ** -22 + 3 * 2.0 ** -24) * want.abs() + 2.0 ** -128 * xd.abs() + 2.0 ** -126
+    ref.assert_close(y, want, tol)

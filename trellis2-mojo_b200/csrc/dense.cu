@@ -70,7 +70,7 @@ __global__ void __launch_bounds__(256) dense_simt_kernel(const DenseArgs a) {
       const int o = col0 + tc + j;
       if (r >= a.rows || o >= a.co) continue;
       float v = acc[i][j] + (a.bias ? __ldg(a.bias + o) : 0.f);
-      v = activate(v, a.act);
+      v = DT == T2SC_DT_F32 ? activate_f32(v, a.act) : activate(v, a.act);
       if (a.res) v += ld1<DT>(a.res, r * a.ldr + o);
       st1<DT>(a.y, r * a.ldy + o, v);
     }

@@ -23,7 +23,9 @@ struct DenseArgs {
 // v / (1 + e^-v) and 0.5 v (1 + tanh(u)) = v / (1 + e^(-2u)), u = sqrt(2/pi)
 // (v + 0.044715 v^3): one exponential, and no cancellation in the negative
 // tail. The exponential may become infinite: any finite v over it is 0, the
-// limit of both, however large v is.
+// limit of both, however large v is. In f32 for results of 16 bits, whose half
+// step of 2^-9 or 2^-12 the quick exponential and division (2^-17 together) stay
+// far below; f32 results take activate_f32.
 __device__ __forceinline__ float silu_any(float v) { return __fdividef(v, 1.0f + __expf(-v)); }
 __device__ __forceinline__ float gelu_tanh(float v) {
   const float u2 = v * (1.5957691216057308f + 0.07135481627f * v * v);
@@ -33,6 +35,12 @@ __device__ __forceinline__ float gelu_tanh(float v) {
 __device__ __forceinline__ float activate(float v, int act) {
   if (act & T2SC_SILU) return silu_any(v);
   if (act & T2SC_GELU) return gelu_tanh(v);
+  return v;
+}
+
+__device__ __forceinline__ float activate_f32(float v, int act) {
+  if (act & T2SC_SILU) return v / (1.0f + expf(-v));
+  if (act & T2SC_GELU) return v / (1.0f + expf(-v * (1.5957691216057308f + 0.07135481627f * v * v)));
   return v;
 }
 
