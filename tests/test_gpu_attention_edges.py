@@ -212,3 +212,30 @@ def test_f32_activations_to_f32_rounding(t2sc, act, rows):
     want = xd / (1 + torch.exp(-t))
     tol = (6 * t.abs() * 2.0 ** -24 * (act == "gelu") + 2.0 ** -22 + 3 * 2.0 ** -24) * want.abs() + 2.0 ** -128 * xd.abs() + 2.0 ** -126
     ref.assert_close(y, want, tol)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("q_len,n,d", [(1, 300, 64), (4, 300, 64), (130, 300, 64), (130, 3000, 64), (90, 1000, 128), (20000, 300, 104)])
+@pytest.mark.parametrize("scale", [1e4, 3e6, 2e7, 1e20, 1e36, -1e36, 3e38])
+def test_attention_scales_that_leave_the_largest_scores(t2sc, dtype, q_len, n, d, scale):
+    """Whole-numbered scores, exact in f32: with a large scale a row's weights are equal over its largest score (its smallest,
+    with a negative scale) and zero elsewhere; rows of zeros among them weigh all keys the same. The sums of up to n values of V
+    and of weights and the division are off by a rounding each; in 16 bits the weights, which share a factor 2^x with |x| < 1,
+    are rounded to the type before the product with V, off by u relative."""
+    import torch
+    g = _gen(q_len)
+    h = 2
+    dt = getattr(torch, dtype)
+    q = torch.randint(-2, 3, (q_len, h, d), generator=g, device="cuda").to(dt)
+    q[1::3] = 0
+    k = torch.randint(-3, 4, (n, h, d), generator=g, device="cuda").to(dt)
+    v = _normal(g, n, h, d, dtype=dtype)
+    y = t2sc.SequenceLayout([q_len], [n]).attention_device(q, k, v, scale=scale)
+    s = torch.einsum("qhd,khd->hqk", q.double(), k.double()) * (1 if scale > 0 else -1)
+    p = (s == s.amax(-1, keepdim=True)).double()
+    p = p / p.sum(-1, keepdim=True)
+    want = torch.einsum("hqk,khd->qhd", p, v.double())
+    size = torch.einsum("hqk,khd->qhd", p, v.double().abs())
+    u = ref.u(dt)
+    rel = (2 * n + 4) * ref.U32 + (u if dtype != "float32" else 0)
+    ref.assert_close(y, want, rel * size * (1 + u) + u * want.abs() + ref.tiny(dt))

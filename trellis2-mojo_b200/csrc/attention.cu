@@ -2,9 +2,12 @@
 //   out[i, h] = sum_j softmax_j(scale * q[i, h] . k[j, h]) v[j, h],
 // j over the keys of i's sequence; a sequence without keys gives zeros.
 //
-// One pass over the keys: with m the running maximum and l the running sum of
-// a row, a block of scores s updates m' = max(m, s), o = o e^(m - m') + sum
-// e^(s - m') v and l likewise; out = o / l. m, l and o are f32.
+// One pass over the keys: with m the running maximum of q . k and l the running
+// sum of a row, a block of products s updates m' = max(m, s), o = o e^(scale (m
+// - m')) + sum e^(scale (s - m')) v and l likewise; out = o / l. m, l and o are
+// f32. The difference is taken before the scale: near the maximum it is exact,
+// where the difference of two scaled products would keep their roundings, and
+// no finite scale makes it an infinity minus an infinity.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -66,8 +69,10 @@ __global__ void __launch_bounds__(kThreads) attention_simt_kernel(const AttnArgs
   const int64_t at = (int64_t)head * D;
   for (int i = tid; i < kBQ * D; i += kThreads) {
     const int r = i / D, c = i % D;
-    qs[r * pitch + c] = r < here ? ld1<DT>(a.q, (q0 + r) * a.ldq + at + c) * a.scale : 0.f;
+    // a negative scale's sign goes to the query, so that the largest product has the largest weight
+    qs[r * pitch + c] = r < here ? copysignf(1.f, a.scale) * ld1<DT>(a.q, (q0 + r) * a.ldq + at + c) : 0.f;
   }
+  const float scale = fabsf(a.scale);
   float m = -INFINITY, l = 0.f;
   constexpr int P = kMaxHeadDim / 4;
   float o[P];
@@ -97,11 +102,11 @@ __global__ void __launch_bounds__(kThreads) attention_simt_kernel(const AttnArgs
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
     const float base = top == -INFINITY ? 0.f : top;  // every score -inf so far: their weights are 0
-    const float keep = expf(m - base);
+    const float keep = m == -INFINITY ? 0.f : expf((m - base) * scale);
     float sum = 0.f;
 #pragma unroll
     for (int j = 0; j < kBKV / 4; j++) {
-      const float p = expf(s[j] - base);
+      const float p = j * 4 + part < keys ? expf((s[j] - base) * scale) : 0.f;
       ps[row * (kBKV + 1) + j * 4 + part] = p;
       sum += p;
     }

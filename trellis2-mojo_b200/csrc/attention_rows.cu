@@ -68,9 +68,9 @@ __device__ __forceinline__ void unpack8(const uint4 &u, float (&f)[8]) {
 
 // Weight of a partial sum with maximum m in one with maximum `to` (>= m):
 // partial sums without keys have m = -inf and l = 0.
-__device__ __forceinline__ float weight(float m, float to) { return m == to ? 1.f : ex2(m - to); }
+__device__ __forceinline__ float weight(float m, float to, float c) { return m == to ? 1.f : ex2((m - to) * c); }
 
-// Maxima are of scores times log2(e).
+// Maxima are of q . k; differences of them are scaled (attention.cu says why).
 template <int DT, int G, int R, int W>
 __global__ void __launch_bounds__(Shape<W>::kThreads, 16 / W) attention_rows_kernel(const __grid_constant__ RowsArgs x) {
   constexpr int kWarps = W, kThreads = Shape<W>::kThreads, kStageBytes = Shape<W>::kStageBytes;
@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(Shape<W>::kThreads, 16 / W) attention_rows_ker
           for (int c = 0; c < 8; c++) s[i][r] += q[r][c] * kf[c];
 #pragma unroll
           for (int d = G / 2; d > 0; d >>= 1) s[i][r] += __shfl_xor_sync(0xffffffffu, s[i][r], d);
-          s[i][r] = there ? s[i][r] * x.c : -INFINITY;
+          if (!there) s[i][r] = -INFINITY;
         }
       }
 #pragma unroll
@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(Shape<W>::kThreads, 16 / W) attention_rows_ker
         for (int i = 0; i < kSteps; i++) top = fmaxf(top, s[i][r]);
         const float from = top == -INFINITY ? 0.f : top;
         if (top > m[r]) {
-          const float keep = ex2(m[r] - top);
+          const float keep = ex2((m[r] - top) * x.c);
           m[r] = top;
           l[r] *= keep;
 #pragma unroll
@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(Shape<W>::kThreads, 16 / W) attention_rows_ker
         }
 #pragma unroll
         for (int i = 0; i < kSteps; i++) {
-          s[i][r] = ex2(s[i][r] - from);
+          s[i][r] = ex2((s[i][r] - from) * x.c);
           l[r] += s[i][r];
         }
       }
@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(Shape<W>::kThreads, 16 / W) attention_rows_ker
       float top = m[r];
 #pragma unroll
       for (int d = G; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-      const float w = weight(m[r], top);
+      const float w = weight(m[r], top, x.c);
       m[r] = top;
       l[r] *= w;
 #pragma unroll
@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(Shape<W>::kThreads, 16 / W) attention_rows_ker
     for (int w = 0; w < kWarps; w++) top = fmaxf(top, part.m[w][r]);
 #pragma unroll
     for (int w = 0; w < kWarps; w++) {
-      const float f = weight(part.m[w][r], top);
+      const float f = weight(part.m[w][r], top, x.c);
       sum += f * part.l[w][r], v += f * part.o[w][r][c];
     }
     part.cta_o[r][c] = v;
@@ -264,7 +264,7 @@ __global__ void __launch_bounds__(Shape<W>::kThreads, 16 / W) attention_rows_ker
     float top = -INFINITY, sum = 0.f, v = 0.f;
     for (int z = 0; z < x.splits; z++) top = fmaxf(top, ld_cluster(sm100::map_to_rank(m0 + 4 * r, z)));
     for (int z = 0; z < x.splits; z++) {
-      const float f = weight(ld_cluster(sm100::map_to_rank(m0 + 4 * r, z)), top);
+      const float f = weight(ld_cluster(sm100::map_to_rank(m0 + 4 * r, z)), top, x.c);
       sum += f * ld_cluster(sm100::map_to_rank(l0 + 4 * r, z));
       v += f * ld_cluster(sm100::map_to_rank(o0 + 4 * (r * G * 8 + c), z));
     }

@@ -26,7 +26,14 @@
 // maximum has grown by more than a factor 2^kSlack (then l and O are
 // rescaled by the row's thread): before that, weights are up to 2^kSlack and
 // the division by l at the end takes the factor out. In f16 the weights also
-// carry a factor 2^8, so that small ones stay clear of its subnormals.
+// carry a factor 2^8, so that small ones stay clear of its subnormals. One
+// multiply-add makes an exponent, s c - m c with m c rounded once for the row:
+// a factor that all its weights and l share. Above |m c| = 2^kFar that factor
+// approaches 2 (f16 overflows), then m c itself overflows; such rows, whose
+// scores f32 hardly tells apart, are computed once more at the end by their
+// threads, slowly, from differences (s - m) c. (Differences for every row, an
+// addition more, took 1203 + 738 tokens, 12 x 128, from 22.4 to 23.5 us and 23024
+// from 2470 to 2665; a second loop for such warps 24.4 and 2540.)
 //
 // Few query blocks: a cluster of up to 8 CTAs splits the keys of one block
 // and adds up its partial (m, l, O) through distributed shared memory, in
@@ -49,13 +56,14 @@
 namespace t2sc {
 namespace {
 
-constexpr int kBQ = 128, kBK = 128, kUnit = 64, kFew = 8, kMaxSplits = 8;
+constexpr int kBQ = 128, kBK = 128, kUnit = 64, kFew = 8, kMaxSplits = 8, kFar = 23;
 constexpr long long kWaitLimit = 4000000000ll;  // ~2 s of SM clocks
 
 struct TcArgs {
   CUtensorMap map_q, map_k, map_v;
+  const char *q, *k, *v;  // for the far rows alone
   char *out;
-  int64_t ldo;            // elements
+  int64_t ldq, ldk, ldv, ldo;  // elements
   const int4 *seqs;       // sequences, most keys first: first query row, query rows, first key row, key rows
   const int64_t *blocks;  // [batch + 1] query blocks (of NT * 128) before each sequence
   int batch, heads, head_dim, splits;
@@ -104,6 +112,65 @@ __device__ __forceinline__ float ld_cluster1(uint32_t addr) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr));
   return v;
+}
+
+// A row over `keys` keys from differences (s - m) c: its maximum and sum, and
+// its values, to `out` divided by the sum, or to row `row` of partial sums.
+template <int DT, int DP>
+__device__ __noinline__ void far_row(const char *q, const char *k, const char *v, int64_t ldk, int64_t ldv, int keys, int head_dim,
+                                     float c, float *row_m, float *row_l, char *out, float4 *part, int row) {
+  const int chunks = head_dim / 8;
+  auto load8 = [](const char *p, int chunk, float (&f)[8]) {
+    const uint4 u = *(reinterpret_cast<const uint4 *>(p) + chunk);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const float2 t = unpack2<DT>(w[j]);
+      f[2 * j] = t.x, f[2 * j + 1] = t.y;
+    }
+  };
+#pragma unroll 1
+  for (int c0 = 0; c0 < chunks; c0 += 4) {  // 32 channels at a time
+    float m = -INFINITY, l = 0.f, o[32], a[8], b[8];
+#pragma unroll
+    for (int z = 0; z < 32; z++) o[z] = 0.f;
+#pragma unroll 1
+    for (int64_t j = 0; j < keys; j++) {
+      float s = 0.f;
+#pragma unroll 1
+      for (int x = 0; x < chunks; x++) {
+        load8(q, x, a), load8(k + j * ldk * 2, x, b);
+#pragma unroll
+        for (int z = 0; z < 8; z++) s += a[z] * b[z];
+      }
+      if (s > m) {
+        const float f = m == -INFINITY ? 0.f : ex2((m - s) * c);
+        m = s, l *= f;
+#pragma unroll
+        for (int z = 0; z < 32; z++) o[z] *= f;
+      }
+      const float p = ex2((s - (m == -INFINITY ? 0.f : m)) * c);
+      l += p;
+#pragma unroll
+      for (int x = 0; x < 4; x++) {
+        if (c0 + x >= chunks) break;
+        load8(v + j * ldv * 2, c0 + x, b);
+#pragma unroll
+        for (int z = 0; z < 8; z++) o[x * 8 + z] += p * b[z];
+      }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int x = 0; x < 8; x++) {
+      const float *z = o + x * 4;
+      if (c0 * 2 + x >= chunks * 2) break;
+      if (out)
+        *(reinterpret_cast<uint2 *>(out) + c0 * 2 + x) = make_uint2(pack2<DT>(z[0] * inv, z[1] * inv), pack2<DT>(z[2] * inv, z[3] * inv));
+      else
+        part[row * (DP / 4) + ((c0 * 2 + x) ^ (row & (DP / 4 - 1)))] = make_float4(z[0], z[1], z[2], z[3]);
+    }
+    if (!out) *row_m = m, *row_l = l;
+  }
 }
 
 template <int DT, int DP, int NT>
@@ -430,6 +497,12 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
     }
     const bool have = n > 0 && ok;  // O holds sums
     const int row = quad * 32 + lane;
+    const bool far = have && live && i * kBQ + row < here && m != -INFINITY && !(fabsf(m * a.c) < (float)(1 << kFar));
+    auto redo = [&](char *out, float4 *part) {
+      const int64_t at = (int64_t)head * a.head_dim, key = (int64_t)kv0 + (int64_t)t0 * kBK;
+      far_row<DT, DP>(a.q + (((int64_t)q0 + i * kBQ + row) * a.ldq + at) * 2, a.k + (key * a.ldk + at) * 2, a.v + (key * a.ldv + at) * 2,
+                      a.ldk, a.ldv, keys, a.head_dim, a.c, row_m + row, row_l + row, out, part, row);
+    };
     if (a.splits == 1) {
       if (live && ok) {
         // the query block's shared memory is free now: 32 rows x 64 channels at a time through it
@@ -464,6 +537,7 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
           }
           __syncwarp();
         }
+        if (far) redo(a.out + ((row0 + lane) * a.ldo + (int64_t)head * a.head_dim) * 2, nullptr);
       }
     } else if (NT == 1) {
       // partial sums for the cluster: rows of f32 over the ring, 16-byte chunks swizzled by row
@@ -479,6 +553,7 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
           for (int c = 0; c < 8; c++)
             part[(c0 / 4 + c) ^ (row & (DP / 4 - 1))] = make_float4(v[c * 4], v[c * 4 + 1], v[c * 4 + 2], v[c * 4 + 3]);
         }
+        if (far) redo(nullptr, reinterpret_cast<float4 *>(ring));
       }
       __syncwarp();
       sm100::cluster_sync();
@@ -532,7 +607,8 @@ int launch(t2sc_seqs *s, const AttnArgs &a, int splits, std::string &err) {
   const bool keys = s->kv_off[s->batch] > s->kv_off[0];
   T2SC_TRY(encode(&t.map_k, keys ? a.k : a.q, keys ? a.ldk : a.ldq, keys ? s->kv_rows : 1));  // never read without keys
   T2SC_TRY(encode(&t.map_v, keys ? a.v : a.q, keys ? a.ldv : a.ldq, keys ? s->kv_rows : 1));
-  t.out = a.out, t.ldo = a.ldo;
+  t.q = a.q, t.k = a.k, t.v = a.v, t.out = a.out;
+  t.ldq = a.ldq, t.ldk = a.ldk, t.ldv = a.ldv, t.ldo = a.ldo;
   t.seqs = s->d_sorted;
   t.blocks = s->d_blocks + (NT == 2 ? 0 : s->batch + 1);
   t.batch = (int)s->batch, t.heads = a.heads, t.head_dim = a.head_dim, t.splits = splits;
