@@ -239,3 +239,18 @@ def test_attention_scales_that_leave_the_largest_scores(t2sc, dtype, q_len, n, d
     u = ref.u(dt)
     rel = (2 * n + 4) * ref.U32 + (u if dtype != "float32" else 0)
     ref.assert_close(y, want, rel * size * (1 + u) + u * want.abs() + ref.tiny(dt))
+
+
+@pytest.mark.parametrize("rows,co,pad", [(2000, 64, 0), (2000, 192, 0), (2000, 130, 0), (1500, 61, 3)])
+def test_linear_narrow_tiles_in_place(t2sc, rows, co, pad):
+    """Tiles of 64 columns, whose second epilogue warps have no columns of their own, with the residual in place."""
+    import torch
+    g = _gen(rows + co)
+    x, w, b = _normal(g, rows, 136, dtype="bfloat16"), _normal(g, co, 136, std=0.1, dtype="bfloat16"), _normal(g, co)
+    buf = torch.full((rows + 2, co + pad), float("nan"), device="cuda", dtype=x.dtype)
+    y = buf[:rows, :co]
+    y.copy_(_normal(g, rows, co, dtype="bfloat16"))
+    want = ref.linear(x, w, b, "gelu", y.clone())
+    t2sc.dense_linear_device(x, w, b, activation="gelu", residual=y, out=y)
+    assert torch.isnan(buf[rows:]).all() and torch.isnan(buf[:, co:]).all()
+    ref.assert_close(y, *want)

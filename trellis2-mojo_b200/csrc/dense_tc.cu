@@ -72,12 +72,6 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
   return __all_sync(0xffffffffu, ok);
 }
 
-template <int DT>
-__device__ __forceinline__ float ld16(const char *p) {
-  if (DT == T2SC_DT_BF16) return __bfloat162float(*reinterpret_cast<const __nv_bfloat16 *>(p));
-  return __half2float(*reinterpret_cast<const __half *>(p));
-}
-
 template <int DT, int CG, int BN>
 __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_constant__ DenseTcArgs a) {
   using S = Shape<CG, BN>;
@@ -264,8 +258,10 @@ __global__ void __launch_bounds__(kThreads, 1) dense_tc_kernel(const __grid_cons
       };
       // column c of row r in the staging block
       auto single = [&](int r, int c) { return reinterpret_cast<uint16_t *>(stage + r * 128 + ((c >> 3 ^ (r & 7)) << 4) + (c & 7) * 2); };
-      load_bias(n0 + half * 64);
-      if (a.res) load_residual(n0 + half * 64);
+      if (half * 64 < BN) {
+        load_bias(n0 + half * 64);
+        if (a.res) load_residual(n0 + half * 64);
+      }
       if (!warp_wait(tfull0 + 8 * b, (acc >> 1) & 1, abort, a.err)) break;
       sm100::tc_fence_after();
       const uint32_t taddr = tmem + b * BN + ((uint32_t)(quad * 32) << 16);
