@@ -254,3 +254,17 @@ def test_linear_narrow_tiles_in_place(t2sc, rows, co, pad):
     t2sc.dense_linear_device(x, w, b, activation="gelu", residual=y, out=y)
     assert torch.isnan(buf[rows:]).all() and torch.isnan(buf[:, co:]).all()
     ref.assert_close(y, *want)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("rows,ci,co", [(700, 4096, 9000), (130, 8192, 5003)])
+def test_linear_weights_of_several_bands(t2sc, dtype, rows, ci, co):
+    """Weights above 32 MB: column tiles in bands, the last one narrower, over several rows of tiles."""
+    import torch
+    g = _gen(rows)
+    x, w, b = _normal(g, rows, ci, dtype=dtype), _normal(g, co, ci, std=ci ** -0.5, dtype=dtype), _normal(g, co)
+    buf = torch.full((rows + 2, co + 3), float("nan"), device="cuda", dtype=x.dtype)
+    y = buf[:rows, :co]
+    t2sc.dense_linear_device(x, w, b, activation="silu", out=y)
+    assert torch.isnan(buf[rows:]).all() and torch.isnan(buf[:, co:]).all()
+    ref.assert_close(y, *ref.linear(x, w, b, "silu"))
