@@ -280,7 +280,9 @@ int t2sc_c2s_block_forward_device(t2sc_c2s_block *block, t2sc_coords *coords, co
  * elements, so q, k and v can be slices of one packed [N, 3, heads,
  * head_dim] projection. A stride of a buffer of more than one row is at
  * least the row's width and at most 2^28. All calls are asynchronous on the
- * context's stream and capturable in a CUDA graph. */
+ * context's stream and capturable in a CUDA graph. A bounded device wait that
+ * gave up is reported as T2SC_ERR_TIMEOUT by the next of these calls on the
+ * context, or by t2sc_ctx_synchronize. */
 
 /* y [rows, co] = act(x [rows, ci] @ w [co, ci]^T + bias) + residual, all of
  * dtype (bias: device f32 [co] or NULL), with sums, activation and residual

@@ -50,3 +50,20 @@ def test_non_coherent_loads_are_of_the_handles_own_tables(name):
     asked = [re.match(r"\s*(reinterpret_cast<[^>]*>\()?\s*([\w.]+)", text[m.end():]).group(2)
              for m in re.finditer(r"\b__ldg\(", text)]
     assert set(asked) <= {"a.seqs", "a.blocks", "a.turns"}, asked
+
+
+@pytest.mark.parametrize("name,entry", [("dense.cu", "t2sc_dense_linear_device"), ("rope.cu", "t2sc_rope_apply_device"),
+                                        ("rope.cu", "t2sc_qk_norm_rope_device"), ("attention.cu", "t2sc_attention_device")])
+def test_a_wait_that_gave_up_reaches_the_next_call(name, entry):
+    """The attention block's kernels follow torch's streams and need not be synchronised through their context: they note a wait
+    that gave up in host memory (the device self-test checks the way there), and each operator reports it before it launches."""
+    text = open(os.path.join(CSRC, name)).read()
+    body = text[text.index(f"int {entry}("):]
+    body = body[:body.index("\n}\n")]
+    assert body.index("T2SC_TRY(earlier_failure(ctx))") < body.index("DeviceGuard")
+
+
+@pytest.mark.parametrize("name", [f for f in SOURCES if f != "rope.cu" and f != "dense_rows.cu"])
+def test_bounded_waits_report_into_host_memory(name):
+    """(rope.cu and dense_rows.cu wait for nothing.)"""
+    assert "ctx->d_wait" in SOURCES[name] and "d_err" not in SOURCES[name]

@@ -77,10 +77,17 @@ int check_sync(t2sc_ctx *ctx) {
   if (flags & kDevErrTimeout)
     return fail(ctx, T2SC_ERR_TIMEOUT, "a bounded device wait timed out; results of the last call are invalid");
   if (flags) return fail(ctx, T2SC_ERR_INVALID, "device error flags set: " + std::to_string(flags));
-  return T2SC_OK;
+  return earlier_failure(ctx);
 }
 
 }  // namespace
+
+int t2sc::earlier_failure(t2sc_ctx *ctx) {
+  volatile int *flags = ctx->h_wait;
+  if (!*flags) return T2SC_OK;
+  *flags = 0;
+  return fail(ctx, T2SC_ERR_TIMEOUT, "a bounded device wait of an earlier call timed out; that call's results are invalid");
+}
 
 int t2sc::read_dev_err(t2sc_ctx *ctx, int *flags) {
   std::string &err = ctx->last_error;
@@ -120,6 +127,10 @@ int t2sc_ctx_create(int device, t2sc_ctx **out) {
     }
     ctx->stream = ctx->own_stream;
     if (cudaMalloc((void **)&ctx->d_err, sizeof(int)) != cudaSuccess) return T2SC_ERR_OOM;
+    if (cudaHostAlloc((void **)&ctx->h_wait, sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable) != cudaSuccess)
+      return T2SC_ERR_OOM;
+    *ctx->h_wait = 0;
+    if (cudaHostGetDevicePointer((void **)&ctx->d_wait, ctx->h_wait, 0) != cudaSuccess) return T2SC_ERR_CUDA;
     if (cudaMemsetAsync(ctx->d_err, 0, sizeof(int), ctx->own_stream) != cudaSuccess ||
         cudaStreamSynchronize(ctx->own_stream) != cudaSuccess)
       return T2SC_ERR_CUDA;
@@ -139,6 +150,7 @@ int t2sc_ctx_destroy(t2sc_ctx *ctx) {
     if (p) cudaFree(p);
   for (auto &kv : ctx->id_maps) free_map(kv.second);
   cudaFree(ctx->d_err);
+  cudaFreeHost(ctx->h_wait);
   if (ctx->own_stream) cudaStreamDestroy(ctx->own_stream);
   if (ctx->up_stream) cudaStreamDestroy(ctx->up_stream);
   if (ctx->down_stream) cudaStreamDestroy(ctx->down_stream);

@@ -267,6 +267,7 @@ int t2sc_attention_device(t2sc_seqs *seqs, const void *q, int64_t q_stride, cons
     a.out = static_cast<char *>(out);
     a.ldq = q_stride, a.ldk = k_stride, a.ldv = v_stride, a.ldo = out_stride;
     a.seqs = seqs->d_seqs, a.blocks32 = seqs->d_blocks + 2 * (seqs->batch + 1), a.batch = (int)seqs->batch, a.heads = heads, a.head_dim = head_dim, a.scale = scale;
+    T2SC_TRY(earlier_failure(ctx));
     DeviceGuard g(ctx->device);
     if (attention_rows_takes(seqs, a, dtype)) return attention_rows(seqs, a, dtype, ctx->last_error);
     return attention_tc_takes(seqs, a, dtype) ? attention_tc(seqs, a, dtype, ctx->last_error)

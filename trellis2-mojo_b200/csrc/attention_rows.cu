@@ -291,7 +291,7 @@ int launch(t2sc_seqs *s, const AttnArgs &a, std::string &err) {
   RowsArgs x;
   x.a = a;
   x.c = a.scale * 1.4426950408889634f;
-  x.err = ctx->d_err;
+  x.err = ctx->d_wait;
   constexpr int block = W * (32 / G) * 2;
   // The number of key splits that ends first: rounds of clusters x blocks of
   // the longest sequence a CTA takes (+ 2 of 32 KB for what it costs to begin

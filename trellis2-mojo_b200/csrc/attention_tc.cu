@@ -612,7 +612,7 @@ int launch(t2sc_seqs *s, const AttnArgs &a, int splits, std::string &err) {
   t.seqs = s->d_sorted;
   t.blocks = s->d_blocks + (NT == 2 ? 0 : s->batch + 1);
   t.batch = (int)s->batch, t.heads = a.heads, t.head_dim = a.head_dim, t.splits = splits;
-  t.c = a.scale * 1.4426950408889634f, t.err = ctx->d_err;
+  t.c = a.scale * 1.4426950408889634f, t.err = ctx->d_wait;
   const int64_t grid = (NT == 2 ? s->blocks256 : s->blocks128) * a.heads * splits;
   if (grid > INT32_MAX) return fail(ctx, T2SC_ERR_UNSUPPORTED, "attention: too many query blocks in one call");
   for (int b = 0; b <= kFew && b <= s->batch; b++) {

@@ -129,6 +129,7 @@ extern "C" int t2sc_dense_linear_device(t2sc_ctx *ctx, const void *x, int64_t x_
     a.ldx = x_stride, a.ldw = w_stride, a.ldr = residual_stride, a.ldy = y_stride;
     a.rows = rows, a.co = co, a.ci = ci;
     a.act = flags & (T2SC_SILU | T2SC_GELU);
+    T2SC_TRY(earlier_failure(ctx));
     DeviceGuard g(ctx->device);
     if (dense_rows_takes(a, dtype)) return dense_rows(ctx, a, dtype, ctx->last_error);
     if (dense_skinny_takes(ctx, a, dtype)) return dense_skinny(ctx, a, dtype, ctx->last_error);

@@ -260,7 +260,7 @@ int launch(t2sc_ctx *ctx, const DenseArgs &a, std::string &err) {
   auto on8 = [&](const void *p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 8 == 0 && (a.rows <= 1 || ld % 4 == 0); };
   t.vec = a.co % 4 == 0 && on8(a.y, a.ldy) && (!a.res || on8(a.res, a.ldr));
   t.row_tiles = ((int)a.rows + N - 1) / N;
-  t.k_iters = (a.ci + kBK - 1) / kBK, t.act = a.act, t.err = ctx->d_err;
+  t.k_iters = (a.ci + kBK - 1) / kBK, t.act = a.act, t.err = ctx->d_wait;
   const int64_t tiles = (int64_t)((a.co + kM - 1) / kM) * t.row_tiles;
   t.slices = slices_of(tiles, t.k_iters, ctx->num_sms);
   if (tiles * t.slices > INT32_MAX) return fail(ctx, T2SC_ERR_UNSUPPORTED, "dense_linear: too many outputs");

@@ -386,7 +386,7 @@ int launch(t2sc_ctx *ctx, const DenseArgs &a, std::string &err) {
   T2SC_TRY(tensormap_16bit(&t.map_x, DT, 2, a.x, dx, sx, bx, err));
   T2SC_TRY(tensormap_16bit(&t.map_w, DT, 2, a.w, dw, sw, bw, err));
   t.res = a.res, t.y = a.y, t.bias = a.bias, t.ldr = a.ldr, t.ldy = a.ldy, t.rows = a.rows, t.co = a.co;
-  t.k_iters = (a.ci + kBK - 1) / kBK, t.act = a.act, t.err = ctx->d_err;
+  t.k_iters = (a.ci + kBK - 1) / kBK, t.act = a.act, t.err = ctx->d_wait;
   t.m_tiles = (int)((a.rows + kTileM * CG - 1) / (kTileM * CG)), t.n_tiles = (a.co + BN - 1) / BN;
   auto on16 = [&](const void *p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (a.rows <= 1 || ld % 8 == 0); };
   t.vec = on16(a.y, a.ldy) && (!a.res || on16(a.res, a.ldr));

@@ -43,6 +43,10 @@ struct t2sc_ctx {
   std::map<cudaStream_t, cudaEvent_t> left;
   int64_t launches_waited = 0;  // launches up to the last switch or wait
   int *d_err = nullptr;      // device error flags (one int)
+  // Flags of the attention block's kernels, whose calls follow other streams
+  // and may never be synchronised through the context: a word of host memory
+  // that kernels write (d_wait) and the next call reads (h_wait).
+  int *h_wait = nullptr, *d_wait = nullptr;
   int64_t launches = 0;      // kernels launched by this context
   std::string last_error;
   // identity row maps of the linear layers, one per row count, shared by
@@ -171,6 +175,9 @@ int cascade_coords_device(t2sc_ctx *ctx, const int32_t *hr_coords, int64_t n, in
 
 // ---- error-flag helpers (api.cu) ----
 int read_dev_err(t2sc_ctx *ctx, int *flags);
+// T2SC_ERR_TIMEOUT, once, where a kernel of an earlier call has given up since;
+// waits for nothing.
+int earlier_failure(t2sc_ctx *ctx);
 
 inline int cuda_status(cudaError_t e, std::string &err, const char *what) {
   if (e == cudaSuccess) return T2SC_OK;

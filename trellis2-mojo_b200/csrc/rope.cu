@@ -448,6 +448,7 @@ int t2sc_rope_apply_device(t2sc_rope *rope, const int32_t *coords, const void *x
     T2SC_TRY(enter(ctx, a, 0, x, x_stride, y, y_stride, dtype, "rope", &ri, &ro));
     if (overlaps(ro, Rows{coords, 4, rows, 4, 4})) return fail(ctx, T2SC_ERR_INVALID, "rope: the output overlaps coords");
     enter_rope(a, rope, coords);
+    T2SC_TRY(earlier_failure(ctx));
     DeviceGuard g(ctx->device);
     return launch_any(ctx, a, false, rope->layout == T2SC_ROPE_PAIRS, dtype);
   });
@@ -491,6 +492,7 @@ int t2sc_qk_norm_rope_device(t2sc_ctx *ctx, t2sc_rope *rope, const int32_t *coor
       if (overlaps(qo, cr) || (k && overlaps(ko, cr))) return fail(ctx, T2SC_ERR_INVALID, "qk_norm_rope: an output overlaps coords");
       enter_rope(a, rope, coords);
     }
+    T2SC_TRY(earlier_failure(ctx));
     DeviceGuard g(ctx->device);
     return launch_any(ctx, a, true, !rope || rope->layout == T2SC_ROPE_PAIRS, dtype);
   });

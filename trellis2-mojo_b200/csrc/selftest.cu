@@ -2,7 +2,9 @@
 // trellis2_mojo/gpu/context.mojo:7-12, 139-158): a small compute check, and
 // a check of the bounded-wait path every conv pipeline relies on. The
 // second part waits on an mbarrier that nothing completes, with a short
-// limit, and must come back with the timeout flag set instead of hanging.
+// limit, and must come back with the timeout flag set instead of hanging: once
+// in device memory, once in the word that the next call of the attention
+// block's operators reads, which has to report it, once.
 #include "internal.h"
 #include "sm100.cuh"
 
@@ -41,6 +43,8 @@ extern "C" int t2sc_ctx_selftest(t2sc_ctx *ctx, int wait_us) {
   if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
   if (prev != ctx->device) cudaSetDevice(ctx->device);
   int rc = [&]() -> int {
+    const int before = earlier_failure(ctx);
+    if (before != T2SC_OK) return before;
     const int n = 256;
     float h_in[n], h_out[n];
     for (int i = 0; i < n; i++) h_in[i] = (float)i - 100.0f;
@@ -69,6 +73,16 @@ extern "C" int t2sc_ctx_selftest(t2sc_ctx *ctx, int wait_us) {
       if (r != T2SC_OK) break;
       if (!(h_flags & kDevErrTimeout) || (h_flags & kDevErrInternal)) {
         err = "selftest: the bounded wait did not report its timeout";
+        r = T2SC_ERR_CUDA;
+        break;
+      }
+      selftest_kernel<<<1, 64, 0, ctx->stream>>>(d, d + n, n, 2000LL * wait_us, ctx->d_wait);
+      ctx->launches++;
+      if ((r = cuda_status(cudaGetLastError(), err, "selftest launch")) != T2SC_OK) break;
+      if ((r = cuda_status(cudaStreamSynchronize(ctx->stream), err, "selftest")) != T2SC_OK) break;
+      const bool reported = earlier_failure(ctx) == T2SC_ERR_TIMEOUT, again = earlier_failure(ctx) != T2SC_OK;
+      if (!reported || again) {
+        err = "selftest: the timeout did not reach the next call, or reached two";
         r = T2SC_ERR_CUDA;
       }
     } while (0);

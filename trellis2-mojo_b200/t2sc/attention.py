@@ -5,7 +5,9 @@ stream (the stream of the Context that they are given stays as it was set).
 They are for inference: under grad mode, inputs that require gradients are
 refused. Several threads may call
 them with one Context and its handles, or without one; each call runs on its
-own thread's current stream.
+own thread's current stream. A kernel that gave up a bounded wait, so that its
+result is invalid, is reported by the next call with the Context, or by
+Context.synchronize.
   dense_linear_device      act(x @ w^T + bias) + residual   (linear, trellis2_mojo/modules/nn.mojo:27-266)
   RotaryPositionEmbedder   rotary positions over x, y, z    (trellis2_mojo/modules/rope.mojo)
   qk_norm_rope_device      per-head RMS norm + rotation     (bias_rms_rope_qkv, trellis2_mojo/gpu/attention.mojo:507)
