@@ -394,9 +394,14 @@ class SparseMultiHeadAttention:
         rows = x.shape[0]
         if rows != layout.q_rows:
             raise ValueError("SparseMultiHeadAttention: x must have the layout's rows")
+        if not self.cross and layout.kv_offsets is not layout.q_offsets and \
+                not np.array_equal(layout.kv_offsets, layout.q_offsets):
+            raise ValueError("SparseMultiHeadAttention: self-attention needs a layout whose keys are its queries")
         if self.cross:
             if context is None:
                 raise ValueError("SparseMultiHeadAttention: cross-attention needs a context")
+            if context.shape[0] != layout.kv_rows:
+                raise ValueError("SparseMultiHeadAttention: context must have the layout's key rows")
             q = dense_linear_device(x, *self._q, ctx=self.ctx).view(rows, h, d)
             kv = dense_linear_device(context, *self._kv, ctx=self.ctx).view(context.shape[0], 2, h, d)
             k, v = kv[:, 0], kv[:, 1]
