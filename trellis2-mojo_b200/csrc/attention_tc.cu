@@ -31,7 +31,7 @@
 // a factor that all its weights and l share. Above |m c| = 2^kFar that factor
 // approaches 2 (f16 overflows), then m c itself overflows; such rows, whose
 // scores f32 hardly tells apart, are computed once more at the end by their
-// threads, slowly, from differences (s - m) c. (Differences for every row, an
+// warp, row by row, from differences (s - m) c. (Differences for every row, an
 // addition more, took 1203 + 738 tokens, 12 x 128, from 22.4 to 23.5 us and 23024
 // from 2470 to 2665; a second loop for such warps 24.4 and 2540.)
 //
@@ -114,14 +114,22 @@ __device__ __forceinline__ float ld_cluster1(uint32_t addr) {
   return v;
 }
 
-// A row over `keys` keys from differences (s - m) c: its maximum and sum, and
-// its values, to `out` divided by the sum, or to row `row` of partial sums.
+// The rows of a warp in `rows` over `keys` keys from differences (s - m) c, one
+// after the other: 8 channels a lane, G lanes a key, as in attention_rows.cu. A
+// row's values go to `out`, divided by their sum, or with its maximum and sum to
+// the partial sums. q, out and the sums are those of the warp's first row,
+// `row0` of the block.
 template <int DT, int DP>
-__device__ __noinline__ void far_row(const char *q, const char *k, const char *v, int64_t ldk, int64_t ldv, int keys, int head_dim,
-                                     float c, float *row_m, float *row_l, char *out, float4 *part, int row) {
-  const int chunks = head_dim / 8;
-  auto load8 = [](const char *p, int chunk, float (&f)[8]) {
-    const uint4 u = *(reinterpret_cast<const uint4 *>(p) + chunk);
+__device__ __noinline__ void far_rows(uint32_t rows, const char *q, int64_t ldq, const char *k, int64_t ldk, const char *v, int64_t ldv,
+                                      int keys, int head_dim, float c, char *out, int64_t ldo, float4 *part, int row0, float *row_m,
+                                      float *row_l) {
+  constexpr int G = DP / 8, kKeys = 32 / G, kSteps = 4;
+  const int lane = threadIdx.x & 31, sub = lane % G, group = lane / G;
+  const bool in = sub * 8 < head_dim;
+  auto load8 = [&](const char *p, bool there) {
+    return there && in ? *(reinterpret_cast<const uint4 *>(p) + sub) : make_uint4(0, 0, 0, 0);
+  };
+  auto unpack8 = [](const uint4 &u, float (&f)[8]) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -130,46 +138,75 @@ __device__ __noinline__ void far_row(const char *q, const char *k, const char *v
     }
   };
 #pragma unroll 1
-  for (int c0 = 0; c0 < chunks; c0 += 4) {  // 32 channels at a time
-    float m = -INFINITY, l = 0.f, o[32], a[8], b[8];
+  for (; rows; rows &= rows - 1) {
+    const int r = __ffs(rows) - 1;
+    float m = -INFINITY, l = 0.f, o[8], a[8], b[8];
+    unpack8(load8(q + r * ldq * 2, true), a);
 #pragma unroll
-    for (int z = 0; z < 32; z++) o[z] = 0.f;
+    for (int z = 0; z < 8; z++) o[z] = 0.f;
 #pragma unroll 1
-    for (int64_t j = 0; j < keys; j++) {
-      float s = 0.f;
-#pragma unroll 1
-      for (int x = 0; x < chunks; x++) {
-        load8(q, x, a), load8(k + j * ldk * 2, x, b);
+    for (int64_t j0 = group; j0 - group < keys; j0 += kKeys * kSteps) {
+      uint4 kr[kSteps], vr[kSteps];
+      float s[kSteps], top = m;
 #pragma unroll
-        for (int z = 0; z < 8; z++) s += a[z] * b[z];
+      for (int i = 0; i < kSteps; i++) {
+        const int64_t j = j0 + i * kKeys;
+        kr[i] = load8(k + j * ldk * 2, j < keys), vr[i] = load8(v + j * ldv * 2, j < keys);
       }
-      if (s > m) {
-        const float f = m == -INFINITY ? 0.f : ex2((m - s) * c);
-        m = s, l *= f;
 #pragma unroll
-        for (int z = 0; z < 32; z++) o[z] *= f;
+      for (int i = 0; i < kSteps; i++) {
+        unpack8(kr[i], b);
+        s[i] = 0.f;
+#pragma unroll
+        for (int z = 0; z < 8; z++) s[i] += a[z] * b[z];
+#pragma unroll
+        for (int d = G / 2; d > 0; d >>= 1) s[i] += __shfl_xor_sync(0xffffffffu, s[i], d);
+        if (j0 + i * kKeys >= keys) s[i] = -INFINITY;
+        top = fmaxf(top, s[i]);
       }
-      const float p = ex2((s - (m == -INFINITY ? 0.f : m)) * c);
-      l += p;
+      const float from = top == -INFINITY ? 0.f : top;
+      if (top > m) {
+        const float f = ex2((m - top) * c);
+        m = top, l *= f;
 #pragma unroll
-      for (int x = 0; x < 4; x++) {
-        if (c0 + x >= chunks) break;
-        load8(v + j * ldv * 2, c0 + x, b);
+        for (int z = 0; z < 8; z++) o[z] *= f;
+      }
 #pragma unroll
-        for (int z = 0; z < 8; z++) o[x * 8 + z] += p * b[z];
+      for (int i = 0; i < kSteps; i++) {
+        const float p = ex2((s[i] - from) * c);
+        unpack8(vr[i], b);
+        l += p;
+#pragma unroll
+        for (int z = 0; z < 8; z++) o[z] += p * b[z];
       }
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    float top = m;
 #pragma unroll
-    for (int x = 0; x < 8; x++) {
-      const float *z = o + x * 4;
-      if (c0 * 2 + x >= chunks * 2) break;
-      if (out)
-        *(reinterpret_cast<uint2 *>(out) + c0 * 2 + x) = make_uint2(pack2<DT>(z[0] * inv, z[1] * inv), pack2<DT>(z[2] * inv, z[3] * inv));
-      else
-        part[row * (DP / 4) + ((c0 * 2 + x) ^ (row & (DP / 4 - 1)))] = make_float4(z[0], z[1], z[2], z[3]);
+    for (int d = G; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    const float f = m == top ? 1.f : ex2((m - top) * c);
+    l *= f;
+#pragma unroll
+    for (int d = G; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+#pragma unroll
+    for (int z = 0; z < 8; z++) {
+      o[z] *= f;
+#pragma unroll
+      for (int d = G; d < 32; d <<= 1) o[z] += __shfl_xor_sync(0xffffffffu, o[z], d);
     }
-    if (!out) *row_m = m, *row_l = l;
+    if (group == 0 && in) {
+      if (out) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+        for (int z = 0; z < 8; z++) o[z] *= inv;
+        *(reinterpret_cast<uint4 *>(out + r * ldo * 2) + sub) =
+            make_uint4(pack2<DT>(o[0], o[1]), pack2<DT>(o[2], o[3]), pack2<DT>(o[4], o[5]), pack2<DT>(o[6], o[7]));
+      } else {
+        const int row = row0 + r, swizzle = row & (DP / 4 - 1);
+        part[row * (DP / 4) + ((sub * 2) ^ swizzle)] = make_float4(o[0], o[1], o[2], o[3]);
+        part[row * (DP / 4) + ((sub * 2 + 1) ^ swizzle)] = make_float4(o[4], o[5], o[6], o[7]);
+      }
+    }
+    if (!out && lane == 0) row_m[r] = top, row_l[r] = l;
   }
 }
 
@@ -497,11 +534,12 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
     }
     const bool have = n > 0 && ok;  // O holds sums
     const int row = quad * 32 + lane;
-    const bool far = have && live && i * kBQ + row < here && m != -INFINITY && !(fabsf(m * a.c) < (float)(1 << kFar));
+    const uint32_t far = __ballot_sync(
+        0xffffffffu, have && live && i * kBQ + row < here && m != -INFINITY && !(fabsf(m * a.c) < (float)(1 << kFar)));
     auto redo = [&](char *out, float4 *part) {
-      const int64_t at = (int64_t)head * a.head_dim, key = (int64_t)kv0 + (int64_t)t0 * kBK;
-      far_row<DT, DP>(a.q + (((int64_t)q0 + i * kBQ + row) * a.ldq + at) * 2, a.k + (key * a.ldk + at) * 2, a.v + (key * a.ldv + at) * 2,
-                      a.ldk, a.ldv, keys, a.head_dim, a.c, row_m + row, row_l + row, out, part, row);
+      const int64_t at = (int64_t)head * a.head_dim, key = (int64_t)kv0 + (int64_t)t0 * kBK, first = (int64_t)q0 + i * kBQ + quad * 32;
+      far_rows<DT, DP>(far, a.q + (first * a.ldq + at) * 2, a.ldq, a.k + (key * a.ldk + at) * 2, a.ldk, a.v + (key * a.ldv + at) * 2, a.ldv,
+                       keys, a.head_dim, a.c, out, a.ldo, part, quad * 32, row_m + quad * 32, row_l + quad * 32);
     };
     if (a.splits == 1) {
       if (live && ok) {
@@ -537,7 +575,7 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
           }
           __syncwarp();
         }
-        if (far) redo(a.out + ((row0 + lane) * a.ldo + (int64_t)head * a.head_dim) * 2, nullptr);
+        if (far) redo(a.out + (row0 * a.ldo + (int64_t)head * a.head_dim) * 2, nullptr);
       }
     } else if (NT == 1) {
       // partial sums for the cluster: rows of f32 over the ring, 16-byte chunks swizzled by row
@@ -553,6 +591,7 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, NT == 2 ? 1 : 2) atte
           for (int c = 0; c < 8; c++)
             part[(c0 / 4 + c) ^ (row & (DP / 4 - 1))] = make_float4(v[c * 4], v[c * 4 + 1], v[c * 4 + 2], v[c * 4 + 3]);
         }
+        __syncwarp();
         if (far) redo(nullptr, reinterpret_cast<float4 *>(ring));
       }
       __syncwarp();
