@@ -28,6 +28,7 @@ from .sparse import _DTYPES, Context, SparseTensor
 _ACTIVATIONS = {None: 0, "silu": _lib.SILU, "gelu": _lib.GELU}
 _LAYOUTS = {"pairs": _lib.ROPE_PAIRS, "halves": _lib.ROPE_HALVES}
 _CODES = {torch.float32: _lib.DT_F32, torch.float16: _lib.DT_F16, torch.bfloat16: _lib.DT_BF16}
+_Tensor = torch.Tensor
 _linear, _rope_apply = lib.t2sc_dense_linear_device, lib.t2sc_rope_apply_device
 _qk_norm_rope, _attention = lib.t2sc_qk_norm_rope_device, lib.t2sc_attention_device
 
@@ -41,11 +42,12 @@ def _code(t, what):
 
 def _rows2d(t, device, dtype, what):
     """(rows, width, row stride) of a [rows, width] tensor whose rows are contiguous."""
-    if not isinstance(t, torch.Tensor) or t.get_device() != device:
+    if not isinstance(t, _Tensor) or t.get_device() != device:
         raise ValueError(f"{what} must be a CUDA tensor on cuda:{device}")
-    if t.dtype is not dtype or t.dim() != 2:
+    shape = t.shape
+    if t.dtype is not dtype or len(shape) != 2:
         raise ValueError(f"{what} must be [rows, width] of {dtype}")
-    rows, width = t.shape
+    rows, width = shape
     if t.is_contiguous():
         return rows, width, width
     stride, inner = t.stride()
@@ -56,11 +58,12 @@ def _rows2d(t, device, dtype, what):
 
 def _heads3d(t, device, dtype, what):
     """(rows, heads, head_dim, row stride) of a [rows, heads, head_dim] tensor whose rows are contiguous."""
-    if not isinstance(t, torch.Tensor) or t.get_device() != device:
+    if not isinstance(t, _Tensor) or t.get_device() != device:
         raise ValueError(f"{what} must be a CUDA tensor on cuda:{device}")
-    if t.dtype is not dtype or t.dim() != 3:
+    shape = t.shape
+    if t.dtype is not dtype or len(shape) != 3:
         raise ValueError(f"{what} must be [rows, heads, head_dim] of {dtype}")
-    rows, h, d = t.shape
+    rows, h, d = shape
     if t.is_contiguous():
         return rows, h, d, h * d
     stride, per_head, inner = t.stride()
@@ -78,43 +81,45 @@ def _row_stride(rows, width, stride, what):
 
 
 def _f32(t, device, shape, what):
-    if not isinstance(t, torch.Tensor) or t.get_device() != device or t.dtype is not torch.float32 or \
+    if not isinstance(t, _Tensor) or t.get_device() != device or t.dtype is not torch.float32 or \
             t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{what} must be contiguous float32 {list(shape)} on cuda:{device}")
     return t.data_ptr()
 
 
 def _coords(t, device, rows):
-    if not isinstance(t, torch.Tensor) or t.get_device() != device or t.dtype is not torch.int32 or \
+    if not isinstance(t, _Tensor) or t.get_device() != device or t.dtype is not torch.int32 or \
             t.shape != (rows, 4) or not t.is_contiguous():
         raise ValueError(f"coords must be contiguous int32 [rows, 4] on cuda:{device}")
     return t.data_ptr()
 
 
-def _no_gradients(*tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+def _no_gradient():
+    """Some tensor of the call requires gradients."""
+    if torch.is_grad_enabled():
         raise ValueError("the operator has no gradient: call it under torch.no_grad(), or with detached tensors")
 
 
 def _context(ctx, t):
     if ctx is not None:
         return ctx
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+    if not isinstance(t, _Tensor) or not t.is_cuda:
         raise ValueError("the operator takes CUDA tensors")
     return Context.default(t.get_device())
 
 
 def _on_torch_stream(ctx):
     """The library context to call with, its work on torch's current stream of the device. Under the context's lock,
-    which is held until the call is made and its error is read."""
+    which is held until the call is made and its error is read (acquired by name: `with` takes twice as long)."""
     stream = torch.cuda.current_stream(ctx.device).cuda_stream if _raw_stream is None else _raw_stream(ctx.device)
     stream = stream or 1    # handle 0 would name the context's own stream, 1 is cudaStreamLegacy
     beside = ctx._beside_torch or ctx.beside_torch()
-    if not beside.handle:
+    handle = beside.handle
+    if handle is None:
         raise ValueError("the Context is closed")
     if beside.stream != stream:
         beside.use(stream)
-    return beside.handle
+    return handle
 
 
 # the handle alone, without a Stream object around it (2 us less a call)
@@ -141,21 +146,27 @@ def dense_linear_device(x, weight, bias=None, activation=None, residual=None, ou
         if r != rows or w != co:
             raise ValueError("dense_linear: residual must be [rows, co]")
         res, flags = residual.data_ptr(), flags | _lib.RESIDUAL
-    if out is None:
+    given = out is not None
+    if not given:
         out, ldy = x.new_empty((rows, co)), co
     else:
         r, w, ldy = _rows2d(out, device, dtype, "dense_linear: out")
         if r != rows or w != co:
             raise ValueError("dense_linear: out must be [rows, co]")
     b = None if bias is None else _f32(bias, device, (co,), "dense_linear: bias")
-    _no_gradients(x, weight, bias, residual, out)
+    if x.requires_grad or weight.requires_grad or (given and out.requires_grad) or \
+            (bias is not None and bias.requires_grad) or (residual is not None and residual.requires_grad):
+        _no_gradient()
     if rows:
-        with ctx._lock:
+        ctx._lock.acquire()
+        try:
             handle = _on_torch_stream(ctx)
             rc = _linear(handle, x.data_ptr(), ldx, weight.data_ptr(), ldw, b, res, ldr, out.data_ptr(), ldy, rows, co, ci,
                          flags, code)
             if rc:
                 check(rc, handle)
+        finally:
+            ctx._lock.release()
     return out
 
 
@@ -192,19 +203,24 @@ class RotaryPositionEmbedder:
         if d != self.head_dim or heads < 1:
             raise ValueError("RotaryPositionEmbedder: x must be [rows, heads, head_dim]")
         at = _coords(coords, device, rows)
-        if out is None:
+        given = out is not None
+        if not given:
             out, ldy = x.new_empty((rows, heads, d)), heads * d
         else:
             r, h, e, ldy = _heads3d(out, device, dtype, "RotaryPositionEmbedder: out")
             if (r, h, e) != (rows, heads, d):
                 raise ValueError("RotaryPositionEmbedder: out must have x's shape")
-        _no_gradients(x, out)
+        if x.requires_grad or (given and out.requires_grad):
+            _no_gradient()
         if rows:
-            with ctx._lock:
+            ctx._lock.acquire()
+            try:
                 handle = _on_torch_stream(ctx)
                 rc = _rope_apply(self.handle, at, x.data_ptr(), ldx, out.data_ptr(), ldy, rows, heads, code)
                 if rc:
                     check(rc, handle)
+            finally:
+                ctx._lock.release()
         return out
 
     def __del__(self):
@@ -250,14 +266,19 @@ def qk_norm_rope_device(q, k, gain_q, gain_k, coords=None, rope=None, eps=1e-6, 
     elif out_k is not None:
         raise ValueError("qk_norm_rope: out_k without k")
     at = _coords(coords, device, rows) if rope is not None else None
-    _no_gradients(q, k, gain_q, None if k is None else gain_k, out_q, out_k)
+    if q.requires_grad or gain_q.requires_grad or out_q.requires_grad or \
+            (k is not None and (k.requires_grad or gain_k.requires_grad or out_k.requires_grad)):
+        _no_gradient()
     if rows:
-        with ctx._lock:
+        ctx._lock.acquire()
+        try:
             handle = _on_torch_stream(ctx)
             rc = _qk_norm_rope(handle, None if rope is None else rope.handle, at, q.data_ptr(), ldq, kp, ldk, gq, gk,
                                out_q.data_ptr(), ldqo, kop, ldko, rows, heads, d, eps, code)
             if rc:
                 check(rc, handle)
+        finally:
+            ctx._lock.release()
     return out_q, out_k
 
 
@@ -312,19 +333,24 @@ class SequenceLayout:
             raise ValueError("attention: k and v must be [rows, heads, head_dim] with q's heads and head_dim")
         if rows < self.q_rows or kv_rows < self.kv_rows:
             raise ValueError("attention: fewer rows than the layout has")
-        if out is None:
+        given = out is not None
+        if not given:
             out, ldo = q.new_empty((rows, heads, d)), heads * d
         else:
             r, h, e, ldo = _heads3d(out, device, dtype, "attention: out")
             if (r, h, e) != (rows, heads, d):
                 raise ValueError("attention: out must have q's shape")
-        _no_gradients(q, k, v, out)
-        with ctx._lock:
+        if q.requires_grad or k.requires_grad or v.requires_grad or (given and out.requires_grad):
+            _no_gradient()
+        ctx._lock.acquire()
+        try:
             handle = _on_torch_stream(ctx)
             rc = _attention(self.handle, q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, out.data_ptr(), ldo, heads, d,
                             d ** -0.5 if scale is None else scale, code)
             if rc:
                 check(rc, handle)
+        finally:
+            ctx._lock.release()
         return out
 
     def __del__(self):
