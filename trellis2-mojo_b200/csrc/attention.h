@@ -29,6 +29,13 @@ struct t2sc_seqs {
 
 namespace t2sc {
 
+// 2^x, relative error 2^-22; results below 2^-126 are zero.
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 struct AttnArgs {
   const char *q = nullptr, *k = nullptr, *v = nullptr;
   char *out = nullptr;

@@ -46,24 +46,10 @@ struct RowsArgs {
   int *err = nullptr;
 };
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ float ld_cluster(uint32_t addr) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr));
   return v;
-}
-template <int DT>
-__device__ __forceinline__ void unpack8(const uint4 &u, float (&f)[8]) {
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int j = 0; j < 4; j++) {
-    const float2 p = unpack2<DT>(w[j]);
-    f[2 * j] = p.x, f[2 * j + 1] = p.y;
-  }
 }
 
 // Weight of a partial sum with maximum m in one with maximum `to` (>= m):

@@ -96,12 +96,6 @@ __device__ __forceinline__ T uniform(T v) {
   return __shfl_sync(0xffffffffu, v, 0);
 }
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 __device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
@@ -129,19 +123,11 @@ __device__ __noinline__ void far_rows(uint32_t rows, const char *q, int64_t ldq,
   auto load8 = [&](const char *p, bool there) {
     return there && in ? *(reinterpret_cast<const uint4 *>(p) + sub) : make_uint4(0, 0, 0, 0);
   };
-  auto unpack8 = [](const uint4 &u, float (&f)[8]) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const float2 t = unpack2<DT>(w[j]);
-      f[2 * j] = t.x, f[2 * j + 1] = t.y;
-    }
-  };
 #pragma unroll 1
   for (; rows; rows &= rows - 1) {
     const int r = __ffs(rows) - 1;
     float m = -INFINITY, l = 0.f, o[8], a[8], b[8];
-    unpack8(load8(q + r * ldq * 2, true), a);
+    unpack8<DT>(load8(q + r * ldq * 2, true), a);
 #pragma unroll
     for (int z = 0; z < 8; z++) o[z] = 0.f;
 #pragma unroll 1
@@ -155,7 +141,7 @@ __device__ __noinline__ void far_rows(uint32_t rows, const char *q, int64_t ldq,
       }
 #pragma unroll
       for (int i = 0; i < kSteps; i++) {
-        unpack8(kr[i], b);
+        unpack8<DT>(kr[i], b);
         s[i] = 0.f;
 #pragma unroll
         for (int z = 0; z < 8; z++) s[i] += a[z] * b[z];
@@ -174,7 +160,7 @@ __device__ __noinline__ void far_rows(uint32_t rows, const char *q, int64_t ldq,
 #pragma unroll
       for (int i = 0; i < kSteps; i++) {
         const float p = ex2((s[i] - from) * c);
-        unpack8(vr[i], b);
+        unpack8<DT>(vr[i], b);
         l += p;
 #pragma unroll
         for (int z = 0; z < 8; z++) o[z] += p * b[z];

@@ -23,16 +23,6 @@ namespace {
 constexpr int kMaxRows = 2, kWarps = 8, kOut = 4;
 
 template <int DT>
-__device__ __forceinline__ void unpack8(const uint4 &u, float (&f)[8]) {
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int j = 0; j < 4; j++) {
-    const float2 p = unpack2<DT>(w[j]);
-    f[2 * j] = p.x, f[2 * j + 1] = p.y;
-  }
-}
-
-template <int DT>
 __device__ __forceinline__ float ld16(const char *p, int64_t i) {
   if (DT == T2SC_DT_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(p)[i]);
   return __half2float(reinterpret_cast<const __half *>(p)[i]);

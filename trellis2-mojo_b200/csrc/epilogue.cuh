@@ -32,6 +32,15 @@ __device__ __forceinline__ float2 unpack2(uint32_t v) {
     return __half22float2(h);
   }
 }
+template <int DT>
+__device__ __forceinline__ void unpack8(const uint4 &u, float (&f)[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const float2 p = unpack2<DT>(w[j]);
+    f[2 * j] = p.x, f[2 * j + 1] = p.y;
+  }
+}
 
 // v / (1 + exp(-v)); the exponent is clamped so the divisor stays in the
 // range where the fast division is accurate (SiLU(v) for v < -80 is below
