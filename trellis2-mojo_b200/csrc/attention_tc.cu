@@ -11,7 +11,11 @@
 //               MN-major), f32 O in TMEM
 // and a warpgroup per query block, one thread a row, turns S into P in
 // between: p = 2^(s c - m c), c = scale log2(e), m the running maximum, P
-// rounded to the 16-bit type and written over S.
+// rounded to the 16-bit type and written over S. The rounding is what the
+// tensor cores ask of an operand: half a step of the type, 2^-8 in bf16 and
+// 2^-11 in f16, beside the result's own rounding (0.0023 and 0.00029 off 64 bits
+// where weights in f32 would be 0.0017 and 0.00021 off). l sums the weights as
+// they were before it.
 //
 // A query block has two S buffers of 64 columns, so that the scores of the
 // next unit are there when the softmax of this one is done: O takes up to 128
@@ -661,11 +665,11 @@ int launch_dp(t2sc_seqs *s, const AttnArgs &a, std::string &err) {
   // the parts' exchange. The end is that of the longest sequences' rounds of
   // CTAs, or, where others follow them, of all CTAs' time spread over the SMs
   // and half a CTA, and not before the rounds that they would take with a unit
-  // each. 300 queries over 20000 keys, 12 x 128: 75 us with the 6
-  // parts this finds, 98 with 8 (two rounds), 99 with 4, 262 with two blocks a
-  // CTA; 20 x 300 tokens, 16 x 64: 39 us with one part, 47 with two blocks a
-  // CTA; 21888 queries over 1029 keys, 16 x 64: 180 us with one block, 189
-  // with two, 12 x 128 179 and 150.
+  // each. 300 queries over 20000 keys, 12 x 128: 71 us with the 6
+  // parts this finds, 97 with 8 (two rounds), 95 with 4, 247 with two blocks a
+  // CTA; 20 x 300 tokens, 16 x 64: 34 us with one part, 42 with two blocks a
+  // CTA; 21888 queries over 1029 keys, 16 x 64: 177 us with one block, 187
+  // with two, 12 x 128 163 and 147 (profiles/attention_block_models.txt).
   constexpr double kFixed = 8, kPair = 1.25, kShared = DP == 64 ? 1.25 : 1.6, kExchange = 3;
   const double units = (double)((s->max_kv + kUnit - 1) / kUnit), heads = a.heads, sms = s->ctx->num_sms;
   auto rounds = [&](int64_t blocks, int64_t slots) { return (blocks * a.heads + slots - 1) / slots; };

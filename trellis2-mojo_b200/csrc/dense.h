@@ -24,7 +24,7 @@ struct DenseArgs {
 // (v + 0.044715 v^3): one exponential, and no cancellation in the negative
 // tail. The exponential may become infinite: any finite v over it is 0, the
 // limit of both, however large v is. In f32 for results of 16 bits, whose half
-// step of 2^-9 or 2^-12 the quick exponential and division (2^-17 together) stay
+// step of 2^-8 or 2^-11 the quick exponential and division (2^-17 together) stay
 // far below; f32 results take activate_f32.
 __device__ __forceinline__ float silu_any(float v) { return __fdividef(v, 1.0f + __expf(-v)); }
 __device__ __forceinline__ float gelu_tanh(float v) {

@@ -288,11 +288,11 @@ int launch_dt(t2sc_ctx *ctx, const DenseArgs &a, std::string &err) {
 
 // Up to 64 rows. Above, tiles of 128 rows are full enough for the row-major
 // kernel, which is the faster one unless it has too few tiles for a long K
-// axis, which it does not split: [256, 1536] -> 6144 10.7 us there, 18.0
-// here; [256, 6144] -> 1536 24.6 there, 13.1 here. What a call takes here, in
+// axis, which it does not split: [256, 1536] -> 6144 10.1 us there, 18.1
+// here; [256, 6144] -> 1536 24.0 there, 12.8 here. What a call takes here, in
 // microseconds: 6, a K step 0.25 on an SM of its own and 0.5 on a shared one,
-// and 0.04 a row that a CTA finishes (measured as in the other model, within
-// 15 %).
+// and 0.04 a row that a CTA finishes (within 15 % where it is chosen,
+// profiles/attention_block_models.txt).
 bool dense_skinny_takes(t2sc_ctx *ctx, const DenseArgs &a, int dtype) {
   if (!dense_tc_takes(a, dtype) || a.rows > 65536) return false;
   if (a.rows <= 64) return true;

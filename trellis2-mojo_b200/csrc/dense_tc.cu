@@ -405,8 +405,9 @@ int launch(t2sc_ctx *ctx, const DenseArgs &a, std::string &err) {
 
 // The tile shapes: rounds of tiles x (a K step x K steps + the tile's own) + the
 // launch, the first tiles' way in and the last one's epilogue, in microseconds
-// as measured with weights out of L2 ([64..1000] rows, 1024..8192 -> 128..6144:
-// within 7 %). A step is bound by what an SM takes in, 55 of its 64 bytes a
+// as measured with weights out of L2 (128..4736 rows, 1024..8192 -> 512..6144:
+// within 8 %; few tiles over a long K axis, where the K-split kernel is the
+// faster one, up to 29 %: profiles/attention_block_models.txt). A step is bound by what an SM takes in, 55 of its 64 bytes a
 // clock from L2, but for the pair's 256 columns, where the products are close.
 struct Option {
   int cg, bn;
