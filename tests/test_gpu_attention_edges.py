@@ -268,3 +268,83 @@ def test_linear_weights_of_several_bands(t2sc, dtype, rows, ci, co):
     t2sc.dense_linear_device(x, w, b, activation="silu", out=y)
     assert torch.isnan(buf[rows:]).all() and torch.isnan(buf[:, co:]).all()
     ref.assert_close(y, *ref.linear(x, w, b, "silu"))
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("q_lens,kv_lens,d", [([100, 30], [5000, 700], 64), ([90, 60], [6000, 300], 128), ([150, 90], [200, 61], 72),
+                                              ([3000, 700], [3000, 700], 128), ([6000, 6100], [300, 0], 64)])
+def test_attention_of_large_inputs(t2sc, dtype, q_lens, kv_lens, d):
+    """Queries and keys of several thousands, at the usual scale: scores of 2^22 and more, exact in f32, with keys split and not,
+    one and two query blocks a CTA; rows that are small among them, in slices of a wider buffer, and another sequence's NaN behind
+    the keys. Weights are equal over the largest score; bounds as in the test above, and for the small rows the usual ones."""
+    import torch
+    g = _gen(d + len(q_lens))
+    h, dt, nan = 2, getattr(torch, dtype), float("nan")
+    nq, nk = sum(q_lens), sum(kv_lens)
+    buf = torch.full((max(nq, nk) + 5, 3, h, d), nan, device="cuda", dtype=dt)
+    q, k, v = (buf[:n, i] for i, n in enumerate((nq, nk, nk)))
+    q.copy_(torch.randint(-2, 3, q.shape, generator=g, device="cuda") * 4096)
+    k.copy_(torch.randint(-3, 4, k.shape, generator=g, device="cuda") * 2048)
+    small = torch.arange(nq, device="cuda") % 3 == 1
+    q[small] = 0
+    v.copy_(_normal(g, *v.shape))
+    layout = t2sc.SequenceLayout(q_lens, kv_lens)
+    y = layout.attention_device(q, k, v)
+    q0 = k0 = 0
+    u = ref.u(dt)
+    for a, b in zip(q_lens, kv_lens):
+        got = y[q0:q0 + a]
+        if b:
+            kd, vd = k[k0:k0 + b].double(), v[k0:k0 + b].double()
+            s = torch.einsum("qhd,khd->hqk", q[q0:q0 + a].double(), kd)
+            p = (s == s.amax(-1, keepdim=True)).double()
+            p = p / p.sum(-1, keepdim=True)
+            want, size = (torch.einsum("hqk,khd->qhd", p, t) for t in (vd, vd.abs()))
+            ref.assert_close(got, want, ((2 * b + 4) * ref.U32 + u) * size * (1 + u) + u * want.abs() + ref.tiny(dt))
+        else:
+            assert not got.any()
+        q0, k0 = q0 + a, k0 + b
+    # the second sequence's keys and values turn bad: the first one's results keep their bits
+    k[kv_lens[0]:] = nan
+    v[kv_lens[0]:] = float("inf")
+    assert torch.equal(layout.attention_device(q, k, v)[:q_lens[0]], y[:q_lens[0]])
+
+
+def test_two_graphs_at_once(t2sc):
+    """Two graphs of the same operators and handles, replayed on two streams at once, far rows among them: their results keep
+    their bits."""
+    import torch
+    g = _gen(6)
+    lens, h, d = [700, 90, 1], 4, 64
+    n, c = sum(lens), h * d
+    layout, rope = t2sc.SequenceLayout(lens), t2sc.RotaryPositionEmbedder(d)
+    gain = torch.ones(h, d, device="cuda")
+    coords = torch.randint(0, 64, (n, 4), generator=g, device="cuda", dtype=torch.int32)
+    graphs, inputs = [], []
+    for i in range(2):
+        x, w = _normal(g, n, c, dtype="bfloat16"), _normal(g, 3 * c, c, std=c ** -0.5, dtype="bfloat16")
+        inputs.append((x, w))   # a graph reads them where they are
+
+        def block():
+            qkv = t2sc.dense_linear_device(x, w).view(n, 3, h, d)
+            q, k = t2sc.qk_norm_rope_device(qkv[:, 0], qkv[:, 1], gain, gain, coords, rope)
+            a = layout.attention_device(q, k, qkv[:, 2])
+            b = layout.attention_device(q, k, qkv[:, 2], scale=1e9)
+            return a, b, t2sc.dense_linear_device(a.view(n, c), w[:c], activation="gelu", residual=x)
+
+        want = [t.clone() for t in block()]
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = block()
+        graphs.append((graph, torch.cuda.Stream(), got, want))
+    for rep in range(10):
+        for graph, stream, got, want in graphs:
+            with torch.cuda.stream(stream):
+                for t in got:
+                    t.zero_()
+                graph.replay()
+    torch.cuda.synchronize()
+    for graph, stream, got, want in graphs:
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    t2sc.Context.default(0).synchronize()
